@@ -163,6 +163,76 @@ TF_API tf_status tf_rmsnorm_quantize_rows(const void* x, const float* partials, 
 TF_API tf_status tf_silu_gate(const void* gate, const void* up, int64_t m, int64_t f, int64_t ldg, int64_t ldu, void* out, int64_t ldo,
                        void* stream);
 
+/* ---- attention over a paged key-value cache -------------------------------------------------------------------------------------
+ * What stands between the qkv GEMM and the output GEMM of a decoder layer. The reference has no counterpart: its graphs stop at the
+ * operators of README.md:53-85.
+ *
+ * A cache holds the keys and values of many sequences in pages of page_size entries. Entry e of a sequence is slot e % page_size of the
+ * page that the sequence's table names at e / page_size. An entry of one kv head is head_dim dense elements; pages, heads and slots have
+ * strides of their own, the same for k and v, so that any order of the three axes will do. Indexes are 64 bits wide. */
+enum { TF_CACHE_BF16 = 0, TF_CACHE_E4M3 = 1 };
+typedef struct {
+  void* k;              /* 16-byte aligned */
+  void* v;
+  const float* k_scale; /* TF_CACHE_E4M3: f32 [kv_heads] on the device, an entry's value is code * scale; NULL stands for 1. Else NULL */
+  const float* v_scale;
+  int64_t pages, page_size, kv_heads;
+  int64_t head_dim;     /* a multiple of 16, at most 256 */
+  int64_t stride_page, stride_head, stride_slot; /* elements; multiples of 16 bytes */
+  int32_t dtype;        /* TF_CACHE_* */
+  int32_t reserved;     /* 0 */
+} tf_paged_cache;
+
+/* How the pairs that a rotation turns lie in a head of which it turns the first rot elements: (i, i + rot / 2) or (2i, 2i + 1). */
+enum { TF_ROTARY_HALF = 0, TF_ROTARY_INTERLEAVED = 1 };
+enum { TF_BF16 = 0, TF_F32 = 1 };
+
+/* Rotary positions: pair i of every head of token t is turned by the angle positions[t] * f_i and multiplied by `magnitude`; with `inverse` by
+ * the negative angle, which is the gradient of the forward call. Elements from rot on are copied. f32 arithmetic, one rounding at the end.
+ *   x, out     [tokens, heads, head_dim] of `dtype` (TF_BF16, TF_F32); token and head strides in elements. out may be x itself (in place), but
+ *              must not overlap it in another way
+ *   positions  int32 or int64 [tokens] (position_bits); any value, negative ones turn back
+ *   turns      uint64 [rot / 2]: the fraction of a full turn that f_i makes per position, times 2^64. Products wrap modulo a turn, so a far
+ *              position loses nothing
+ *   rot        even, 2 <= rot <= head_dim <= 1024 */
+TF_API tf_status tf_rotary(const void* x, int32_t dtype, int64_t tokens, int64_t heads, int64_t head_dim, int64_t x_stride_token, int64_t x_stride_head,
+                           const void* positions, int32_t position_bits, const uint64_t* turns, int64_t rot, int32_t layout, float magnitude,
+                           int32_t inverse, void* out, int64_t out_stride_token, int64_t out_stride_head, void* stream);
+
+/* Writes the keys and values of new tokens into a paged cache, turning keys (and, on the way, queries) by their positions.
+ *   k, v       bf16 [tokens, kv_heads, head_dim], 16-byte aligned, strides in elements, multiples of 8
+ *   tables     int32 [table_rows, table_cols], row stride table_stride: the pages of each sequence
+ *   positions  int32 or int64 [tokens]: the entry that a token's key and value become, and the position of its rotation
+ *   rows       int32 [tokens]: the table row of each token's sequence; NULL: token t belongs to row t / (tokens / table_rows)
+ *   q, q_out   bf16 [tokens, q_heads, head_dim] or both NULL (q_heads 0); q_out may be q
+ *   turns      as in tf_rotary, or NULL (rot 0): nothing is turned
+ * An e4m3 entry is the code nearest to x * (1 / scale) (1 / scale rounded once), saturating at 448. k is turned in f32 and rounded once.
+ * A token whose position is negative or beyond the table, whose row is outside the table, or whose page is outside the cache is left out: nothing
+ * of it is written to the cache (its query is turned like any other). When two tokens name one entry, which of them stays is not specified. */
+TF_API tf_status tf_cache_append(const tf_paged_cache* cache, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
+                                 int64_t v_stride_token, int64_t v_stride_head, int64_t tokens, const int32_t* tables, int64_t table_rows,
+                                 int64_t table_cols, int64_t table_stride, const void* positions, int32_t position_bits, const int32_t* rows, const void* q,
+                                 int64_t q_heads, int64_t q_stride_token, int64_t q_stride_head, void* q_out, int64_t q_out_stride_token,
+                                 int64_t q_out_stride_head, const uint64_t* turns, int64_t rot, int32_t layout, float magnitude, void* stream);
+
+/* Attention of the last `queries` tokens of each sequence over its entries in a paged cache:
+ *   out[b, i, h] = sum_e w_e v_e,  w = softmax over the visible entries e of scale * q[b, i, h] . k_e of kv head h / (q_heads / kv_heads)
+ * Query i of sequence b, which has L = lengths[b] entries and n = counts[b] queries (counts NULL: all `queries`), sees the entries in
+ * [max(0, E - window), E) with E = L - n + 1 + i (window 0: from 0 on). Queries n and later are padding. Where a query sees nothing, out is 0
+ * and lse -inf. An entry whose page number is outside the cache is seen by nobody; lengths and counts are taken within [0, what the table can name]
+ * and [0, queries].
+ *   q, out     bf16 [seqs * queries, q_heads, head_dim], 16-byte aligned, strides in elements, multiples of 8; out must not overlap q
+ *   tables     int32 [seqs, table_cols], row stride table_stride
+ *   lse        f32 [seqs * queries, q_heads] dense or NULL: ln sum_e exp(scale * q . k_e)
+ *   workspace  tf_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, whose content does not matter
+ * Scores, softmax statistics and sums are f32. The order of the sums depends on all lengths of the call, not on timing. */
+TF_API int64_t tf_paged_attention_workspace_bytes(int64_t seqs, int64_t queries, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t cache_dtype,
+                                                  int64_t max_entries);
+TF_API tf_status tf_paged_attention(const tf_paged_cache* cache, const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t seqs, int64_t queries,
+                                    int64_t q_heads, const int32_t* tables, int64_t table_cols, int64_t table_stride, const int32_t* lengths,
+                                    const int32_t* counts, float scale, int64_t window, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                                    float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Block-scaled GEMM on tcgen05 tensor cores: out[M,N] = bf16( sum_k deq(a)[m,k] * deq(b)[n,k] ), f32 accumulate.
  * Replaces the pinned cublasLtMatmul of `@tilefish.library("gemm", acc=f32)` (python/src/tilefish/_library.py:9-16) for
  * BlockScaled operands, which the reference cannot run.

@@ -48,4 +48,8 @@ def __getattr__(name):  # the run-time half imports torch lazily
 
         rt = importlib.import_module(".runtime", __name__)
         return rt if name == "runtime" else getattr(rt, name)
+    if name in ("rotary", "cache_append", "paged_attention", "PagedCache", "RotaryTable", "rotary_frequencies"):
+        import importlib
+
+        return getattr(importlib.import_module(".attention", __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -25,10 +25,22 @@ TF_ERR_DEVICE_TIMEOUT = 6
 
 FMT_MXFP8, FMT_MXFP4, FMT_NVFP4 = 0, 1, 2
 SCALES_PLAIN, SCALES_SWIZZLED = 0, 1
+CACHE_BF16, CACHE_E4M3 = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+TYPE_BF16, TYPE_F32 = 0, 1
 EPI_NONE, EPI_SILU_GATE, EPI_RESIDUAL = 0, 1, 2
 
 _P = c_void_p
 _FP = ctypes.POINTER(c_float)
+
+
+
+class PagedCacheDescriptor(ctypes.Structure):
+    """``tf_paged_cache`` of the header."""
+
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("pages", c_int64), ("page_size", c_int64), ("kv_heads", c_int64), ("head_dim", c_int64),
+                ("stride_page", c_int64), ("stride_head", c_int64), ("stride_slot", c_int64), ("dtype", c_int32), ("reserved", c_int32)]
+
 
 # name -> (restype, argtypes); every symbol include/tilefish_b200.h declares
 SIGNATURES = {
@@ -49,6 +61,13 @@ SIGNATURES = {
     "tf_unswizzle_scales": (c_int32, [_P, c_int64, c_int64, _P, _P]),
     "tf_residual_add_rmsnorm": (c_int32, [_P, _P, _P, _P, c_int64, c_int64, c_float, c_int32, _P, _P, c_int32, _P, _P, _P]),
     "tf_silu_gate": (c_int32, [_P, _P, c_int64, c_int64, c_int64, c_int64, _P, c_int64, _P]),
+    "tf_rotary": (c_int32, [_P, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int32, _P, c_int64, c_int32, c_float, c_int32, _P, c_int64,
+                            c_int64, _P]),
+    "tf_cache_append": (c_int32, [_P, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int64, _P, c_int64, c_int64, c_int64, _P, c_int32, _P, _P, c_int64, c_int64,
+                                  c_int64, _P, c_int64, c_int64, _P, c_int64, c_int32, c_float, _P]),
+    "tf_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_int64]),
+    "tf_paged_attention": (c_int32, [_P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, c_float, c_int64, _P, c_int64, c_int64,
+                                     _P, _P, c_int64, _P]),
     "tf_gemm_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int32, c_int32]),
     "tf_gemm_splits": (c_int32, [c_int64, c_int64, c_int64, c_int32, c_int32]),
     "tf_gemm_launch_form": (c_int32, [c_int64, c_int64, c_int64, c_int32, c_int32, _P]),

@@ -1,0 +1,461 @@
+"""The attention half of a decoder layer: rotary positions, a paged key-value cache, and attention of new tokens over it.
+
+Three operators in the manner of ``kernels.py`` (torch tensors in, C ABI calls out, every precondition checked before anything is enqueued):
+
+* ``rotary``           turns [tokens, heads, head_dim] by their positions (or back: ``inverse``, which is also its gradient);
+* ``cache_append``     writes keys and values of new tokens into a ``PagedCache`` (bf16 or e4m3 entries), turning k and q on the way;
+* ``paged_attention``  attention of the last tokens of each sequence over the cache, split over its length.
+
+``attention_block`` puts them between the qkv and the output GEMM (residual_add_rmsnorm -> gemm -> cache_append -> paged_attention -> gemm), and
+``decoder_layer`` puts that in front of ``mlp.decoder_block``. The reference has no counterpart: its README's graphs stop at the MLP block
+(README.md:53-85).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from dataclasses import dataclass
+from fractions import Fraction
+from typing import Optional
+
+from . import _native as N
+from . import kernels as K
+from .kernels import _check, _dense, _pre, _stream, _torch
+
+LAYOUTS = {"half": N.ROTARY_HALF, "interleaved": N.ROTARY_INTERLEAVED}
+_PI = Fraction("3.14159265358979323846264338327950288419716939937510")
+
+
+def _here(device) -> None:
+    current = _torch()._C._cuda_getDevice()
+    if device.index != current:
+        _pre(False, f"the tensors are on {device}, the current device is cuda:{current}: make it current (with torch.cuda.device(...))", "device")
+
+
+def _stride(t, axis: int) -> int:
+    """An axis' stride, 0 for one that is never stepped along (its stride says nothing then)."""
+    return t.stride(axis) if t.shape[axis] > 1 else 0
+
+
+def _overlap(a, b) -> bool:
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride()))) * t.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+
+
+def _dense_inner(t, name: str, unit: int) -> None:
+    """The last axis dense, the others at any stride that is a multiple of ``unit`` elements."""
+    if t.stride(2) == 1 and _stride(t, 0) % unit == 0 and _stride(t, 1) % unit == 0:
+        return
+    _pre(t.shape[2] <= 1 or t.stride(2) == 1, f"{name}: the last axis must be dense (strides {tuple(t.stride())})", "contiguous", name)
+    _pre(_stride(t, 0) % unit == 0 and _stride(t, 1) % unit == 0, f"{name}: strides {tuple(t.stride())} must be multiples of {unit} elements", "alignment", name)
+
+
+def _result(t, name: str) -> None:
+    """An axis of a result has no stride 0: several elements would be one."""
+    _pre(all(s <= 1 or st > 0 for s, st in zip(t.shape, t.stride())), f"{name}: a broadcast view cannot be written", "alias", name)
+
+
+# ---- rotary positions ---------------------------------------------------------------------------------------------------------
+
+
+def _turns(frequencies):
+    """Frequencies (radians per position) as the fraction of a full turn per position, times 2^64, in two's complement."""
+    out = []
+    for f in frequencies:
+        turns = round(Fraction(f) / (2 * _PI) * 2**64) % 2**64
+        out.append(turns - 2**64 if turns >= 2**63 else turns)
+    return out
+
+
+class RotaryTable:
+    """What a rotation needs besides positions: one inverse frequency per pair, how pairs lie in a head, and what the result is multiplied by.
+
+    ``inv_freq``   radians per position, rot / 2 of them (a tensor or a sequence; taken in 64 bits, read on the host once, here)
+    ``layout``     "half": pairs (i, i + rot / 2); "interleaved": pairs (2i, 2i + 1)
+    ``magnitude``  factor of the turned elements (long-context scalings use it); elements from rot on are left alone
+    """
+
+    __slots__ = ("rot", "layout", "magnitude", "turns", "_layout")
+
+    def __init__(self, inv_freq, *, layout: str = "half", magnitude: float = 1.0, device=None) -> None:
+        torch = _torch()
+        _pre(layout in LAYOUTS, f"unknown layout {layout!r}: one of {sorted(LAYOUTS)}", "argument", "layout")
+        _pre(math.isfinite(magnitude), f"magnitude: {magnitude} is not finite", "argument", "magnitude")
+        if isinstance(inv_freq, torch.Tensor):
+            _pre(inv_freq.dim() == 1, f"inv_freq: expected rank 1, got {inv_freq.dim()}", "rank", "inv_freq")
+            if device is None and inv_freq.is_cuda:
+                device = inv_freq.device
+            inv_freq = inv_freq.double().tolist()
+        values = [float(f) for f in inv_freq]
+        _pre(1 <= len(values) <= 512, f"inv_freq: {len(values)} frequencies; 1 to 512 are possible", "shape", "inv_freq")
+        _pre(all(math.isfinite(f) for f in values), "inv_freq: not finite", "argument", "inv_freq")
+        self.rot, self.layout, self.magnitude, self._layout = 2 * len(values), layout, float(magnitude), LAYOUTS[layout]
+        self.turns = torch.tensor(_turns(values), dtype=torch.int64, device=device if device is not None else "cuda")
+
+    def __repr__(self) -> str:
+        return f"RotaryTable(rot={self.rot}, {self.layout}, magnitude={self.magnitude:g})"
+
+
+def rotary_frequencies(rot: int, *, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0, length: int = 0, low: float = 1.0,
+                       high: Optional[float] = None):
+    """(inverse frequencies, magnitude) for heads of which ``rot`` elements are turned: base^(-2i / rot), stretched for contexts ``factor`` times
+    as long as the ``length`` a model was trained on:
+
+    * "linear"  every frequency divided by ``factor``;
+    * "ntk"     the base raised so that the lowest frequency is divided by ``factor`` and the highest is kept;
+    * "bands"   frequencies that make fewer than ``low`` turns over ``length`` divided by ``factor``, those above ``high`` (4) kept, blended between
+                by their number of turns;
+    * "yarn"    the same kept and divided ends (``high`` 32), blended by index (Peng et al., "YaRN", 2023), with magnitude 0.1 ln(factor) + 1.
+    """
+    _pre(rot >= 2 and rot % 2 == 0, f"rot={rot} must be even and at least 2", "divisible", "rot")
+    _pre(base > 0 and factor >= 1, f"base={base} must be positive and factor={factor} at least 1", "argument", "factor")
+    _pre(scaling in (None, "linear", "ntk", "bands", "yarn"), f"unknown scaling {scaling!r}", "argument", "scaling")
+    half = rot // 2
+    if scaling == "ntk" and rot > 2:
+        base = base * factor ** (rot / (rot - 2))
+    inv = [base ** (-2.0 * i / rot) for i in range(half)]
+    if scaling == "linear" or (scaling == "ntk" and rot == 2):
+        return [f / factor for f in inv], 1.0
+    if scaling in (None, "ntk"):
+        return inv, 1.0
+    high = (4.0 if scaling == "bands" else 32.0) if high is None else high
+    _pre(length > 0 and 0 < low < high, f"scaling {scaling!r} needs length > 0 and 0 < low < high (length={length}, low={low}, high={high})", "argument", "length")
+    if scaling == "bands":
+        keep = [min(1.0, max(0.0, (length * f / (2 * math.pi) - low) / (high - low))) for f in inv]
+        return [f * (k + (1 - k) / factor) for f, k in zip(inv, keep)], 1.0
+
+    def index_of(turns: float) -> float:  # the index whose frequency makes so many turns over `length`
+        return rot * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    first, last = max(0, math.floor(index_of(high))), min(half - 1, math.ceil(index_of(low)))
+    keep = [1 - min(1.0, max(0.0, (i - first) / max(last - first, 1e-3))) for i in range(half)]
+    return [f * (k + (1 - k) / factor) for f, k in zip(inv, keep)], 0.1 * math.log(factor) + 1.0
+
+
+def _check_positions(positions, tokens: int, device) -> int:
+    torch = _torch()
+    wide = isinstance(positions, torch.Tensor) and positions.dtype == torch.int64
+    _check(positions, "positions", torch.int64 if wide else torch.int32, 1, device, align=8 if wide else 4)
+    if positions.shape[0] != tokens:
+        _pre(False, f"positions: {positions.shape[0]} of them for {tokens} tokens", "shape", "positions")
+    _dense(positions, "positions")
+    return 64 if wide else 32
+
+
+def _check_table(table, dim: int, device) -> None:
+    _pre(isinstance(table, RotaryTable), f"expected a RotaryTable, got {type(table).__name__}", "dtype", "table")
+    if table.turns.device != device:
+        _pre(False, f"the table is on {table.turns.device}, the other arguments are on {device}", "device", "table")
+    if table.rot > dim:
+        _pre(False, f"the table turns {table.rot} elements of a head of {dim}", "shape", "table")
+
+
+def rotary(x, positions, table: RotaryTable, *, out=None, inverse: bool = False, stream=None):
+    """``x`` (bf16 or f32 [tokens, heads, head_dim], dense heads at any strides) with each token's heads turned by its position; f32 arithmetic, one rounding.
+    ``inverse`` turns back by the same angle: the transposed map, so the gradient of ``rotary`` is ``rotary(grad, ..., inverse=True)``. ``out=x`` works in place.
+    Positions are int32 or int64 of any size: an angle is exact to 2^-65 turns times the position."""
+    torch = _torch()
+    f32 = isinstance(x, torch.Tensor) and x.dtype == torch.float32
+    dtype = torch.float32 if f32 else torch.bfloat16
+    item = 4 if f32 else 2
+    _check(x, "x", dtype, 3, align=item)
+    device = x.device
+    _here(device)
+    tokens, heads, dim = x.shape
+    _check_table(table, dim, device)
+    bits = _check_positions(positions, tokens, device)
+    _dense_inner(x, "x", 1)
+    _pre(dim <= 1024, f"x: head_dim {dim} is more than 1024", "unsupported", "x")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+    else:
+        _check(out, "out", dtype, 3, device, align=item)
+        _pre(tuple(out.shape) == (tokens, heads, dim), f"out: shape {tuple(out.shape)}, expected {(tokens, heads, dim)}", "shape", "out")
+        _dense_inner(out, "out", 1)
+        _result(out, "out")
+        same = out.data_ptr() == x.data_ptr() and all(_stride(out, i) == _stride(x, i) for i in range(2))
+        _pre(same or not _overlap(out, x), "out overlaps x without being x", "alias", "out")
+    if tokens == 0 or heads == 0:
+        return out
+    N.check(N.load().tf_rotary(x.data_ptr(), N.TYPE_F32 if f32 else N.TYPE_BF16, tokens, heads, dim, _stride(x, 0), _stride(x, 1), positions.data_ptr(), bits,
+                               table.turns.data_ptr(), table.rot, table._layout, table.magnitude, 1 if inverse else 0, out.data_ptr(), _stride(out, 0),
+                               _stride(out, 1), _stream(stream)), "tf_rotary")
+    return out
+
+
+# ---- the paged cache ------------------------------------------------------------------------------------------------------------
+
+
+class PagedCache:
+    """Keys and values of many sequences in pages.
+
+    ``k``, ``v``  [pages, kv_heads, page_size, head_dim], bf16, or uint8 holding e4m3 codes; the last axis dense, the others at any strides (the same for
+                  both), so ``empty(...)``'s order and views of [pages, page_size, kv_heads, head_dim] tensors are both fine
+    ``k_scale``, ``v_scale``  float32 [kv_heads] for e4m3 (an entry's value is code * scale; None: 1)
+
+    Which pages belong to which sequence stands in the int32 [sequences, width] tables that the operators take, not here.
+    """
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "_desc", "_ref")
+
+    def __init__(self, k, v, k_scale=None, v_scale=None) -> None:
+        torch = _torch()
+        codes = isinstance(k, torch.Tensor) and k.dtype == torch.uint8
+        dtype, unit = (torch.uint8, 16) if codes else (torch.bfloat16, 8)
+        _check(k, "k", dtype, 4)
+        _check(v, "v", dtype, 4, k.device)
+        _pre(k.shape == v.shape, f"v: shape {tuple(v.shape)}, expected {tuple(k.shape)}", "shape", "v")
+        _pre(min(k.shape) > 0, f"k: shape {tuple(k.shape)} has an empty axis", "shape", "k")
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        _pre(self.head_dim % 16 == 0 and self.head_dim <= 256, f"k: head_dim {self.head_dim} is not a multiple of 16 up to 256", "divisible", "k")
+        _pre(k.stride(3) == 1 and v.stride(3) == 1, "k, v: the last axis must be dense", "contiguous", "k")
+        strides = [_stride(k, i) for i in range(3)]
+        _pre(strides == [_stride(v, i) for i in range(3)], f"v: strides {tuple(v.stride())}, expected those of k, {tuple(k.stride())}", "contiguous", "v")
+        _pre(all(s % unit == 0 for s in strides), f"k: strides {tuple(k.stride())} must be multiples of {unit} elements", "alignment", "k")
+        axes = sorted((st, n) for st, n in zip(strides, k.shape[:3]) if n > 1)
+        reach = self.head_dim
+        for st, n in axes:
+            _pre(st >= reach, f"k: strides {tuple(k.stride())}: entries overlap", "alias", "k")
+            reach = st * (n - 1) + reach
+        _pre(k.data_ptr() != v.data_ptr(), "k and v are the same memory", "alias", "v")
+        for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if s is not None:
+                _pre(codes, f"{name}: a bf16 cache has no scales", "argument", name)
+                _check(s, name, torch.float32, 1, k.device, align=4)
+                _dense(s, name)
+                _pre(s.shape[0] == self.kv_heads, f"{name}: {s.shape[0]} of them for {self.kv_heads} heads", "shape", name)
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self._desc = N.PagedCacheDescriptor(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+                                            v_scale.data_ptr() if v_scale is not None else None, self.pages, self.page_size, self.kv_heads, self.head_dim,
+                                            strides[0], strides[1], strides[2], N.CACHE_E4M3 if codes else N.CACHE_BF16, 0)
+        self._ref = ctypes.addressof(self._desc)
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "bf16", *, k_scale=None, v_scale=None, device="cuda") -> "PagedCache":
+        """A cache of its own memory, ``dtype`` "bf16" or "e4m3"; entries that were not written hold anything."""
+        torch = _torch()
+        _pre(dtype in ("bf16", "e4m3"), f"unknown cache dtype {dtype!r}", "dtype", "dtype")
+        k, v = (torch.empty((pages, kv_heads, page_size, head_dim), dtype=torch.bfloat16 if dtype == "bf16" else torch.uint8, device=device) for _ in range(2))
+        return cls(k, v, k_scale, v_scale)
+
+    @property
+    def dtype(self) -> str:
+        return "bf16" if self._desc.dtype == N.CACHE_BF16 else "e4m3"
+
+    def __repr__(self) -> str:
+        return f"PagedCache({self.dtype}, pages={self.pages}, page_size={self.page_size}, kv_heads={self.kv_heads}, head_dim={self.head_dim})"
+
+
+def _check_tables(tables, device) -> None:
+    _check(tables, "tables", _torch().int32, 2, device, align=4)
+    _pre(tables.shape[1] > 0 and (tables.stride(1) == 1 or tables.shape[1] == 1), f"tables: rows must be dense and not empty (shape {tuple(tables.shape)})", "contiguous",
+         "tables")
+
+
+def _check_int32(t, name: str, n: int, device) -> None:
+    _check(t, name, _torch().int32, 1, device, align=4)
+    _dense(t, name)
+    if t.shape[0] != n:
+        _pre(False, f"{name}: {t.shape[0]} of them, expected {n}", "shape", name)
+
+
+def _check_heads(t, name: str, tokens: Optional[int], heads: Optional[int], dim: int, device) -> None:
+    _check(t, name, _torch().bfloat16, 3, device)
+    if (tokens is not None and t.shape[0] != tokens) or (heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
+        _pre(False, f"{name}: shape {tuple(t.shape)}, expected [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, {dim}]", "shape", name)
+    _dense_inner(t, name, 8)
+
+
+def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=None, rotary: Optional[RotaryTable] = None, q_out=None, stream=None):
+    """Writes the keys and values (bf16 [tokens, kv_heads, head_dim]) of new tokens into the cache, in one launch with the rotation of k and q.
+
+    Token t becomes entry ``positions[t]`` (int32 or int64) of the sequence whose pages stand in row ``rows[t]`` of ``tables`` (int32 [sequences, width]);
+    without ``rows`` the tokens belong to the sequences in turn, tokens / sequences each. With ``rotary`` k and q (bf16 [tokens, q_heads, head_dim]) are
+    turned by ``positions``; returns the turned q (``q_out``, which may be q itself, or a new tensor), or None without q.
+
+    A token with a negative position (padding), one beyond its table, a row outside the tables or a page outside the cache is not written. Two tokens
+    for one entry: which of them stays is not specified."""
+    torch = _torch()
+    _pre(isinstance(cache, PagedCache), f"cache: expected a PagedCache, got {type(cache).__name__}", "dtype", "cache")
+    device, dim = cache.device, cache.head_dim
+    _here(device)
+    _check_heads(k, "k", None, cache.kv_heads, dim, device)
+    tokens = k.shape[0]
+    _check_heads(v, "v", tokens, cache.kv_heads, dim, device)
+    _check_tables(tables, device)
+    bits = _check_positions(positions, tokens, device)
+    if rows is not None:
+        _check_int32(rows, "rows", tokens, device)
+    else:
+        _pre(tokens == 0 or (tables.shape[0] > 0 and tokens % tables.shape[0] == 0),
+             f"k: {tokens} tokens cannot be dealt out evenly to {tables.shape[0]} sequences; give rows", "divisible", "k")
+    if rotary is not None:
+        _check_table(rotary, dim, device)
+    q_heads, qp, qs, qop, qos = 0, None, (0, 0), None, (0, 0)
+    if q is not None:
+        _check_heads(q, "q", tokens, None, dim, device)
+        q_heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((tokens, q_heads, dim), dtype=torch.bfloat16, device=device)
+        else:
+            _check_heads(q_out, "q_out", tokens, q_heads, dim, device)
+            _result(q_out, "q_out")
+            same = q_out.data_ptr() == q.data_ptr() and all(_stride(q_out, i) == _stride(q, i) for i in range(2))
+            _pre(same or not _overlap(q_out, q), "q_out overlaps q without being q", "alias", "q_out")
+        if q_heads:
+            qp, qs, qop, qos = q.data_ptr(), (_stride(q, 0), _stride(q, 1)), q_out.data_ptr(), (_stride(q_out, 0), _stride(q_out, 1))
+    else:
+        _pre(q_out is None, "q_out without q", "argument", "q_out")
+    if tokens == 0 or tables.shape[0] == 0:
+        _pre(tokens == 0, "tables: no sequences", "shape", "tables")
+        return q_out
+    N.check(N.load().tf_cache_append(cache._ref, k.data_ptr(), _stride(k, 0), _stride(k, 1), v.data_ptr(), _stride(v, 0), _stride(v, 1), tokens, tables.data_ptr(),
+                                     tables.shape[0], tables.shape[1], _stride(tables, 0), positions.data_ptr(), bits, rows.data_ptr() if rows is not None else None,
+                                     qp, q_heads, qs[0], qs[1], qop, qos[0], qos[1], rotary.turns.data_ptr() if rotary is not None else None,
+                                     rotary.rot if rotary is not None else 0, rotary._layout if rotary is not None else 0,
+                                     rotary.magnitude if rotary is not None else 1.0, _stream(stream)), "tf_cache_append")
+    return q_out
+
+
+# ---- attention over the cache ---------------------------------------------------------------------------------------------------
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device: int, seqs: int, queries: int, q_heads: int, kv_heads: int, dim: int, dtype: int, entries: int) -> int:
+    return int(N.load().tf_paged_attention_workspace_bytes(seqs, queries, q_heads, kv_heads, dim, dtype, entries))
+
+
+def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale: Optional[float] = None, window: int = 0, out=None, return_lse: bool = False,
+                    lse=None, workspace=None, stream=None):
+    """Attention of the last tokens of each sequence over its entries in the cache; bf16 [tokens, q_heads, head_dim].
+
+    ``q``        bf16 [sequences * queries, q_heads, head_dim]; q_heads a multiple of the cache's kv_heads (which share their queries' heads evenly)
+    ``tables``   int32 [sequences, width]: the pages of each sequence; those behind its length are not looked at
+    ``lengths``  int32 [sequences]: entries of each sequence, the new tokens' among them (``cache_append`` comes first)
+    ``counts``   int32 [sequences]: how many of a sequence's queries are real (None: all); the others are padding at its end
+
+    The last real query of a sequence sees all its entries, the one before all but the last, and so on; ``window`` > 0 bounds it to that many of the newest.
+    ``scale`` is 1 / sqrt(head_dim) unless given. With ``return_lse`` (or ``lse``, float32 [tokens, q_heads]) returns (out, lse), lse = ln of the sum of
+    exp(scale * q . k). A query that sees nothing (padding, an empty sequence) gets 0 and -inf. Entries on pages outside the cache are seen by nobody, and
+    what is not seen does not matter, infinities and NaN included."""
+    torch = _torch()
+    _pre(isinstance(cache, PagedCache), f"cache: expected a PagedCache, got {type(cache).__name__}", "dtype", "cache")
+    device, dim = cache.device, cache.head_dim
+    _here(device)
+    _check_heads(q, "q", None, None, dim, device)
+    _check_tables(tables, device)
+    tokens, heads = q.shape[0], q.shape[1]
+    seqs, width = tables.shape
+    _check_int32(lengths, "lengths", seqs, device)
+    if counts is not None:
+        _check_int32(counts, "counts", seqs, device)
+    if heads == 0 or heads % cache.kv_heads:
+        _pre(False, f"q: {heads} heads are not a multiple of the cache's {cache.kv_heads}", "divisible", "q")
+    if tokens and (seqs == 0 or tokens % seqs):
+        _pre(False, f"q: {tokens} tokens cannot be dealt out evenly to {seqs} sequences", "divisible", "q")
+    if scale is None:
+        scale = dim**-0.5
+    elif not math.isfinite(scale):
+        _pre(False, f"scale: {scale} is not finite", "argument", "scale")
+    if window < 0:
+        _pre(False, f"window: {window} is negative", "argument", "window")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=torch.bfloat16, device=device)
+    else:
+        _check_heads(out, "out", tokens, heads, dim, device)
+        _result(out, "out")
+        _pre(not _overlap(out, q), "out overlaps q", "alias", "out")
+    if lse is not None:
+        _check(lse, "lse", torch.float32, 2, device, align=4)
+        _pre(tuple(lse.shape) == (tokens, heads), f"lse: shape {tuple(lse.shape)}, expected {(tokens, heads)}", "shape", "lse")
+        _dense(lse, "lse")
+        return_lse = True
+    elif return_lse:
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
+    if tokens:
+        queries = tokens // seqs
+        need = _workspace_bytes(device.index, seqs, queries, heads, cache.kv_heads, dim, cache._desc.dtype, width * cache.page_size)
+        if need < 0:
+            _pre(False, f"q: {seqs} sequences of {queries} queries are more than this operator takes", "unsupported", "q")
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        else:
+            _check(workspace, "workspace", torch.uint8, 1, device)
+            _dense(workspace, "workspace")
+            _pre(workspace.numel() >= need, f"workspace: {need} bytes needed", "workspace", "workspace")
+        N.check(N.load().tf_paged_attention(cache._ref, q.data_ptr(), _stride(q, 0), _stride(q, 1), seqs, queries, heads, tables.data_ptr(), width,
+                                            _stride(tables, 0), lengths.data_ptr(), counts.data_ptr() if counts is not None else None, scale, window, out.data_ptr(),
+                                            _stride(out, 0), _stride(out, 1), lse.data_ptr() if lse is not None else None,
+                                            workspace.data_ptr() if workspace is not None else None, workspace.numel() if workspace is not None else 0,
+                                            _stream(stream)), "tf_paged_attention")
+    return (out, lse) if return_lse else out
+
+
+def attention_workspace_bytes(cache: PagedCache, sequences: int, queries: int, q_heads: int, width: int) -> int:
+    """Bytes of the ``workspace`` that ``paged_attention`` takes for tables of ``width`` pages (for callers that keep one; it must not serve two calls at once)."""
+    return _workspace_bytes(cache.device.index, sequences, queries, q_heads, cache.kv_heads, cache.head_dim, cache._desc.dtype, width * cache.page_size)
+
+
+# ---- the block ------------------------------------------------------------------------------------------------------------------
+
+
+@dataclass
+class AttentionWeights:
+    """One layer's attention weights on one device. ``w_qkv``: [(q_heads + 2 kv_heads) * head_dim, H] (query, key, value rows); ``w_o``: [H, q_heads * head_dim]."""
+
+    w_n: "object"  # bf16 [H]
+    w_qkv: K.BlockScaledTensor
+    w_o: K.BlockScaledTensor
+    q_heads: int
+    kv_heads: int
+
+    @property
+    def fmt(self) -> str:
+        return self.w_qkv.fmt
+
+
+def quantize_attention_weights(w_n, w_qkv, w_o, fmt: str, *, q_heads: int, kv_heads: int) -> AttentionWeights:
+    """Quantizes bf16 ``w_qkv`` [(q_heads + 2 kv_heads) * head_dim, H] and ``w_o`` [H, q_heads * head_dim]."""
+    rows, h = w_qkv.shape
+    _pre(q_heads > 0 and kv_heads > 0 and q_heads % kv_heads == 0, f"q_heads={q_heads} is not a multiple of kv_heads={kv_heads}", "divisible", "q_heads")
+    _pre(rows % (q_heads + 2 * kv_heads) == 0, f"w_qkv: {rows} rows are not {q_heads} + 2 * {kv_heads} heads", "shape", "w_qkv")
+    dim = rows // (q_heads + 2 * kv_heads)
+    _pre(tuple(w_o.shape) == (h, q_heads * dim), f"w_o: shape {tuple(w_o.shape)}, expected {(h, q_heads * dim)}", "shape", "w_o")
+    return AttentionWeights(w_n, K.quantize(w_qkv, fmt), K.quantize(w_o, fmt), q_heads, kv_heads)
+
+
+def attention_block(x, residual, w: AttentionWeights, cache: PagedCache, tables, positions, lengths, rotary: Optional[RotaryTable] = None, *, rows=None, counts=None,
+                    window: int = 0, eps: float = 1e-6):
+    """One attention block: ``residual += x`` (f32, in place), returns bf16 [tokens, H] = attention(rmsnorm(residual) * w_n) @ w_o^T, the keys and values of the
+    tokens written into the cache on the way. ``positions``, ``tables``, ``rows`` as in ``cache_append``, ``lengths`` (after these tokens) and ``counts`` as in
+    ``paged_attention``; the tokens of a sequence stand together, as many for each."""
+    torch = _torch()
+    fmt = w.fmt
+    dim = cache.head_dim
+    _pre(w.w_qkv.shape[0] == (w.q_heads + 2 * w.kv_heads) * dim and w.kv_heads == cache.kv_heads,
+         f"the weights' heads ({w.q_heads} + 2 * {w.kv_heads}, {w.w_qkv.shape[0]} rows) do not match the cache's ({cache.kv_heads} of {dim})", "shape", "cache")
+    if fmt == "nvfp4":
+        amax = torch.zeros(1, dtype=torch.float32, device=x.device)
+        h = K.residual_add_rmsnorm(x, residual, w.w_n, eps, amax_out=amax)
+        hq = K.quantize(h, fmt, amax=amax)
+    else:
+        _, hq = K.residual_add_rmsnorm(x, residual, w.w_n, eps, quantize_to=fmt, want_bf16=False)
+    qkv = K.gemm_blockscaled(hq, w.w_qkv).view(x.shape[0], -1, dim)
+    q, k, v = qkv.split([w.q_heads, w.kv_heads, w.kv_heads], dim=1)
+    cache_append(cache, k, v, tables, positions, rows=rows, q=q, rotary=rotary, q_out=q)
+    o = paged_attention(q, cache, tables, lengths, counts=counts, window=window)
+    return K.gemm(o.view(x.shape[0], -1), w.w_o)
+
+
+def decoder_layer(x, residual, attention: AttentionWeights, mlp, cache: PagedCache, tables, positions, lengths, rotary: Optional[RotaryTable] = None, *, rows=None,
+                  counts=None, window: int = 0, eps: float = 1e-6):
+    """A whole decoder layer: ``attention_block``, then ``mlp.decoder_block`` on its result (``mlp``: ``MlpWeights``). The result is the next layer's ``x``."""
+    from .mlp import decoder_block
+
+    y = attention_block(x, residual, attention, cache, tables, positions, lengths, rotary, rows=rows, counts=counts, window=window, eps=eps)
+    return decoder_block(y, residual, mlp, eps)
