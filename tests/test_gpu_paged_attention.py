@@ -67,7 +67,10 @@ def setup(A, lengths, queries, kv, group, dim, page, dtype, order="heads first",
 
 def run(A, q, cache, tables, lengths, **kwargs):
     counts = kwargs.pop("counts", None)
-    out, lse = A.paged_attention(q.cuda(), cache, tables.cuda(), lengths.cuda(), counts=counts.cuda() if counts is not None else None, return_lse=True, **kwargs)
+    need = A.attention_workspace_bytes(cache, len(lengths), q.shape[0] // len(lengths), q.shape[1], tables.shape[1])
+    workspace = torch.full((max(16, need),), 0xFF, dtype=torch.uint8, device="cuda")  # NaN: what the call did not write shows
+    out, lse = A.paged_attention(q.cuda(), cache, tables.cuda(), lengths.cuda(), counts=counts.cuda() if counts is not None else None, return_lse=True,
+                                 workspace=workspace, **kwargs)
     R.check_attention(out, lse, R.attention(q, cache.k, cache.v, tables, lengths, counts, kwargs.get("scale"), kwargs.get("window", 0), cache.k_scale, cache.v_scale))
     return out, lse
 

@@ -1,0 +1,712 @@
+// Attention of new tokens over a paged key-value cache, split over its length and joined.
+//
+// The rows of one kv head (its query heads times the new tokens) read the same keys, so they are the 16-row operand of mma.sync m16n8k16 and
+// keys stream through once. Bound by HBM: a bf16 key and value of 128 elements are 512 bytes for 4 * 128 operations per row, 24 bytes a clock
+// and SM, while 16 rows use about a tenth of the tensor cores and of the issue slots.
+//
+// One pass with a running maximum and sum (base 2, f32). Each warp (or team of 2 or 4 warps with 16 rows each, where there are more than 16
+// rows) has a ring of its own in shared memory, filled by cp.async: a tile's wait is a warp's wait, never the block's. The four warps of a block are
+// joined through shared memory at the end of a segment.
+//
+// The work is the list of all (sequence, row tile, kv head, unit of keys), cut into as many equal contiguous ranges as there are blocks, whatever
+// the lengths are (they are read on the device, so a captured call follows them). A block writes the result of a head whose keys it has seen
+// all of; of others it leaves its maximum, sum and unnormalised sum of values in the workspace, and paged_attention_join_kernel adds them up in the order of the keys.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include <cmath>
+
+#include "paged_cache.h"
+
+namespace tf {
+
+// floor(n / d) for 0 <= n < 2^31 by a multiplication: with 2^l >= d, m = ceil(2^(31 + l) / d) exceeds the quotient by less than 2^l / d parts.
+struct Divisor {
+  uint32_t mul, shift;
+  int d;
+};
+static Divisor divisor(int d) {
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  return {(uint32_t)(((1ull << (31 + l)) + d - 1) / d), (uint32_t)(31 + l), d};
+}
+
+struct AttendArgs {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t stride_page, stride_head, stride_slot;  // bytes
+  int pages, kv_heads, d;
+  Divisor page;
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  float* lse;
+  int64_t q_ldt, q_ldh, out_ldt, out_ldh;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const int32_t* counts;
+  int entries;  // what a table can name
+  int spans;    // sequences x row tiles
+  int queries, q_heads, row_tiles, window;
+  Divisor group;
+  float scale_log2;
+  float* part_sums;   // [slots][rows][d]
+  float2* part_stats; // [slots][rows]: maximum, sum
+};
+
+constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
+constexpr int kMaxAttendBlocks = 1024;
+
+template <int DP, bool F8, int TEAM>
+struct AttendCfg {
+  static constexpr int kTeams = kAttendWarps / TEAM, kRows = 16 * TEAM;
+  static constexpr int kRowBytes = DP * (F8 ? 1 : 2);
+  static constexpr int kKeys = kRowBytes >= (TEAM == 1 ? 256 : 512) ? 16 : 32;  // of a team's tile
+  static constexpr int kLoadRows = kKeys / TEAM;                                // of them, a warp loads
+  static constexpr int kUnit = kKeys * kTeams;
+  static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
+  static constexpr int kFit = 65536 / (kTeams * 2 * kHalf);
+  static constexpr int kStages = kFit < 2 ? 2 : kFit > 4 ? 4 : kFit;
+  static constexpr int kRing = kTeams * kStages * 2 * kHalf;
+  static constexpr int kPitch = DP + 8;  // floats of a row that is joined: rows start in other banks
+  static constexpr int kJoin = kTeams * kRows * kPitch * 4;
+  static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kBlocksPerSm = DP <= 128 ? 3 : F8 ? 2 : 1;
+  // an e4m3 entry is multiplied as f16: weights are scaled by 2^15 (the largest is 2^15), so that small ones keep their bits
+  static constexpr float kShift = F8 ? 15.0f : 0.0f;
+};
+
+__device__ __forceinline__ int divide(int n, Divisor v) { return (int)(((uint64_t)(uint32_t)n * v.mul) >> v.shift); }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 16 bytes global -> shared without registers; zeros where `bytes` is 0 (the address is then not read).
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_matrices_turned(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// two e4m3 codes (the lower or upper half of a word) -> two f16, exactly
+__device__ __forceinline__ uint32_t codes_to_f16x2(uint32_t w, bool upper) {
+  uint32_t r;
+  if (upper)
+    asm("{ .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, hi; }" : "=r"(r) : "r"(w));
+  else
+    asm("{ .reg .b16 lo, hi;\n mov.b32 {lo, hi}, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo; }" : "=r"(r) : "r"(w));
+  return r;
+}
+template <int TEAM>
+__device__ __forceinline__ void team_sync(int team) {
+  if constexpr (TEAM == 1)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TEAM) : "memory");
+}
+
+// What the rows of one row tile of one sequence see: keys [lo, hi) between them. The first row's limit is `first`, the last real row's hi.
+struct Span {
+  int start, hi, units;  // start: lo rounded down to a whole unit
+  int first, last_lo;    // every row sees [last_lo, first)
+  int length, count;
+};
+
+template <int ROWS, int UNIT>
+__device__ __forceinline__ Span span_of(const AttendArgs& p, int index) {
+  const int b = p.row_tiles == 1 ? index : index / p.row_tiles, tile = p.row_tiles == 1 ? 0 : index - b * p.row_tiles;
+  Span s;
+  const int len = p.lengths[b], cnt = p.counts ? p.counts[b] : p.queries;
+  s.length = len < 0 ? 0 : len > p.entries ? p.entries : len;
+  s.count = cnt < 0 ? 0 : cnt > p.queries ? p.queries : cnt;
+  const int r0 = tile * ROWS;
+  int r1 = p.queries * p.group.d - 1;
+  if (r1 > r0 + ROWS - 1) r1 = r0 + ROWS - 1;
+  const int i0 = divide(r0, p.group);
+  int i1 = divide(r1, p.group);
+  if (i1 > s.count - 1) i1 = s.count - 1;
+  s.start = s.hi = s.units = s.first = s.last_lo = 0;
+  if (i0 > i1) return s;
+  const int base = s.length - s.count + 1;
+  s.first = base + i0;
+  s.hi = base + i1;
+  if (s.hi <= 0) {
+    s.hi = 0;
+    return s;
+  }
+  int lo = 0;
+  if (p.window > 0) {
+    lo = s.first > p.window ? s.first - p.window : 0;
+    s.last_lo = s.hi > p.window ? s.hi - p.window : 0;
+  }
+  s.start = lo / UNIT * UNIT;
+  s.units = (s.hi - s.start + UNIT - 1) / UNIT;
+  return s;
+}
+
+// Sums over a block of 128 threads. `scratch` holds one value per warp; the caller does not touch it without a barrier.
+__device__ __forceinline__ long long block_sum(long long x, long long* scratch) {
+  for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(~0u, x, i);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
+  __syncthreads();
+  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+}
+
+template <int DP, bool F8, int TEAM>
+__global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlocksPerSm)) paged_attention_kernel(const AttendArgs p) {
+  using C = AttendCfg<DP, F8, TEAM>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_scratch[kAttendWarps], s_before;
+  __shared__ int s_index;
+  __shared__ uint32_t s_seen[kAttendWarps / TEAM][C::kStages][TEAM];
+  __shared__ float2 s_stats[C::kTeams * C::kRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / TEAM, member = warp % TEAM;
+
+  // this block's range of the list
+  long long mine = 0;
+  int first_units = 0;
+  for (int i = threadIdx.x; i < p.spans; i += kAttendThreads) {
+    const int u = span_of<C::kRows, C::kUnit>(p, i).units;
+    if (i < kAttendThreads) first_units = u;
+    mine += u;
+  }
+  const long long total = block_sum(mine, s_scratch) * p.kv_heads;
+  const long long blocks = total < gridDim.x ? total : gridDim.x;  // none of them without a unit: the join relies on it
+  if (blockIdx.x >= blocks) return;
+  const long long u0 = total * blockIdx.x / blocks, u1 = total * (blockIdx.x + 1) / blocks;
+  long long run = 0;  // units of the spans before this chunk
+  for (int at = 0;; at += kAttendThreads) {
+    const int i = at + threadIdx.x;
+    const int u = at == 0 ? first_units : i < p.spans ? span_of<C::kRows, C::kUnit>(p, i).units : 0;
+    long long upto = u;
+    for (int x = 1; x < 32; x <<= 1) {
+      const long long y = __shfl_up_sync(~0u, upto, x);
+      if (lane >= x) upto += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_scratch[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += s_scratch[w];
+    upto += run;
+    if ((upto - u) * p.kv_heads <= u0 && u0 < upto * p.kv_heads) {
+      s_index = i;
+      s_before = (upto - u) * p.kv_heads;
+    }
+    run += s_scratch[0] + s_scratch[1] + s_scratch[2] + s_scratch[3];
+    if (u0 < run * p.kv_heads) break;
+  }
+  __syncthreads();
+
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + team * C::kStages * 2 * C::kHalf;
+  constexpr int kChunks = C::kRowBytes / 16;      // of a staged row
+  constexpr int kRowsPerCopy = 32 / kChunks;      // rows that one copy instruction of a warp covers
+  const int chunks = p.d * (F8 ? 1 : 2) / 16;     // that hold data
+  const int copy_row = lane / kChunks, copy_chunk = lane % kChunks;
+  // chunk c of row r lies at c ^ swizzle(r): the eight rows of a matrix load are in other banks
+  auto swizzle = [](int row) { return C::kRowBytes >= 128 ? row & 7 : (row >> 1) & 3; };
+
+  int index = s_index;
+  long long before = s_before;
+  for (long long u = u0; u < u1;) {
+    const Span sp = span_of<C::kRows, C::kUnit>(p, index);
+    if (sp.units == 0) {
+      ++index;
+      continue;
+    }
+    const int kv = (int)((u - before) / sp.units), unit = (int)((u - before) - (long long)kv * sp.units);
+    const int n = (long long)(sp.units - unit) < u1 - u ? sp.units - unit : (int)(u1 - u);
+    const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row0 = (index - b * p.row_tiles) * C::kRows;
+    const int key0 = sp.start + unit * C::kUnit + team * C::kKeys;  // of this team's first tile; its tiles are a unit apart
+    int tiles = key0 < sp.hi ? (sp.hi - key0 + C::kUnit - 1) / C::kUnit : 0;
+    if (tiles > n) tiles = n;
+
+    // the pages of a tile's rows are asked for a tile ahead of the copies
+    const int32_t* table = p.tables + b * p.table_stride;
+    const uint8_t* kbase = p.k + kv * p.stride_head;
+    const uint8_t* vbase = p.v + kv * p.stride_head;
+    auto page_of = [&](int tile) {
+      const int key = key0 + tile * C::kUnit + member * C::kLoadRows + lane;
+      return tile < tiles && lane < C::kLoadRows && key < sp.hi ? table[divide(key, p.page)] : -1;
+    };
+    int page = page_of(0);
+    auto issue = [&](int tile) {
+      if (tile < tiles) {
+        const int key = key0 + tile * C::kUnit + member * C::kLoadRows + lane;
+        const bool ok = page >= 0 && page < p.pages;
+        const int64_t off = ok ? page * p.stride_page + (int64_t)(key - divide(key, p.page) * p.page.d) * p.stride_slot : 0;
+        const uint32_t seen = __ballot_sync(~0u, ok);
+        const int stage = tile % C::kStages;
+        if (lane == 0) s_seen[team][stage][member] = seen;
+        const uint32_t to = ring + stage * 2 * C::kHalf;
+#pragma unroll
+        for (int i = 0; i < (C::kLoadRows + kRowsPerCopy - 1) / kRowsPerCopy; ++i) {
+          const int r = i * kRowsPerCopy + copy_row;  // of this warp's rows
+          const int64_t o = __shfl_sync(~0u, off, r & 31);
+          const int row = member * C::kLoadRows + r, bytes = (seen >> (r & 31)) & 1 ? 16 : 0;
+          if (r < C::kLoadRows && copy_chunk < chunks) {
+            const uint32_t dst = to + row * C::kRowBytes + ((copy_chunk ^ swizzle(row)) << 4);
+            copy_async(dst, kbase + o + copy_chunk * 16, bytes);
+            copy_async(dst + C::kHalf, vbase + o + copy_chunk * 16, bytes);
+          }
+        }
+        page = page_of(tile + 1);
+      }
+      copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) issue(i);
+
+    // this thread's two rows: the query operand, scale and limits
+    uint32_t qf[DP / 16][4];
+    float row_scale[2];
+    int limit[2], lowest[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row0 + member * 16 + (lane >> 2) + 8 * h, i = divide(r, p.group);
+      const bool real = r < p.queries * p.group.d;
+      limit[h] = real && i < sp.count ? sp.length - sp.count + 1 + i : 0;
+      lowest[h] = p.window > 0 && limit[h] > p.window ? limit[h] - p.window : 0;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((int64_t)b * p.queries + i) * p.q_ldt + ((int64_t)kv * p.group.d + r - i * p.group.d) * p.q_ldh);
+      float top = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          // a matrix load of e4m3 codes leaves four neighbours in a thread: elements 4c .. 4c + 3 stand at k = 2c, 2c + 1, 2c + 8, 2c + 9
+          const int at = F8 ? kk * 8 + (lane & 3) * 2 + x : kk * 8 + (lane & 3) + 4 * x;
+          const uint32_t w = real && kk * 16 < p.d ? src[at] : 0u;
+          qf[kk][h + 2 * x] = w;
+          if constexpr (F8) top = fmaxf(top, fmaxf(fabsf(bf16lo_to_f32(w)), fabsf(bf16hi_to_f32(w))));
+        }
+      }
+      row_scale[h] = p.scale_log2;
+      if constexpr (F8) {
+        // bf16 -> f16 without loss: the row is scaled by a power of two that puts its largest element into [2^14, 2^15)
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        const int e = (int)(__float_as_uint(top) >> 23);  // biased exponent; 0 and infinities are left as they are
+        const int up = e == 0 || e == 255 ? 0 : 127 + 14 - e;
+        const float a = __uint_as_float((uint32_t)(127 + (up >> 1)) << 23), c = __uint_as_float((uint32_t)(127 + (up - (up >> 1))) << 23);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t w = qf[kk][h + 2 * x];
+            qf[kk][h + 2 * x] = pack_f16x2(bf16lo_to_f32(w) * a * c, bf16hi_to_f32(w) * a * c);
+          }
+        const float ia = __uint_as_float((uint32_t)(127 - (up >> 1)) << 23), ic = __uint_as_float((uint32_t)(127 - (up - (up >> 1))) << 23);
+        row_scale[h] = row_scale[h] * (p.k_scale ? load_f32(p.k_scale + kv) : 1.0f) * ia * ic;
+      }
+    }
+    float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < DP / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+
+    for (int tile = 0; tile < tiles; ++tile) {
+      copy_wait<C::kStages - 2>();
+      team_sync<TEAM>(team);
+      issue(tile + C::kStages - 1);
+      const int stage = tile % C::kStages, key = key0 + tile * C::kUnit;
+      const uint32_t kt = ring + stage * 2 * C::kHalf, vt = kt + C::kHalf;
+      uint32_t seen = 0;
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) seen |= s_seen[team][stage][w] << (w * C::kLoadRows);
+
+      float s[C::kKeys / 8][4];
+#pragma unroll
+      for (int j = 0; j < C::kKeys / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+      if constexpr (F8) {
+        const int row = (lane & 7) + (lane & 8), sw = swizzle(row);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; kk += 2) {
+          if (kk * 16 >= p.d) break;
+#pragma unroll
+          for (int j = 0; j < C::kKeys / 16; ++j) {
+            uint32_t r[4];
+            load_matrices(r, kt + (j * 16 + row) * C::kRowBytes + (((kk + (lane >> 4)) ^ sw) << 4));
+            multiply<true>(s[2 * j], qf[kk], codes_to_f16x2(r[0], false), codes_to_f16x2(r[0], true));
+            multiply<true>(s[2 * j + 1], qf[kk], codes_to_f16x2(r[1], false), codes_to_f16x2(r[1], true));
+            if ((kk + 1) * 16 < p.d) {
+              multiply<true>(s[2 * j], qf[kk + 1], codes_to_f16x2(r[2], false), codes_to_f16x2(r[2], true));
+              multiply<true>(s[2 * j + 1], qf[kk + 1], codes_to_f16x2(r[3], false), codes_to_f16x2(r[3], true));
+            }
+          }
+        }
+      } else {
+        const int row = (lane & 7) + ((lane >> 4) << 3), sw = swizzle(row), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          if (kk * 16 >= p.d) break;
+#pragma unroll
+          for (int j = 0; j < C::kKeys / 16; ++j) {
+            uint32_t r[4];
+            load_matrices(r, kt + (j * 16 + row) * C::kRowBytes + (((2 * kk + half) ^ sw) << 4));
+            multiply<false>(s[2 * j], qf[kk], r[0], r[1]);
+            multiply<false>(s[2 * j + 1], qf[kk], r[2], r[3]);
+          }
+        }
+      }
+
+      const bool whole = seen == (uint32_t)((1ull << C::kKeys) - 1);
+      const bool inside = key >= sp.last_lo && key + C::kKeys <= sp.first;  // every row sees all of the tile's keys that anyone sees
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < C::kKeys / 8; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float y = s[j][x] * row_scale[x >> 1];
+          if (!(whole && inside)) {
+            const int c = 8 * j + 2 * (lane & 3) + (x & 1), e = key + c;
+            if (!((seen >> c) & 1) || e < lowest[x >> 1] || e >= limit[x >> 1]) y = -INFINITY;
+          }
+          s[j][x] = y;
+          top[x >> 1] = fmaxf(top[x >> 1], y);
+        }
+      float base[2];
+      bool moved = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+        top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+        top[h] = fmaxf(top[h], m[h]);
+        base[h] = top[h] == -INFINITY ? 0.0f : top[h];
+        moved |= top[h] != m[h];
+      }
+      if (__any_sync(~0u, moved)) {
+        float keep[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          keep[h] = exp2_approx(m[h] - base[h]);
+          l[h] *= keep[h];
+          m[h] = top[h];
+        }
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j) {
+          o[j][0] *= keep[0], o[j][1] *= keep[0];
+          o[j][2] *= keep[1], o[j][3] *= keep[1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < C::kKeys / 8; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          s[j][x] = exp2_approx(s[j][x] - base[x >> 1] + C::kShift);
+          l[x >> 1] += s[j][x];
+        }
+
+      // A value that some rows see and others do not reaches both through the product, the latter with weight 0: harmless unless it is not finite.
+      bool odd = false;
+      if (!inside) {
+        const uint8_t* values = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
+        for (int i = lane; i < C::kKeys * chunks; i += 32) {
+          const int row = i / chunks, ch = i - row * chunks;
+          const uint4 w = *reinterpret_cast<const uint4*>(values + row * C::kRowBytes + ((ch ^ swizzle(row)) << 4));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t y = x == 0 ? w.x : x == 1 ? w.y : x == 2 ? w.z : w.w;
+            if constexpr (F8)
+              odd |= __vcmpeq4(y & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
+            else
+              odd |= __vcmpgeu2(y & 0x7FFF7FFFu, 0x7F807F80u) != 0;
+          }
+        }
+        odd = __any_sync(~0u, odd);
+      }
+      if (!odd) {
+#pragma unroll
+        for (int j = 0; j < C::kKeys / 16; ++j) {
+          uint32_t hi[4];
+          [[maybe_unused]] uint32_t lo[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {  // the scores' registers are the weights' operand: keys 2c, 2c + 1 and 2c + 8, 2c + 9 of rows r and r + 8
+            const float a = s[2 * j + (x >> 1)][2 * (x & 1)], c = s[2 * j + (x >> 1)][2 * (x & 1) + 1];
+            if constexpr (F8) {
+              hi[x] = pack_f16x2(a, c);
+            } else {
+              // 16 bits of a weight in two products: one of 8 bits would add an error as large as the result's own rounding
+              hi[x] = pack_bf16x2(a, c);
+              lo[x] = pack_bf16x2(a - bf16lo_to_f32(hi[x]), c - bf16hi_to_f32(hi[x]));
+            }
+          }
+          const int row = (lane & 7) + (lane & 8), sw = swizzle(row);
+          const uint32_t at = vt + (j * 16 + row) * C::kRowBytes;
+          if constexpr (F8) {
+#pragma unroll
+            for (int t = 0; t < DP / 16; t += 2) {
+              if (t * 16 >= p.d) break;
+              uint32_t r[4];
+              load_matrices_turned(r, at + (((t + (lane >> 4)) ^ sw) << 4));
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                if ((t + x) * 16 >= p.d) break;
+                // a thread holds elements (2c', 2c' + 1) of two keys: bytes to (key, key + 1) pairs, the even elements in one product, the odd ones in another
+                const uint32_t w0 = __byte_perm(r[2 * x], 0, 0x3120), w1 = __byte_perm(r[2 * x + 1], 0, 0x3120);
+                multiply<true>(o[2 * (t + x)], hi, codes_to_f16x2(w0, false), codes_to_f16x2(w1, false));
+                multiply<true>(o[2 * (t + x) + 1], hi, codes_to_f16x2(w0, true), codes_to_f16x2(w1, true));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) {
+              if (t * 16 >= p.d) break;
+              uint32_t r[4];
+              load_matrices_turned(r, at + (((2 * t + (lane >> 4)) ^ sw) << 4));
+              multiply<false>(o[2 * t], hi, r[0], r[1]);
+              multiply<false>(o[2 * t], lo, r[0], r[1]);
+              multiply<false>(o[2 * t + 1], hi, r[2], r[3]);
+              multiply<false>(o[2 * t + 1], lo, r[2], r[3]);
+            }
+          }
+        }
+      } else {
+        const uint8_t* values = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
+#pragma unroll
+        for (int eight = 0; eight < C::kKeys / 8; ++eight)
+#pragma unroll 1
+          for (int x8 = 0; x8 < 8; ++x8) {
+            const int c = 8 * eight + x8;
+            float w[2];
+            bool sees[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float w0 = s[eight][2 * h], w1 = s[eight][2 * h + 1];
+              w[h] = __shfl_sync(~0u, x8 & 1 ? w1 : w0, (lane & ~3) | (x8 >> 1));
+              sees[h] = ((seen >> c) & 1) && key + c >= lowest[h] && key + c < limit[h];
+            }
+#pragma unroll
+            for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int e = F8 ? (j >> 1) * 16 + 4 * (lane & 3) + 2 * x + (j & 1) : j * 8 + 2 * (lane & 3) + x, byte = F8 ? e : 2 * e;
+                if (e < p.d) {
+                  const uint8_t* from = values + c * C::kRowBytes + (((byte >> 4) ^ swizzle(c)) << 4) + (byte & 15);
+                  const float y = F8 ? e4m3_to_f32(*from) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(from));
+                  if (sees[0]) o[j][x] = fmaf(w[0], y, o[j][x]);
+                  if (sees[1]) o[j][2 + x] = fmaf(w[1], y, o[j][2 + x]);
+                }
+              }
+          }
+      }
+    }
+
+    // join the teams, in their order
+    copy_wait<0>();
+    __syncthreads();  // the ring is free
+    float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(~0u, l[h], 1);
+      l[h] += __shfl_xor_sync(~0u, l[h], 2);
+      const int r = team * C::kRows + member * 16 + (lane >> 2) + 8 * h;
+      if ((lane & 3) == 0) s_stats[r] = make_float2(m[h], l[h]);
+#pragma unroll
+      for (int j = 0; j < DP / 8; ++j) {
+        if constexpr (F8) {
+          if (j & 1) continue;
+          const int e = (j >> 1) * 16 + 4 * (lane & 3);
+          if (e < p.d) *reinterpret_cast<float4*>(sums + r * C::kPitch + e) = make_float4(o[j][2 * h], o[j + 1][2 * h], o[j][2 * h + 1], o[j + 1][2 * h + 1]);
+        } else {
+          const int e = j * 8 + 2 * (lane & 3);
+          if (e < p.d) *reinterpret_cast<float2*>(sums + r * C::kPitch + e) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+        }
+      }
+    }
+    __syncthreads();
+    const bool all = n == sp.units;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (u == u0 ? 0 : 1);
+    int rows = p.queries * p.group.d - row0;
+    if (rows > C::kRows) rows = C::kRows;
+    for (int r = warp; r < rows; r += kAttendWarps) {
+      const int i = divide(row0 + r, p.group), head = kv * p.group.d + row0 + r - i * p.group.d;
+      float top = -INFINITY, sum = 0.0f, w[C::kTeams];
+#pragma unroll
+      for (int t = 0; t < C::kTeams; ++t) top = fmaxf(top, s_stats[t * C::kRows + r].x);
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int t = 0; t < C::kTeams; ++t) {
+        w[t] = exp2_approx(s_stats[t * C::kRows + r].x - base);
+        sum = fmaf(w[t], s_stats[t * C::kRows + r].y, sum);
+      }
+      if (i >= sp.count) sum = 0.0f;  // padding: it went along unmasked
+      const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
+      const int64_t token = (int64_t)b * p.queries + i;
+      for (int e = 4 * lane; e < p.d; e += 128) {
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int t = 0; t < C::kTeams; ++t) {
+          const float4 y = *reinterpret_cast<const float4*>(sums + (t * C::kRows + r) * C::kPitch + e);
+          x.x = fmaf(w[t], y.x, x.x), x.y = fmaf(w[t], y.y, x.y), x.z = fmaf(w[t], y.z, x.z), x.w = fmaf(w[t], y.w, x.w);
+        }
+        if (all) {
+          uint2 pair = make_uint2(pack_bf16x2(x.x * finish, x.y * finish), pack_bf16x2(x.z * finish, x.w * finish));
+          if (sum == 0.0f) pair = make_uint2(0u, 0u);  // a row that sees nothing, whatever the others' values were
+          *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = pair;
+        } else {
+          *reinterpret_cast<float4*>(p.part_sums + (slot * C::kRows + r) * p.d + e) = x;
+        }
+      }
+      if (lane == 0) {
+        if (!all)
+          p.part_stats[slot * C::kRows + r] = make_float2(top, sum);
+        else if (p.lse)
+          p.lse[token * p.q_heads + head] = sum == 0.0f ? -INFINITY : (base + log2f(sum) - C::kShift) * 0.6931471805599453f;
+      }
+    }
+    __syncthreads();  // before the next segment's copies
+    u += n;
+    if (u == before + (long long)sp.units * p.kv_heads) {
+      before = u;
+      ++index;
+    }
+  }
+}
+
+// One block per row of a (span, kv head): adds up what the blocks that shared it left, or writes the result of a row that sees nothing.
+template <int ROWS, int UNIT>
+__global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(const AttendArgs p, int grid, float shift) {
+  __shared__ long long s_scratch[kAttendWarps];
+  __shared__ float s_weight[kMaxAttendBlocks], s_part[kAttendWarps];
+  __shared__ float4 s_sum[kAttendThreads];
+  const int index = blockIdx.x / p.kv_heads, kv = blockIdx.x - index * p.kv_heads, r = blockIdx.y;
+  const int b = index / p.row_tiles, row0 = (index - b * p.row_tiles) * ROWS;
+  if (row0 + r >= p.queries * p.group.d) return;
+  const Span sp = span_of<ROWS, UNIT>(p, index);
+  const int units = sp.units, i = divide(row0 + r, p.group), head = kv * p.group.d + row0 + r - i * p.group.d;
+  const int64_t token = (int64_t)b * p.queries + i;
+  __nv_bfloat16* out = p.out + token * p.out_ldt + head * p.out_ldh;
+  if (units == 0 || i >= sp.count) {
+    for (int e = 4 * threadIdx.x; e < p.d; e += 4 * kAttendThreads) *reinterpret_cast<uint2*>(out + e) = make_uint2(0u, 0u);
+    if (threadIdx.x == 0 && p.lse) p.lse[token * p.q_heads + head] = -INFINITY;
+    return;
+  }
+  long long all = 0, front = 0;
+  for (int x = threadIdx.x; x < p.spans; x += kAttendThreads) {
+    const int u = span_of<ROWS, UNIT>(p, x).units;
+    all += u;
+    if (x < index) front += u;
+  }
+  const long long total = block_sum(all, s_scratch) * p.kv_heads;
+  const long long first = block_sum(front, s_scratch) * p.kv_heads + (long long)kv * units, last = first + units - 1;
+  const long long blocks = total < grid ? total : grid;
+  // block c has [c * total / blocks, (c + 1) * total / blocks): the one that holds unit u is the last that begins at or before it
+  const int c0 = (int)(((first + 1) * blocks - 1) / total), c1 = (int)(((last + 1) * blocks - 1) / total);
+  if (c0 == c1) return;
+  const int n = c1 - c0 + 1;
+  auto slot_of = [&](int x) { return 2 * (int64_t)(c0 + x) + (first <= total * (c0 + x) / blocks ? 0 : 1); };
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float top = -INFINITY;
+  for (int x = threadIdx.x; x < n; x += kAttendThreads) {
+    s_weight[x] = p.part_stats[slot_of(x) * ROWS + r].x;
+    top = fmaxf(top, s_weight[x]);
+  }
+  for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+  if (lane == 0) s_part[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_part[0], s_part[1]), fmaxf(s_part[2], s_part[3]));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+  for (int x = threadIdx.x; x < n; x += kAttendThreads) {
+    const float w = exp2_approx(s_weight[x] - base);
+    s_weight[x] = w;
+    sum = fmaf(w, p.part_stats[slot_of(x) * ROWS + r].y, sum);
+  }
+  for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+  __syncthreads();
+  if (lane == 0) s_part[warp] = sum;
+  __syncthreads();
+  sum = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
+
+  const int quads = p.d / 4, groups = kAttendThreads / quads, g = threadIdx.x / quads, e = 4 * (threadIdx.x - g * quads);
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (g < groups) {
+#pragma unroll 4
+    for (int x = g; x < n; x += groups) {
+      const float4 y = *reinterpret_cast<const float4*>(p.part_sums + (slot_of(x) * ROWS + r) * p.d + e);
+      const float w = s_weight[x];
+      acc.x = fmaf(w, y.x, acc.x), acc.y = fmaf(w, y.y, acc.y), acc.z = fmaf(w, y.z, acc.z), acc.w = fmaf(w, y.w, acc.w);
+    }
+    s_sum[threadIdx.x] = acc;
+  }
+  __syncthreads();
+  if (g == 0) {
+    for (int x = 1; x < groups; ++x) {
+      const float4 y = s_sum[x * quads + threadIdx.x];
+      acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+    }
+    const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
+    uint2 pair = make_uint2(pack_bf16x2(acc.x * finish, acc.y * finish), pack_bf16x2(acc.z * finish, acc.w * finish));
+    if (sum == 0.0f) pair = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(out + e) = pair;
+    if (threadIdx.x == 0 && p.lse) p.lse[token * p.q_heads + head] = sum == 0.0f ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
+  }
+}
+
+// Blocks of a call: as many as fit the device at once, or one per unit where the table cannot name more.
+template <int DP, bool F8, int TEAM>
+static int attend_blocks(int64_t spans, int64_t kv_heads, int64_t entries) {
+  using C = AttendCfg<DP, F8, TEAM>;
+  int64_t cap = (int64_t)sm_count() * C::kBlocksPerSm;
+  if (cap > kMaxAttendBlocks) cap = kMaxAttendBlocks;
+  const int64_t heads = spans * kv_heads, each = (entries + C::kUnit - 1) / C::kUnit;
+  return (int)(heads >= cap || each >= cap || heads * each >= cap ? cap : heads * each);
+}
+
+template <int DP, bool F8, int TEAM>
+struct AttendCall {
+  using C = AttendCfg<DP, F8, TEAM>;
+  static int64_t workspace(int64_t spans, int64_t kv_heads, int64_t d, int64_t entries) {
+    return 2 * (int64_t)attend_blocks<DP, F8, TEAM>(spans, kv_heads, entries) * C::kRows * (d + 2) * 4;
+  }
+  static tf_status launch(AttendArgs p, void* workspace, cudaStream_t stream) {
+    auto kernel = paged_attention_kernel<DP, F8, TEAM>;
+    static thread_local int configured_dev = -1;
+    int dev = 0;
+    TF_CUDA(cudaGetDevice(&dev));
+    if (configured_dev != dev) {
+      TF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+      configured_dev = dev;
+    }
+    const int blocks = attend_blocks<DP, F8, TEAM>(p.spans, p.kv_heads, p.entries);
+    p.part_sums = static_cast<float*>(workspace);
+    p.part_stats = reinterpret_cast<float2*>(p.part_sums + 2 * (int64_t)blocks * C::kRows * p.d);
+    kernel<<<blocks, kAttendThreads, C::kSmem, stream>>>(p);
+    TF_LAUNCH_CHECK();
+    int rows = p.queries * p.group.d;
+    if (rows > C::kRows) rows = C::kRows;
+    paged_attention_join_kernel<C::kRows, C::kUnit><<<dim3((unsigned)p.spans * (unsigned)p.kv_heads, (unsigned)rows), kAttendThreads, 0, stream>>>(p, blocks, C::kShift);
+    TF_LAUNCH_CHECK();
+    return TF_OK;
+  }
+};
+
+}  // namespace tf
