@@ -21,17 +21,6 @@
 
 namespace tf {
 
-// floor(n / d) for 0 <= n < 2^31 by a multiplication: with 2^l >= d, m = ceil(2^(31 + l) / d) exceeds the quotient by less than 2^l / d parts.
-struct Divisor {
-  uint32_t mul, shift;
-  int d;
-};
-static Divisor divisor(int d) {
-  int l = 0;
-  while ((1ll << l) < d) ++l;
-  return {(uint32_t)(((1ull << (31 + l)) + d - 1) / d), (uint32_t)(31 + l), d};
-}
-
 struct AttendArgs {
   const uint8_t* k;
   const uint8_t* v;
@@ -79,7 +68,6 @@ struct AttendCfg {
   static constexpr float kShift = F8 ? 15.0f : 0.0f;
 };
 
-__device__ __forceinline__ int divide(int n, Divisor v) { return (int)(((uint64_t)(uint32_t)n * v.mul) >> v.shift); }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

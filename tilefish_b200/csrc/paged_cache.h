@@ -1,4 +1,4 @@
-// What both entry points over a paged cache check of its descriptor.
+// What the rotary and paged-attention kernels share: the check of a cache's descriptor, and a division.
 #pragma once
 
 #include "common.cuh"
@@ -20,5 +20,19 @@ inline tf_status check_cache(const tf_paged_cache* c, const char* fn) {
   if (c->dtype == TF_CACHE_BF16 && (c->k_scale || c->v_scale)) return fail(TF_ERR_INVALID_ARGUMENT, "%s: a bf16 cache has no scales", fn);
   return TF_OK;
 }
+
+// floor(n / d) for 0 <= n < 2^31 by a multiplication: with 2^l >= d, m = ceil(2^(31 + l) / d) exceeds the quotient by less than 2^l / d parts.
+struct Divisor {
+  uint32_t mul, shift;
+  int d;
+};
+inline Divisor divisor(int d) {
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  return {(uint32_t)(((1ull << (31 + l)) + d - 1) / d), (uint32_t)(31 + l), d};
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ int divide(int n, Divisor v) { return (int)(((uint64_t)(uint32_t)n * v.mul) >> v.shift); }
+#endif
 
 }  // namespace tf

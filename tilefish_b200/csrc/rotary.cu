@@ -132,8 +132,212 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(RotaryArgs p) {
   }
 }
 
+// ---- whole vectors -----------------------------------------------------------------------------------------------------------------
+// A block takes rows (token, head) in the tensor's order, `lanes` threads a row and 16 elements a thread: two 16-byte loads for bf16 (half layout: eight
+// pairs, one load from each half). Cosines and sines of the block's tokens are computed once, into shared memory, while the rows' loads are in flight.
+// HBM-bound; a rotation that computes its angle per element is bound by sincospif instead.
+
+struct Sixteen {
+  float v[16];
+};
+
+template <typename T>
+struct Vectors;
+template <>
+struct Vectors<__nv_bfloat16> {
+  uint4 w[2];
+  __device__ __forceinline__ void load(const __nv_bfloat16* lo, const __nv_bfloat16* hi) {
+    w[0] = *reinterpret_cast<const uint4*>(lo);
+    w[1] = *reinterpret_cast<const uint4*>(hi);
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* lo, __nv_bfloat16* hi) const {
+    *reinterpret_cast<uint4*>(lo) = w[0];
+    *reinterpret_cast<uint4*>(hi) = w[1];
+  }
+  __device__ __forceinline__ Sixteen unpack() const {
+    Sixteen x;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t y[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x.v[8 * i + 2 * j] = bf16lo_to_f32(y[j]), x.v[8 * i + 2 * j + 1] = bf16hi_to_f32(y[j]);
+    }
+    return x;
+  }
+  __device__ __forceinline__ void pack(const Sixteen& x) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      w[i] = make_uint4(pack_bf16x2(x.v[8 * i], x.v[8 * i + 1]), pack_bf16x2(x.v[8 * i + 2], x.v[8 * i + 3]), pack_bf16x2(x.v[8 * i + 4], x.v[8 * i + 5]),
+                        pack_bf16x2(x.v[8 * i + 6], x.v[8 * i + 7]));
+  }
+  __device__ __forceinline__ void keep_pair(const Vectors& from, int pair) {  // pair (2 pair, 2 pair + 1) as it was
+    reinterpret_cast<uint32_t*>(w)[pair] = reinterpret_cast<const uint32_t*>(from.w)[pair];
+  }
+};
+template <>
+struct Vectors<float> {
+  float4 w[4];
+  __device__ __forceinline__ void load(const float* lo, const float* hi) {
+    w[0] = reinterpret_cast<const float4*>(lo)[0], w[1] = reinterpret_cast<const float4*>(lo)[1];
+    w[2] = reinterpret_cast<const float4*>(hi)[0], w[3] = reinterpret_cast<const float4*>(hi)[1];
+  }
+  __device__ __forceinline__ void store(float* lo, float* hi) const {
+    reinterpret_cast<float4*>(lo)[0] = w[0], reinterpret_cast<float4*>(lo)[1] = w[1];
+    reinterpret_cast<float4*>(hi)[0] = w[2], reinterpret_cast<float4*>(hi)[1] = w[3];
+  }
+  __device__ __forceinline__ Sixteen unpack() const {
+    Sixteen x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[4 * i] = w[i].x, x.v[4 * i + 1] = w[i].y, x.v[4 * i + 2] = w[i].z, x.v[4 * i + 3] = w[i].w;
+    return x;
+  }
+  __device__ __forceinline__ void pack(const Sixteen& x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = make_float4(x.v[4 * i], x.v[4 * i + 1], x.v[4 * i + 2], x.v[4 * i + 3]);
+  }
+  __device__ __forceinline__ void keep_pair(const Vectors& from, int pair) {
+    reinterpret_cast<float2*>(w)[pair] = reinterpret_cast<const float2*>(from.w)[pair];
+  }
+};
+
+struct VectorPlan {
+  int lanes_log2;      // threads of a row: the power of two that holds its vectors
+  int items;           // 16-element vectors of a row
+  Divisor heads, half; // rows of a token; pairs of a head
+  int max_tokens;      // that one block's rows touch
+};
+
+template <typename T, bool kAppend, bool kInterleaved, int kRows>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_vector_kernel(const RotaryArgs p, const VectorPlan plan) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  float2* table = reinterpret_cast<float2*>(smem);                                            // [tokens of the block][pairs]
+  int64_t* entry = reinterpret_cast<int64_t*>(table + plan.max_tokens * (p.rot / 2));          // [tokens of the block] where keys and values go
+  const int slots = kRotaryThreads >> plan.lanes_log2, slot = threadIdx.x >> plan.lanes_log2, item = threadIdx.x & ((1 << plan.lanes_log2) - 1);
+  const int64_t r0 = (int64_t)blockIdx.x * (slots * kRows), t0 = r0 / p.heads;
+  const int first = (int)(r0 - t0 * p.heads), half = p.rot / 2;
+  // offsets of this thread's two vectors in a row: both halves of eight pairs, or 16 elements in a row
+  const bool pairs = kInterleaved || item * 16 < p.rot;  // half layout: a vector of pairs or of elements that are copied
+  const int lo = !kInterleaved && pairs ? item * 8 : item * 16, hi = !kInterleaved && pairs ? item * 8 + half : item * 16 + 8;
+
+  Vectors<T> x[kRows];
+  int token[kRows], head[kRows];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int r = first + slot + u * slots;
+    token[u] = divide(r, plan.heads);
+    head[u] = r - token[u] * p.heads;
+    const int64_t t = t0 + token[u];
+    if (item >= plan.items || t >= p.tokens) {
+      token[u] = -1;
+      continue;
+    }
+    const T* src = reinterpret_cast<const T*>(p.q) + t * p.q_ldt + head[u] * p.q_ldh;
+    if constexpr (kAppend) {
+      const int h = head[u] - p.q_heads, kv = (int)p.cache.kv_heads;
+      if (h >= 0) src = reinterpret_cast<const T*>(h < kv ? p.k + t * p.k_ldt + h * p.k_ldh : p.v + t * p.v_ldt + (h - kv) * p.v_ldh);
+    }
+    x[u].load(src + lo, src + hi);
+  }
+  {
+    int tokens = divide(first + slots * kRows - 1, plan.heads) + 1;
+    if (tokens > p.tokens - t0) tokens = (int)(p.tokens - t0);
+    for (int i = threadIdx.x; i < tokens * half; i += kRotaryThreads) {
+      const int t = divide(i, plan.half);
+      table[i] = cos_sin(p, position_of(p, t0 + t), i - t * half);
+    }
+    if constexpr (kAppend)
+      for (int t = threadIdx.x; t < tokens; t += kRotaryThreads) entry[t] = entry_offset(p, t0 + t, 0);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    if (token[u] < 0) continue;
+    const int64_t t = t0 + token[u];
+    const int kv = kAppend ? (int)p.cache.kv_heads : 0, h = head[u] - p.q_heads;
+    const bool turned = !kAppend || h < kv;
+    if (turned && pairs) {
+      const float2* cs = table + token[u] * half + item * 8;
+      const Sixteen a = x[u].unpack();
+      Sixteen y = a;
+      const Vectors<T> was = x[u];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int i0 = kInterleaved ? 2 * i : i, i1 = kInterleaved ? 2 * i + 1 : i + 8;
+        if (!kInterleaved || item * 8 + i < half) {
+          const float2 c = cs[i];
+          y.v[i0] = fmaf(a.v[i0], c.x, -(a.v[i1] * c.y));
+          y.v[i1] = fmaf(a.v[i1], c.x, a.v[i0] * c.y);
+        }
+      }
+      if (kAppend && h >= 0 && p.cache.dtype == TF_CACHE_E4M3) {
+        const int64_t at = entry[token[u]];
+        if (at < 0) continue;
+        const float s = p.cache.k_scale ? __frcp_rn(load_f32(p.cache.k_scale + h)) : 1.0f;
+        uint8_t* code = static_cast<uint8_t*>(p.cache.k) + at + h * p.cache.stride_head;
+        *reinterpret_cast<uint2*>(code + lo) =
+            make_uint2(cvt_e4m3x4(y.v[0] * s, y.v[1] * s, y.v[2] * s, y.v[3] * s), cvt_e4m3x4(y.v[4] * s, y.v[5] * s, y.v[6] * s, y.v[7] * s));
+        *reinterpret_cast<uint2*>(code + hi) =
+            make_uint2(cvt_e4m3x4(y.v[8] * s, y.v[9] * s, y.v[10] * s, y.v[11] * s), cvt_e4m3x4(y.v[12] * s, y.v[13] * s, y.v[14] * s, y.v[15] * s));
+        continue;
+      }
+      x[u].pack(y);
+      if constexpr (kInterleaved) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (item * 8 + i >= half) x[u].keep_pair(was, i);  // a copy keeps its bits
+      }
+    }
+    if (!kAppend || h < 0) {
+      if (!pairs && p.in_place) continue;
+      T* dst = reinterpret_cast<T*>(p.q_out) + t * p.qo_ldt + head[u] * p.qo_ldh;
+      x[u].store(dst + lo, dst + hi);
+    } else {
+      const int64_t at = entry[token[u]];
+      if (at < 0) continue;
+      const int hh = h < kv ? h : h - kv;
+      uint8_t* to = static_cast<uint8_t*>(h < kv ? p.cache.k : p.cache.v);
+      if (p.cache.dtype == TF_CACHE_BF16) {
+        T* dst = reinterpret_cast<T*>(to + at) + hh * p.cache.stride_head;
+        x[u].store(dst + lo, dst + hi);
+      } else {
+        const float* scale = h < kv ? p.cache.k_scale : p.cache.v_scale;
+        const float s = scale ? __frcp_rn(load_f32(scale + hh)) : 1.0f;
+        const Sixteen y = x[u].unpack();
+        uint8_t* code = to + at + hh * p.cache.stride_head;
+        *reinterpret_cast<uint2*>(code + lo) =
+            make_uint2(cvt_e4m3x4(y.v[0] * s, y.v[1] * s, y.v[2] * s, y.v[3] * s), cvt_e4m3x4(y.v[4] * s, y.v[5] * s, y.v[6] * s, y.v[7] * s));
+        *reinterpret_cast<uint2*>(code + hi) =
+            make_uint2(cvt_e4m3x4(y.v[8] * s, y.v[9] * s, y.v[10] * s, y.v[11] * s), cvt_e4m3x4(y.v[12] * s, y.v[13] * s, y.v[14] * s, y.v[15] * s));
+      }
+    }
+  }
+}
+
+template <typename T, bool kAppend, int kRows>
+static tf_status launch_rotary_vectors(const RotaryArgs& p, cudaStream_t stream) {
+  VectorPlan plan = {};
+  plan.items = p.d / 16;
+  while ((1 << plan.lanes_log2) < plan.items) ++plan.lanes_log2;
+  plan.heads = divisor(p.heads);
+  plan.half = divisor(p.rot > 0 ? p.rot / 2 : 1);
+  const int rows = (kRotaryThreads >> plan.lanes_log2) * kRows;
+  plan.max_tokens = (rows + p.heads - 2) / p.heads + 1;
+  const int64_t blocks = (p.tokens * p.heads + rows - 1) / rows;
+  if (blocks > INT32_MAX) return fail(TF_ERR_UNSUPPORTED, "%s: %lld rows are too many", __func__, (long long)(p.tokens * p.heads));
+  const size_t smem = (size_t)plan.max_tokens * ((size_t)p.rot / 2 * sizeof(float2) + (kAppend ? sizeof(int64_t) : 0));
+  auto kernel = p.interleaved ? rotary_vector_kernel<T, kAppend, true, kRows> : rotary_vector_kernel<T, kAppend, false, kRows>;
+  kernel<<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(p, plan);
+  TF_LAUNCH_CHECK();
+  return TF_OK;
+}
+
 template <typename T, bool kAppend>
 static tf_status launch_rotary(const RotaryArgs& p, cudaStream_t stream) {
+  // Whole vectors need 16-byte aligned rows, whole vectors of pairs in the half layout, and a row that at most one block's threads hold.
+  const int64_t unit = 16 / (int64_t)sizeof(T);
+  auto aligned = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && a % unit == 0 && b % unit == 0; };
+  if (p.d % 16 == 0 && (p.interleaved || p.rot % 16 == 0) && aligned(p.q, p.q_ldt, p.q_ldh) && aligned(p.q_out, p.qo_ldt, p.qo_ldh))
+    return launch_rotary_vectors<T, kAppend, 2>(p, stream);
   const int64_t total = p.tokens * p.heads * (p.d - p.rot / 2), cap = (int64_t)sm_count() * 8;
   const int64_t need = (total + kRotaryThreads - 1) / kRotaryThreads;
   rotary_kernel<T, kAppend><<<(unsigned)(need < cap ? need : cap), kRotaryThreads, 0, stream>>>(p);
