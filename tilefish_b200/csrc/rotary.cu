@@ -21,7 +21,9 @@ struct RotaryArgs {
   int64_t k_ldt, k_ldh, v_ldt, v_ldh;
   tf_paged_cache cache;
   const int32_t* tables;
-  int64_t table_rows, table_cols, table_stride;
+  int64_t table_rows, table_stride;
+  int entries;  // what a table can name
+  Divisor page;
   const int32_t* rows;
   int64_t tokens_per_row;
   const void* positions;
@@ -51,12 +53,11 @@ __device__ __forceinline__ float2 cos_sin(const RotaryArgs& p, int64_t position,
 __device__ __forceinline__ int64_t entry_offset(const RotaryArgs& p, int64_t t, int head) {
   const int64_t e = position_of(p, t);
   const int64_t row = p.rows ? (int64_t)p.rows[t] : t / p.tokens_per_row;
-  if (e < 0 || row < 0 || row >= p.table_rows) return -1;
-  const int64_t col = e / p.cache.page_size;
-  if (col >= p.table_cols) return -1;
+  if (e < 0 || e >= p.entries || row < 0 || row >= p.table_rows) return -1;
+  const int col = divide((int)e, p.page);
   const int32_t page = p.tables[row * p.table_stride + col];
   if (page < 0 || page >= p.cache.pages) return -1;
-  const int64_t at = page * p.cache.stride_page + head * p.cache.stride_head + (e - col * p.cache.page_size) * p.cache.stride_slot;
+  const int64_t at = page * p.cache.stride_page + head * p.cache.stride_head + ((int)e - col * p.page.d) * p.cache.stride_slot;
   return p.cache.dtype == TF_CACHE_BF16 ? at * 2 : at;
 }
 
@@ -133,93 +134,57 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(RotaryArgs p) {
 }
 
 // ---- whole vectors -----------------------------------------------------------------------------------------------------------------
-// A block takes rows (token, head) in the tensor's order, `lanes` threads a row and 16 elements a thread: two 16-byte loads for bf16 (half layout: eight
-// pairs, one load from each half). Cosines and sines of the block's tokens are computed once, into shared memory, while the rows' loads are in flight.
-// HBM-bound; a rotation that computes its angle per element is bound by sincospif instead.
-
-struct Sixteen {
-  float v[16];
-};
+// A block takes rows (token, head) in the tensor's order, `lanes` threads a row and 16 elements a thread, as vectors of 16 bytes that lie
+// `step` elements apart, so that neighbouring threads' vectors are neighbours. Cosines and sines of the block's tokens are computed once, into
+// shared memory, while the rows' loads are in flight; their order there puts neighbouring threads into different banks (in the order of the pairs
+// 8192 x 64 x 128 bf16 took 54 us, now 41: the copy rate). HBM-bound.
 
 template <typename T>
-struct Vectors;
-template <>
-struct Vectors<__nv_bfloat16> {
-  uint4 w[2];
-  __device__ __forceinline__ void load(const __nv_bfloat16* lo, const __nv_bfloat16* hi) {
-    w[0] = *reinterpret_cast<const uint4*>(lo);
-    w[1] = *reinterpret_cast<const uint4*>(hi);
+struct Vectors {
+  static constexpr int kElems = 16 / (int)sizeof(T), kCount = 16 / kElems;  // of a vector; vectors
+  uint4 w[kCount];
+  __device__ __forceinline__ float get(int v, int e) const {
+    const uint32_t* y = reinterpret_cast<const uint32_t*>(&w[v]);
+    if constexpr (sizeof(T) == 4) return __uint_as_float(y[e]);
+    return e & 1 ? bf16hi_to_f32(y[e >> 1]) : bf16lo_to_f32(y[e >> 1]);
   }
-  __device__ __forceinline__ void store(__nv_bfloat16* lo, __nv_bfloat16* hi) const {
-    *reinterpret_cast<uint4*>(lo) = w[0];
-    *reinterpret_cast<uint4*>(hi) = w[1];
-  }
-  __device__ __forceinline__ Sixteen unpack() const {
-    Sixteen x;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t y[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x.v[8 * i + 2 * j] = bf16lo_to_f32(y[j]), x.v[8 * i + 2 * j + 1] = bf16hi_to_f32(y[j]);
-    }
-    return x;
-  }
-  __device__ __forceinline__ void pack(const Sixteen& x) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      w[i] = make_uint4(pack_bf16x2(x.v[8 * i], x.v[8 * i + 1]), pack_bf16x2(x.v[8 * i + 2], x.v[8 * i + 3]), pack_bf16x2(x.v[8 * i + 4], x.v[8 * i + 5]),
-                        pack_bf16x2(x.v[8 * i + 6], x.v[8 * i + 7]));
-  }
-  __device__ __forceinline__ void keep_pair(const Vectors& from, int pair) {  // pair (2 pair, 2 pair + 1) as it was
-    reinterpret_cast<uint32_t*>(w)[pair] = reinterpret_cast<const uint32_t*>(from.w)[pair];
-  }
-};
-template <>
-struct Vectors<float> {
-  float4 w[4];
-  __device__ __forceinline__ void load(const float* lo, const float* hi) {
-    w[0] = reinterpret_cast<const float4*>(lo)[0], w[1] = reinterpret_cast<const float4*>(lo)[1];
-    w[2] = reinterpret_cast<const float4*>(hi)[0], w[3] = reinterpret_cast<const float4*>(hi)[1];
-  }
-  __device__ __forceinline__ void store(float* lo, float* hi) const {
-    reinterpret_cast<float4*>(lo)[0] = w[0], reinterpret_cast<float4*>(lo)[1] = w[1];
-    reinterpret_cast<float4*>(hi)[0] = w[2], reinterpret_cast<float4*>(hi)[1] = w[3];
-  }
-  __device__ __forceinline__ Sixteen unpack() const {
-    Sixteen x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x.v[4 * i] = w[i].x, x.v[4 * i + 1] = w[i].y, x.v[4 * i + 2] = w[i].z, x.v[4 * i + 3] = w[i].w;
-    return x;
-  }
-  __device__ __forceinline__ void pack(const Sixteen& x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = make_float4(x.v[4 * i], x.v[4 * i + 1], x.v[4 * i + 2], x.v[4 * i + 3]);
-  }
-  __device__ __forceinline__ void keep_pair(const Vectors& from, int pair) {
-    reinterpret_cast<float2*>(w)[pair] = reinterpret_cast<const float2*>(from.w)[pair];
+  // elements e and e + 1
+  __device__ __forceinline__ void set2(int v, int e, float a, float b) {
+    uint32_t* y = reinterpret_cast<uint32_t*>(&w[v]);
+    if constexpr (sizeof(T) == 4)
+      y[e] = __float_as_uint(a), y[e + 1] = __float_as_uint(b);
+    else
+      y[e >> 1] = pack_bf16x2(a, b);
   }
 };
 
 struct VectorPlan {
   int lanes_log2;      // threads of a row: the power of two that holds its vectors
-  int items;           // 16-element vectors of a row
+  int items;           // threads that have 16 elements of it
   Divisor heads, half; // rows of a token; pairs of a head
   int max_tokens;      // that one block's rows touch
+  int lanes, table;    // cosines of pair i of a token: at (i % p) * lanes + i / p of its `table` ones, p pairs in a vector
 };
 
-template <typename T, bool kAppend, bool kInterleaved, int kRows>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_vector_kernel(const RotaryArgs p, const VectorPlan plan) {
+template <typename T, bool kAppend, bool kInterleaved, int kRows, int kBlocks>
+__global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(const RotaryArgs p, const VectorPlan plan) {
+  using X = Vectors<T>;
+  constexpr int kE = X::kElems, kV = X::kCount, kPairs = kInterleaved ? kE / 2 : kE;
   extern __shared__ __align__(16) uint8_t smem[];
-  float2* table = reinterpret_cast<float2*>(smem);                                            // [tokens of the block][pairs]
-  int64_t* entry = reinterpret_cast<int64_t*>(table + plan.max_tokens * (p.rot / 2));          // [tokens of the block] where keys and values go
+  float2* table = reinterpret_cast<float2*>(smem);
+  int64_t* entry = reinterpret_cast<int64_t*>(table + plan.max_tokens * plan.table);  // [tokens of the block] where keys and values go
   const int slots = kRotaryThreads >> plan.lanes_log2, slot = threadIdx.x >> plan.lanes_log2, item = threadIdx.x & ((1 << plan.lanes_log2) - 1);
   const int64_t r0 = (int64_t)blockIdx.x * (slots * kRows), t0 = r0 / p.heads;
   const int first = (int)(r0 - t0 * p.heads), half = p.rot / 2;
-  // offsets of this thread's two vectors in a row: both halves of eight pairs, or 16 elements in a row
-  const bool pairs = kInterleaved || item * 16 < p.rot;  // half layout: a vector of pairs or of elements that are copied
-  const int lo = !kInterleaved && pairs ? item * 8 : item * 16, hi = !kInterleaved && pairs ? item * 8 + half : item * 16 + 8;
+  int tokens = divide(first + slots * kRows - 1, plan.heads) + 1;
+  if (tokens > p.tokens - t0) tokens = (int)(p.tokens - t0);
+  if constexpr (kAppend)  // the longest chain of loads (position, page) goes first
+    for (int t = threadIdx.x; t < tokens; t += kRotaryThreads) entry[t] = entry_offset(p, t0 + t, 0);
 
-  Vectors<T> x[kRows];
+  // this thread's vectors of a row lie at base + v * step. Half layout: vectors v and v + kV / 2 are pairs' two halves, or, from rot on, copied
+  const bool pairs = kInterleaved || item * 16 < p.rot;
+  const int base = pairs ? item * kE : p.rot + (item - p.rot / 16) * kE, step = kInterleaved ? p.d / kV : pairs ? p.rot / kV : (p.d - p.rot) / kV;
+  X x[kRows];
   int token[kRows], head[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
@@ -236,17 +201,12 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_vector_kernel(const Rot
       const int h = head[u] - p.q_heads, kv = (int)p.cache.kv_heads;
       if (h >= 0) src = reinterpret_cast<const T*>(h < kv ? p.k + t * p.k_ldt + h * p.k_ldh : p.v + t * p.v_ldt + (h - kv) * p.v_ldh);
     }
-    x[u].load(src + lo, src + hi);
+#pragma unroll
+    for (int v = 0; v < kV; ++v) x[u].w[v] = *reinterpret_cast<const uint4*>(src + base + v * step);
   }
-  {
-    int tokens = divide(first + slots * kRows - 1, plan.heads) + 1;
-    if (tokens > p.tokens - t0) tokens = (int)(p.tokens - t0);
-    for (int i = threadIdx.x; i < tokens * half; i += kRotaryThreads) {
-      const int t = divide(i, plan.half);
-      table[i] = cos_sin(p, position_of(p, t0 + t), i - t * half);
-    }
-    if constexpr (kAppend)
-      for (int t = threadIdx.x; t < tokens; t += kRotaryThreads) entry[t] = entry_offset(p, t0 + t, 0);
+  for (int i = threadIdx.x; i < tokens * half; i += kRotaryThreads) {
+    const int t = divide(i, plan.half), pair = i - t * half;
+    table[t * plan.table + (pair & (kPairs - 1)) * plan.lanes + pair / kPairs] = cos_sin(p, position_of(p, t0 + t), pair);
   }
   __syncthreads();
 #pragma unroll
@@ -254,81 +214,93 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_vector_kernel(const Rot
     if (token[u] < 0) continue;
     const int64_t t = t0 + token[u];
     const int kv = kAppend ? (int)p.cache.kv_heads : 0, h = head[u] - p.q_heads;
-    const bool turned = !kAppend || h < kv;
-    if (turned && pairs) {
-      const float2* cs = table + token[u] * half + item * 8;
-      const Sixteen a = x[u].unpack();
-      Sixteen y = a;
-      const Vectors<T> was = x[u];
+    const bool turn = pairs && (!kAppend || h < kv);
+    const float2* cs = table + token[u] * plan.table;
+    // `put(v, e, a, b)` receives elements e and e + 1 of vector v, turned
+    auto turned = [&](auto put) {
+      const X y = x[u];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int i0 = kInterleaved ? 2 * i : i, i1 = kInterleaved ? 2 * i + 1 : i + 8;
-        if (!kInterleaved || item * 8 + i < half) {
-          const float2 c = cs[i];
-          y.v[i0] = fmaf(a.v[i0], c.x, -(a.v[i1] * c.y));
-          y.v[i1] = fmaf(a.v[i1], c.x, a.v[i0] * c.y);
+      for (int v = 0; v < (kInterleaved ? kV : kV / 2); ++v) {
+        const float2* c = cs + (base + v * step) / kE;
+#pragma unroll
+        for (int e = 0; e < kE; e += 2) {
+          if constexpr (kInterleaved) {
+            if (base + v * step + e >= p.rot) continue;  // copied: keeps its bits
+            const float2 c0 = c[e / 2 * plan.lanes];
+            const float a = y.get(v, e), b = y.get(v, e + 1);
+            put(v, e, fmaf(a, c0.x, -(b * c0.y)), fmaf(b, c0.x, a * c0.y));
+          } else {
+            const float2 c0 = c[e * plan.lanes], c1 = c[(e + 1) * plan.lanes];
+            const float a0 = y.get(v, e), b0 = y.get(v + kV / 2, e), a1 = y.get(v, e + 1), b1 = y.get(v + kV / 2, e + 1);
+            put(v, e, fmaf(a0, c0.x, -(b0 * c0.y)), fmaf(a1, c1.x, -(b1 * c1.y)));
+            put(v + kV / 2, e, fmaf(b0, c0.x, a0 * c0.y), fmaf(b1, c1.x, a1 * c1.y));
+          }
         }
       }
-      if (kAppend && h >= 0 && p.cache.dtype == TF_CACHE_E4M3) {
-        const int64_t at = entry[token[u]];
-        if (at < 0) continue;
-        const float s = p.cache.k_scale ? __frcp_rn(load_f32(p.cache.k_scale + h)) : 1.0f;
-        uint8_t* code = static_cast<uint8_t*>(p.cache.k) + at + h * p.cache.stride_head;
-        *reinterpret_cast<uint2*>(code + lo) =
-            make_uint2(cvt_e4m3x4(y.v[0] * s, y.v[1] * s, y.v[2] * s, y.v[3] * s), cvt_e4m3x4(y.v[4] * s, y.v[5] * s, y.v[6] * s, y.v[7] * s));
-        *reinterpret_cast<uint2*>(code + hi) =
-            make_uint2(cvt_e4m3x4(y.v[8] * s, y.v[9] * s, y.v[10] * s, y.v[11] * s), cvt_e4m3x4(y.v[12] * s, y.v[13] * s, y.v[14] * s, y.v[15] * s));
-        continue;
-      }
-      x[u].pack(y);
-      if constexpr (kInterleaved) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (item * 8 + i >= half) x[u].keep_pair(was, i);  // a copy keeps its bits
-      }
-    }
-    if (!kAppend || h < 0) {
-      if (!pairs && p.in_place) continue;
-      T* dst = reinterpret_cast<T*>(p.q_out) + t * p.qo_ldt + head[u] * p.qo_ldh;
-      x[u].store(dst + lo, dst + hi);
-    } else {
+    };
+    T* dst = reinterpret_cast<T*>(p.q_out) + t * p.qo_ldt + head[u] * p.qo_ldh;
+    if (kAppend && h >= 0) {
       const int64_t at = entry[token[u]];
       if (at < 0) continue;
       const int hh = h < kv ? h : h - kv;
-      uint8_t* to = static_cast<uint8_t*>(h < kv ? p.cache.k : p.cache.v);
-      if (p.cache.dtype == TF_CACHE_BF16) {
-        T* dst = reinterpret_cast<T*>(to + at) + hh * p.cache.stride_head;
-        x[u].store(dst + lo, dst + hi);
-      } else {
-        const float* scale = h < kv ? p.cache.k_scale : p.cache.v_scale;
-        const float s = scale ? __frcp_rn(load_f32(scale + hh)) : 1.0f;
-        const Sixteen y = x[u].unpack();
-        uint8_t* code = to + at + hh * p.cache.stride_head;
-        *reinterpret_cast<uint2*>(code + lo) =
-            make_uint2(cvt_e4m3x4(y.v[0] * s, y.v[1] * s, y.v[2] * s, y.v[3] * s), cvt_e4m3x4(y.v[4] * s, y.v[5] * s, y.v[6] * s, y.v[7] * s));
-        *reinterpret_cast<uint2*>(code + hi) =
-            make_uint2(cvt_e4m3x4(y.v[8] * s, y.v[9] * s, y.v[10] * s, y.v[11] * s), cvt_e4m3x4(y.v[12] * s, y.v[13] * s, y.v[14] * s, y.v[15] * s));
+      uint8_t* to = static_cast<uint8_t*>(h < kv ? p.cache.k : p.cache.v) + at;
+      if (p.cache.dtype == TF_CACHE_E4M3) {
+        const float* scales = h < kv ? p.cache.k_scale : p.cache.v_scale;
+        const float s = scales ? __frcp_rn(load_f32(scales + hh)) : 1.0f;
+        float y[kV][kE];
+#pragma unroll
+        for (int v = 0; v < kV; ++v)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) y[v][e] = x[u].get(v, e);
+        if (turn) turned([&](int v, int e, float a, float b) { y[v][e] = a, y[v][e + 1] = b; });
+#pragma unroll
+        for (int v = 0; v < kV; ++v) {
+          uint32_t codes[kE / 4];
+#pragma unroll
+          for (int e = 0; e < kE; e += 4) codes[e / 4] = cvt_e4m3x4(y[v][e] * s, y[v][e + 1] * s, y[v][e + 2] * s, y[v][e + 3] * s);
+          if constexpr (kE == 8) *reinterpret_cast<uint2*>(to + hh * p.cache.stride_head + base + v * step) = make_uint2(codes[0], codes[1]);
+        }
+        continue;
       }
+      dst = reinterpret_cast<T*>(to) + hh * p.cache.stride_head;
+    } else if (!pairs && p.in_place) {
+      continue;
     }
+    if (turn) turned([&](int v, int e, float a, float b) { x[u].set2(v, e, a, b); });
+#pragma unroll
+    for (int v = 0; v < kV; ++v) *reinterpret_cast<uint4*>(dst + base + v * step) = x[u].w[v];
   }
 }
 
-template <typename T, bool kAppend, int kRows>
-static tf_status launch_rotary_vectors(const RotaryArgs& p, cudaStream_t stream) {
-  VectorPlan plan = {};
-  plan.items = p.d / 16;
-  while ((1 << plan.lanes_log2) < plan.items) ++plan.lanes_log2;
+template <typename T, bool kAppend, int kRows, int kBlocks>
+static tf_status launch_rotary_rows(const RotaryArgs& p, VectorPlan plan, cudaStream_t stream) {
   plan.heads = divisor(p.heads);
   plan.half = divisor(p.rot > 0 ? p.rot / 2 : 1);
   const int rows = (kRotaryThreads >> plan.lanes_log2) * kRows;
   plan.max_tokens = (rows + p.heads - 2) / p.heads + 1;
   const int64_t blocks = (p.tokens * p.heads + rows - 1) / rows;
   if (blocks > INT32_MAX) return fail(TF_ERR_UNSUPPORTED, "%s: %lld rows are too many", __func__, (long long)(p.tokens * p.heads));
-  const size_t smem = (size_t)plan.max_tokens * ((size_t)p.rot / 2 * sizeof(float2) + (kAppend ? sizeof(int64_t) : 0));
-  auto kernel = p.interleaved ? rotary_vector_kernel<T, kAppend, true, kRows> : rotary_vector_kernel<T, kAppend, false, kRows>;
+  const int per = Vectors<T>::kElems / (p.interleaved ? 2 : 1);
+  plan.lanes = (p.rot / 2 + per - 1) / per;
+  plan.table = per * plan.lanes;
+  const size_t smem = (size_t)plan.max_tokens * (plan.table * sizeof(float2) + (kAppend ? sizeof(int64_t) : 0));
+  auto kernel = p.interleaved ? rotary_vector_kernel<T, kAppend, true, kRows, kBlocks> : rotary_vector_kernel<T, kAppend, false, kRows, kBlocks>;
   kernel<<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(p, plan);
   TF_LAUNCH_CHECK();
   return TF_OK;
+}
+
+// Two rows a thread keep the loads of a long call in flight (8192 x 64 x 128 bf16: 41.2 us with five blocks an SM, 43.2 with four; one row 42.3 to 54); a
+// call that two rows would not spread over two blocks an SM takes one (64 tokens of 80 heads into a cache 3.2 -> 2.9 us). The append kernel
+// spills at five blocks and the f32 one is slower (5.3 us at four for 1777 x 20 x 80, 6.8 at five).
+template <typename T, bool kAppend>
+static tf_status launch_rotary_vectors(const RotaryArgs& p, cudaStream_t stream) {
+  VectorPlan plan = {};
+  plan.items = p.d / 16;
+  while ((1 << plan.lanes_log2) < plan.items) ++plan.lanes_log2;
+  const int64_t two = (int64_t)(kRotaryThreads >> plan.lanes_log2) * 2;
+  if (p.tokens * p.heads <= two * 2 * sm_count()) return launch_rotary_rows<T, kAppend, 1, sizeof(T) == 2 ? 6 : 4>(p, plan, stream);
+  return launch_rotary_rows<T, kAppend, 2, !kAppend && sizeof(T) == 2 ? 5 : kAppend ? 3 : 4>(p, plan, stream);
 }
 
 template <typename T, bool kAppend>
@@ -337,7 +309,7 @@ static tf_status launch_rotary(const RotaryArgs& p, cudaStream_t stream) {
   const int64_t unit = 16 / (int64_t)sizeof(T);
   auto aligned = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && a % unit == 0 && b % unit == 0; };
   if (p.d % 16 == 0 && (p.interleaved || p.rot % 16 == 0) && aligned(p.q, p.q_ldt, p.q_ldh) && aligned(p.q_out, p.qo_ldt, p.qo_ldh))
-    return launch_rotary_vectors<T, kAppend, 2>(p, stream);
+    return launch_rotary_vectors<T, kAppend>(p, stream);
   const int64_t total = p.tokens * p.heads * (p.d - p.rot / 2), cap = (int64_t)sm_count() * 8;
   const int64_t need = (total + kRotaryThreads - 1) / kRotaryThreads;
   rotary_kernel<T, kAppend><<<(unsigned)(need < cap ? need : cap), kRotaryThreads, 0, stream>>>(p);
@@ -411,7 +383,10 @@ extern "C" tf_status tf_cache_append(const tf_paged_cache* cache, const void* k,
   p.k = static_cast<const __nv_bfloat16*>(k), p.k_ldt = k_stride_token, p.k_ldh = k_stride_head;
   p.v = static_cast<const __nv_bfloat16*>(v), p.v_ldt = v_stride_token, p.v_ldh = v_stride_head;
   p.cache = *cache;
-  p.tables = tables, p.table_rows = table_rows, p.table_cols = table_cols, p.table_stride = table_stride;
+  // no sequence has more than 2^30 entries
+  const int64_t most = INT32_MAX / 2, page = cache->page_size > most ? most : cache->page_size;
+  p.tables = tables, p.table_rows = table_rows, p.table_stride = table_stride;
+  p.entries = (int)(table_cols > most / page ? most : table_cols * page), p.page = divisor((int)page);
   p.rows = rows, p.tokens_per_row = rows ? 1 : tokens / table_rows;
   p.positions = positions, p.wide_positions = position_bits == 64;
   p.turns = turns, p.magnitude = magnitude, p.interleaved = layout == TF_ROTARY_INTERLEAVED;
