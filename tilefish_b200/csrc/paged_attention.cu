@@ -1,39 +1,45 @@
-// The entry points of attention over a paged key-value cache. The kernels are in paged_attention.cuh, built by head size in paged_attention_d*.cu.
+// The entry points of attention over a paged key-value cache. The kernels are in paged_attention.cuh, built by head size in paged_attention_<type>_d<size>.cu.
 #include <type_traits>
 
 #include "paged_attention.cuh"
 
 namespace tf {
 
-extern template struct AttendCall<64, false, 1>;
-extern template struct AttendCall<64, false, 2>;
-extern template struct AttendCall<64, false, 4>;
-extern template struct AttendCall<64, true, 1>;
-extern template struct AttendCall<64, true, 2>;
-extern template struct AttendCall<64, true, 4>;
-extern template struct AttendCall<128, false, 1>;
-extern template struct AttendCall<128, false, 2>;
-extern template struct AttendCall<128, false, 4>;
-extern template struct AttendCall<128, true, 1>;
-extern template struct AttendCall<128, true, 2>;
-extern template struct AttendCall<128, true, 4>;
-extern template struct AttendCall<256, false, 1>;
-extern template struct AttendCall<256, false, 2>;
-extern template struct AttendCall<256, false, 4>;
-extern template struct AttendCall<256, true, 1>;
-extern template struct AttendCall<256, true, 2>;
-extern template struct AttendCall<256, true, 4>;
+extern template struct AttendCall<64, false, 8>;
+extern template struct AttendCall<64, false, 16>;
+extern template struct AttendCall<64, false, 32>;
+extern template struct AttendCall<64, false, 64>;
+extern template struct AttendCall<64, true, 8>;
+extern template struct AttendCall<64, true, 16>;
+extern template struct AttendCall<64, true, 32>;
+extern template struct AttendCall<64, true, 64>;
+extern template struct AttendCall<128, false, 8>;
+extern template struct AttendCall<128, false, 16>;
+extern template struct AttendCall<128, false, 32>;
+extern template struct AttendCall<128, false, 64>;
+extern template struct AttendCall<128, true, 8>;
+extern template struct AttendCall<128, true, 16>;
+extern template struct AttendCall<128, true, 32>;
+extern template struct AttendCall<128, true, 64>;
+extern template struct AttendCall<256, false, 8>;
+extern template struct AttendCall<256, false, 16>;
+extern template struct AttendCall<256, false, 32>;
+extern template struct AttendCall<256, false, 64>;
+extern template struct AttendCall<256, true, 8>;
+extern template struct AttendCall<256, true, 16>;
+extern template struct AttendCall<256, true, 32>;
+extern template struct AttendCall<256, true, 64>;
 
-// 16 rows per warp: a team of as many warps as the rows of a kv head need, up to four.
+// As few rows as hold a kv head's query heads times the new tokens, up to 64; more are several tiles.
 template <class Use>
 static auto with_attend_call(int64_t rows, int64_t d, int32_t dtype, Use use) {
-  auto by_team = [&](auto dp, auto f8) {
+  auto by_rows = [&](auto dp, auto f8) {
     constexpr int kDP = decltype(dp)::value;
     constexpr bool kF8 = decltype(f8)::value;
-    return rows <= 16 ? use(AttendCall<kDP, kF8, 1>{}) : rows <= 32 ? use(AttendCall<kDP, kF8, 2>{}) : use(AttendCall<kDP, kF8, 4>{});
+    return rows <= 8 ? use(AttendCall<kDP, kF8, 8>{}) : rows <= 16 ? use(AttendCall<kDP, kF8, 16>{}) : rows <= 32 ? use(AttendCall<kDP, kF8, 32>{}) : use(AttendCall<kDP, kF8, 64>{});
   };
   auto by_dim = [&](auto f8) {
-    return d <= 64 ? by_team(std::integral_constant<int, 64>{}, f8) : d <= 128 ? by_team(std::integral_constant<int, 128>{}, f8) : by_team(std::integral_constant<int, 256>{}, f8);
+    return d <= 64 ? by_rows(std::integral_constant<int, 64>{}, f8) : d <= 128 ? by_rows(std::integral_constant<int, 128>{}, f8) : by_rows(std::integral_constant<int, 256>{}, f8);
   };
   return dtype == TF_CACHE_E4M3 ? by_dim(std::true_type{}) : by_dim(std::false_type{});
 }

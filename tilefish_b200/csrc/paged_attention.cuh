@@ -49,12 +49,14 @@ struct AttendArgs {
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
 constexpr int kMaxAttendBlocks = 1024;
 
-template <int DP, bool F8, int TEAM>
+// ROWS query rows of a kv head: 8 or 16 by a warp of its own, 32 or 64 by a team of two or four.
+template <int DP, bool F8, int ROWS>
 struct AttendCfg {
-  static constexpr int kTeams = kAttendWarps / TEAM, kRows = 16 * TEAM;
+  static constexpr int kTeam = ROWS <= 16 ? 1 : ROWS / 16, kTeams = kAttendWarps / kTeam, kRows = ROWS;
+  static constexpr int kHalves = ROWS == 8 ? 1 : 2;  // a thread has rows r and r + 8 of the 16; with 8 rows the operand's other half is zero
   static constexpr int kRowBytes = DP * (F8 ? 1 : 2);
-  static constexpr int kKeys = kRowBytes >= (TEAM == 1 ? 256 : 512) ? 16 : 32;  // of a team's tile
-  static constexpr int kLoadRows = kKeys / TEAM;                                // of them, a warp loads
+  static constexpr int kKeys = kRowBytes >= (kTeam == 1 ? 256 : 512) ? 16 : 32;  // of a team's tile
+  static constexpr int kLoadRows = kKeys / kTeam;                               // of them, a warp loads
   static constexpr int kUnit = kKeys * kTeams;
   static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
   static constexpr int kFit = 65536 / (kTeams * 2 * kHalf);
@@ -63,6 +65,8 @@ struct AttendCfg {
   static constexpr int kPitch = DP + 8;  // floats of a row that is joined: rows start in other banks
   static constexpr int kJoin = kTeams * kRows * kPitch * 4;
   static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kChunks = kRowBytes / 16;      // of a staged row
+  static constexpr int kRowsPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
   static constexpr int kBlocksPerSm = DP <= 128 ? 3 : F8 ? 2 : 1;
   // an e4m3 entry is multiplied as f16: weights are scaled by 2^15 (the largest is 2^15), so that small ones keep their bits
   static constexpr float kShift = F8 ? 15.0f : 0.0f;
@@ -169,13 +173,14 @@ __device__ __forceinline__ long long block_sum(long long x, long long* scratch) 
   return scratch[0] + scratch[1] + scratch[2] + scratch[3];
 }
 
-template <int DP, bool F8, int TEAM>
-__global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlocksPerSm)) paged_attention_kernel(const AttendArgs p) {
-  using C = AttendCfg<DP, F8, TEAM>;
-  extern __shared__ __align__(128) uint8_t smem[];
+template <int DP, bool F8, int ROWS>
+__global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlocksPerSm)) paged_attention_kernel(const AttendArgs p) {
+  using C = AttendCfg<DP, F8, ROWS>;
+  constexpr int TEAM = C::kTeam, kHalves = C::kHalves;
+  extern __shared__ __align__(1024) uint8_t smem[];  // rows of the ring start on multiples of their size
   __shared__ long long s_scratch[kAttendWarps], s_before;
   __shared__ int s_index;
-  __shared__ uint32_t s_seen[kAttendWarps / TEAM][C::kStages][TEAM];
+  __shared__ uint32_t s_seen[C::kTeams][C::kStages][TEAM];
   __shared__ float2 s_stats[C::kTeams * C::kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / TEAM, member = warp % TEAM;
 
@@ -215,12 +220,15 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
   __syncthreads();
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + team * C::kStages * 2 * C::kHalf;
-  constexpr int kChunks = C::kRowBytes / 16;      // of a staged row
-  constexpr int kRowsPerCopy = 32 / kChunks;      // rows that one copy instruction of a warp covers
-  const int chunks = p.d * (F8 ? 1 : 2) / 16;     // that hold data
-  const int copy_row = lane / kChunks, copy_chunk = lane % kChunks;
-  // chunk c of row r lies at c ^ swizzle(r): the eight rows of a matrix load are in other banks
+  const int chunks = p.d * (F8 ? 1 : 2) / 16;  // of a staged row, that hold data
+  const int copy_row = lane / C::kChunks, copy_chunk = lane % C::kChunks;
+  // Chunk c of row r lies at c ^ swizzle(r): the eight rows of a matrix load are in other banks. Rows start on multiples of their size, so a
+  // step to another chunk, and to a row of the same instruction's series, is an exclusive or with a constant.
   auto swizzle = [](int row) { return C::kRowBytes >= 128 ? row & 7 : (row >> 1) & 3; };
+  const uint32_t copy_to = (member * C::kLoadRows + copy_row) * C::kRowBytes + ((copy_chunk ^ swizzle(member * C::kLoadRows + copy_row)) << 4);
+  const int k_row = F8 ? (lane & 7) + (lane & 8) : (lane & 7) + ((lane >> 4) << 3), v_row = (lane & 7) + (lane & 8);
+  const uint32_t k_from = k_row * C::kRowBytes + (((F8 ? lane >> 4 : (lane >> 3) & 1) ^ swizzle(k_row)) << 4);
+  const uint32_t v_from = v_row * C::kRowBytes + (((lane >> 4) ^ swizzle(v_row)) << 4);
 
   int index = s_index;
   long long before = s_before;
@@ -254,14 +262,15 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
         const uint32_t seen = __ballot_sync(~0u, ok);
         const int stage = tile % C::kStages;
         if (lane == 0) s_seen[team][stage][member] = seen;
-        const uint32_t to = ring + stage * 2 * C::kHalf;
+        const uint32_t to = ring + stage * 2 * C::kHalf + copy_to;
 #pragma unroll
-        for (int i = 0; i < (C::kLoadRows + kRowsPerCopy - 1) / kRowsPerCopy; ++i) {
-          const int r = i * kRowsPerCopy + copy_row;  // of this warp's rows
+        for (int i = 0; i < (C::kLoadRows + C::kRowsPerCopy - 1) / C::kRowsPerCopy; ++i) {
+          const int r = i * C::kRowsPerCopy + copy_row;  // of this warp's rows
           const int64_t o = __shfl_sync(~0u, off, r & 31);
-          const int row = member * C::kLoadRows + r, bytes = (seen >> (r & 31)) & 1 ? 16 : 0;
-          if (r < C::kLoadRows && copy_chunk < chunks) {
-            const uint32_t dst = to + row * C::kRowBytes + ((copy_chunk ^ swizzle(row)) << 4);
+          const int bytes = (seen >> (r & 31)) & 1 ? 16 : 0;
+          if (C::kLoadRows % C::kRowsPerCopy && r >= C::kLoadRows) continue;
+          if (copy_chunk < chunks) {
+            const uint32_t dst = (to ^ (swizzle(i * C::kRowsPerCopy) << 4)) + i * C::kRowsPerCopy * C::kRowBytes;
             copy_async(dst, kbase + o + copy_chunk * 16, bytes);
             copy_async(dst + C::kHalf, vbase + o + copy_chunk * 16, bytes);
           }
@@ -270,15 +279,28 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
       }
       copy_commit();
     };
+    if (p.d < DP) {
+      // the products run over DP elements: the keys' others are zero, as the queries' are (the values' give columns that nobody reads)
+      for (int i = lane; i < C::kStages * C::kKeys / TEAM * C::kChunks; i += 32) {
+        const int ch = i % C::kChunks, r = i / C::kChunks * TEAM + member, row = r % C::kKeys;
+        if (ch >= chunks)
+          *reinterpret_cast<uint4*>(smem + team * C::kStages * 2 * C::kHalf + r / C::kKeys * 2 * C::kHalf + row * C::kRowBytes + ((ch ^ swizzle(row)) << 4)) =
+              make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < C::kStages - 1; ++i) issue(i);
 
     // this thread's two rows: the query operand, scale and limits
     uint32_t qf[DP / 16][4];
-    float row_scale[2];
-    int limit[2], lowest[2];
+    float row_scale[kHalves];
+    int limit[kHalves], lowest[kHalves];
+    if constexpr (kHalves == 1) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int kk = 0; kk < DP / 16; ++kk) qf[kk][1] = qf[kk][3] = 0u;
+    }
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
       const int r = row0 + member * 16 + (lane >> 2) + 8 * h, i = divide(r, p.group);
       const bool real = r < p.queries * p.group.d;
       limit[h] = real && i < sp.count ? sp.length - sp.count + 1 + i : 0;
@@ -315,7 +337,9 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
         row_scale[h] = row_scale[h] * (p.k_scale ? load_f32(p.k_scale + kv) : 1.0f) * ia * ic;
       }
     }
-    float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float o[DP / 8][4], m[kHalves], l[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) m[h] = -INFINITY, l[h] = 0.0f;
 #pragma unroll
     for (int j = 0; j < DP / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
 
@@ -332,57 +356,45 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
       float s[C::kKeys / 8][4];
 #pragma unroll
       for (int j = 0; j < C::kKeys / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-      if constexpr (F8) {
-        const int row = (lane & 7) + (lane & 8), sw = swizzle(row);
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; kk += 2) {
-          if (kk * 16 >= p.d) break;
+      for (int kk = 0; kk < DP / 16; kk += F8 ? 2 : 1)
 #pragma unroll
-          for (int j = 0; j < C::kKeys / 16; ++j) {
-            uint32_t r[4];
-            load_matrices(r, kt + (j * 16 + row) * C::kRowBytes + (((kk + (lane >> 4)) ^ sw) << 4));
+        for (int j = 0; j < C::kKeys / 16; ++j) {
+          uint32_t r[4];
+          load_matrices(r, ((kt + k_from) ^ (kk << (F8 ? 4 : 5))) + j * 16 * C::kRowBytes);
+          if constexpr (F8) {
             multiply<true>(s[2 * j], qf[kk], codes_to_f16x2(r[0], false), codes_to_f16x2(r[0], true));
             multiply<true>(s[2 * j + 1], qf[kk], codes_to_f16x2(r[1], false), codes_to_f16x2(r[1], true));
-            if ((kk + 1) * 16 < p.d) {
-              multiply<true>(s[2 * j], qf[kk + 1], codes_to_f16x2(r[2], false), codes_to_f16x2(r[2], true));
-              multiply<true>(s[2 * j + 1], qf[kk + 1], codes_to_f16x2(r[3], false), codes_to_f16x2(r[3], true));
-            }
-          }
-        }
-      } else {
-        const int row = (lane & 7) + ((lane >> 4) << 3), sw = swizzle(row), half = (lane >> 3) & 1;
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          if (kk * 16 >= p.d) break;
-#pragma unroll
-          for (int j = 0; j < C::kKeys / 16; ++j) {
-            uint32_t r[4];
-            load_matrices(r, kt + (j * 16 + row) * C::kRowBytes + (((2 * kk + half) ^ sw) << 4));
+            multiply<true>(s[2 * j], qf[kk + 1], codes_to_f16x2(r[2], false), codes_to_f16x2(r[2], true));
+            multiply<true>(s[2 * j + 1], qf[kk + 1], codes_to_f16x2(r[3], false), codes_to_f16x2(r[3], true));
+          } else {
             multiply<false>(s[2 * j], qf[kk], r[0], r[1]);
             multiply<false>(s[2 * j + 1], qf[kk], r[2], r[3]);
           }
         }
-      }
 
       const bool whole = seen == (uint32_t)((1ull << C::kKeys) - 1);
       const bool inside = key >= sp.last_lo && key + C::kKeys <= sp.first;  // every row sees all of the tile's keys that anyone sees
-      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < C::kKeys / 8; ++j)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          float y = s[j][x] * row_scale[x >> 1];
-          if (!(whole && inside)) {
+        for (int x = 0; x < 2 * kHalves; ++x) s[j][x] *= row_scale[x >> 1];
+      if (!(whole && inside)) {
+#pragma unroll
+        for (int j = 0; j < C::kKeys / 8; ++j)
+#pragma unroll
+          for (int x = 0; x < 2 * kHalves; ++x) {
             const int c = 8 * j + 2 * (lane & 3) + (x & 1), e = key + c;
-            if (!((seen >> c) & 1) || e < lowest[x >> 1] || e >= limit[x >> 1]) y = -INFINITY;
+            if (!((seen >> c) & 1) || e < lowest[x >> 1] || e >= limit[x >> 1]) s[j][x] = -INFINITY;
           }
-          s[j][x] = y;
-          top[x >> 1] = fmaxf(top[x >> 1], y);
-        }
-      float base[2];
+      }
+      float top[kHalves], base[kHalves];
       bool moved = false;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kHalves; ++h) {
+        top[h] = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+#pragma unroll
+        for (int j = 1; j < C::kKeys / 8; ++j) top[h] = fmaxf(top[h], fmaxf(s[j][2 * h], s[j][2 * h + 1]));
         top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
         top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
         top[h] = fmaxf(top[h], m[h]);
@@ -390,26 +402,24 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
         moved |= top[h] != m[h];
       }
       if (__any_sync(~0u, moved)) {
-        float keep[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          keep[h] = exp2_approx(m[h] - base[h]);
-          l[h] *= keep[h];
+        for (int h = 0; h < kHalves; ++h) {
+          const float keep = exp2_approx(m[h] - base[h]);
+          l[h] *= keep;
           m[h] = top[h];
-        }
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j) {
-          o[j][0] *= keep[0], o[j][1] *= keep[0];
-          o[j][2] *= keep[1], o[j][3] *= keep[1];
+          for (int j = 0; j < DP / 8; ++j) o[j][2 * h] *= keep, o[j][2 * h + 1] *= keep;
         }
       }
 #pragma unroll
-      for (int j = 0; j < C::kKeys / 8; ++j)
+      for (int h = 0; h < kHalves; ++h) {
+        const float shift = C::kShift - base[h];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          s[j][x] = exp2_approx(s[j][x] - base[x >> 1] + C::kShift);
-          l[x >> 1] += s[j][x];
+        for (int j = 0; j < C::kKeys / 8; ++j) {
+          s[j][2 * h] = exp2_approx(s[j][2 * h] + shift), s[j][2 * h + 1] = exp2_approx(s[j][2 * h + 1] + shift);
+          l[h] += s[j][2 * h] + s[j][2 * h + 1];
         }
+      }
 
       // A value that some rows see and others do not reaches both through the product, the latter with weight 0: harmless unless it is not finite.
       bool odd = false;
@@ -432,10 +442,11 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
       if (!odd) {
 #pragma unroll
         for (int j = 0; j < C::kKeys / 16; ++j) {
-          uint32_t hi[4];
-          [[maybe_unused]] uint32_t lo[4];
+          uint32_t hi[4] = {0u, 0u, 0u, 0u};
+          [[maybe_unused]] uint32_t lo[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
           for (int x = 0; x < 4; ++x) {  // the scores' registers are the weights' operand: keys 2c, 2c + 1 and 2c + 8, 2c + 9 of rows r and r + 8
+            if (kHalves == 1 && (x & 1)) continue;
             const float a = s[2 * j + (x >> 1)][2 * (x & 1)], c = s[2 * j + (x >> 1)][2 * (x & 1) + 1];
             if constexpr (F8) {
               hi[x] = pack_f16x2(a, c);
@@ -445,32 +456,22 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
               lo[x] = pack_bf16x2(a - bf16lo_to_f32(hi[x]), c - bf16hi_to_f32(hi[x]));
             }
           }
-          const int row = (lane & 7) + (lane & 8), sw = swizzle(row);
-          const uint32_t at = vt + (j * 16 + row) * C::kRowBytes;
-          if constexpr (F8) {
 #pragma unroll
-            for (int t = 0; t < DP / 16; t += 2) {
-              if (t * 16 >= p.d) break;
-              uint32_t r[4];
-              load_matrices_turned(r, at + (((t + (lane >> 4)) ^ sw) << 4));
+          for (int t = 0; t < DP / 16; t += F8 ? 2 : 1) {
+            uint32_t r[4];
+            load_matrices_turned(r, ((vt + v_from) ^ (t << (F8 ? 4 : 5))) + j * 16 * C::kRowBytes);
+            if constexpr (F8) {
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                if ((t + x) * 16 >= p.d) break;
                 // a thread holds elements (2c', 2c' + 1) of two keys: bytes to (key, key + 1) pairs, the even elements in one product, the odd ones in another
                 const uint32_t w0 = __byte_perm(r[2 * x], 0, 0x3120), w1 = __byte_perm(r[2 * x + 1], 0, 0x3120);
                 multiply<true>(o[2 * (t + x)], hi, codes_to_f16x2(w0, false), codes_to_f16x2(w1, false));
                 multiply<true>(o[2 * (t + x) + 1], hi, codes_to_f16x2(w0, true), codes_to_f16x2(w1, true));
               }
-            }
-          } else {
-#pragma unroll
-            for (int t = 0; t < DP / 16; ++t) {
-              if (t * 16 >= p.d) break;
-              uint32_t r[4];
-              load_matrices_turned(r, at + (((2 * t + (lane >> 4)) ^ sw) << 4));
+            } else {
               multiply<false>(o[2 * t], hi, r[0], r[1]);
-              multiply<false>(o[2 * t], lo, r[0], r[1]);
               multiply<false>(o[2 * t + 1], hi, r[2], r[3]);
+              multiply<false>(o[2 * t], lo, r[0], r[1]);
               multiply<false>(o[2 * t + 1], lo, r[2], r[3]);
             }
           }
@@ -482,10 +483,10 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
 #pragma unroll 1
           for (int x8 = 0; x8 < 8; ++x8) {
             const int c = 8 * eight + x8;
-            float w[2];
-            bool sees[2];
+            float w[kHalves];
+            bool sees[kHalves];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kHalves; ++h) {
               const float w0 = s[eight][2 * h], w1 = s[eight][2 * h + 1];
               w[h] = __shfl_sync(~0u, x8 & 1 ? w1 : w0, (lane & ~3) | (x8 >> 1));
               sees[h] = ((seen >> c) & 1) && key + c >= lowest[h] && key + c < limit[h];
@@ -495,12 +496,11 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
                 const int e = F8 ? (j >> 1) * 16 + 4 * (lane & 3) + 2 * x + (j & 1) : j * 8 + 2 * (lane & 3) + x, byte = F8 ? e : 2 * e;
-                if (e < p.d) {
-                  const uint8_t* from = values + c * C::kRowBytes + (((byte >> 4) ^ swizzle(c)) << 4) + (byte & 15);
-                  const float y = F8 ? e4m3_to_f32(*from) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(from));
-                  if (sees[0]) o[j][x] = fmaf(w[0], y, o[j][x]);
-                  if (sees[1]) o[j][2 + x] = fmaf(w[1], y, o[j][2 + x]);
-                }
+                const uint8_t* from = values + c * C::kRowBytes + (((byte >> 4) ^ swizzle(c)) << 4) + (byte & 15);
+                const float y = F8 ? e4m3_to_f32(*from) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(from));
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+                  if (sees[h]) o[j][2 * h + x] = fmaf(w[h], y, o[j][2 * h + x]);
               }
           }
       }
@@ -511,21 +511,18 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, TEAM>::kBlo
     __syncthreads();  // the ring is free
     float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kHalves; ++h) {
       l[h] += __shfl_xor_sync(~0u, l[h], 1);
       l[h] += __shfl_xor_sync(~0u, l[h], 2);
       const int r = team * C::kRows + member * 16 + (lane >> 2) + 8 * h;
       if ((lane & 3) == 0) s_stats[r] = make_float2(m[h], l[h]);
+      float* row = sums + r * C::kPitch;
 #pragma unroll
-      for (int j = 0; j < DP / 8; ++j) {
-        if constexpr (F8) {
-          if (j & 1) continue;
-          const int e = (j >> 1) * 16 + 4 * (lane & 3);
-          if (e < p.d) *reinterpret_cast<float4*>(sums + r * C::kPitch + e) = make_float4(o[j][2 * h], o[j + 1][2 * h], o[j][2 * h + 1], o[j + 1][2 * h + 1]);
-        } else {
-          const int e = j * 8 + 2 * (lane & 3);
-          if (e < p.d) *reinterpret_cast<float2*>(sums + r * C::kPitch + e) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
-        }
+      for (int j = 0; j < DP / 8; j += F8 ? 2 : 1) {
+        if constexpr (F8)
+          *reinterpret_cast<float4*>(row + j * 8 + 4 * (lane & 3)) = make_float4(o[j][2 * h], o[j + 1][2 * h], o[j][2 * h + 1], o[j + 1][2 * h + 1]);
+        else
+          *reinterpret_cast<float2*>(row + j * 8 + 2 * (lane & 3)) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
       }
     }
     __syncthreads();
@@ -660,23 +657,23 @@ __global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(co
 }
 
 // Blocks of a call: as many as fit the device at once, or one per unit where the table cannot name more.
-template <int DP, bool F8, int TEAM>
+template <int DP, bool F8, int ROWS>
 static int attend_blocks(int64_t spans, int64_t kv_heads, int64_t entries) {
-  using C = AttendCfg<DP, F8, TEAM>;
+  using C = AttendCfg<DP, F8, ROWS>;
   int64_t cap = (int64_t)sm_count() * C::kBlocksPerSm;
   if (cap > kMaxAttendBlocks) cap = kMaxAttendBlocks;
   const int64_t heads = spans * kv_heads, each = (entries + C::kUnit - 1) / C::kUnit;
   return (int)(heads >= cap || each >= cap || heads * each >= cap ? cap : heads * each);
 }
 
-template <int DP, bool F8, int TEAM>
+template <int DP, bool F8, int ROWS>
 struct AttendCall {
-  using C = AttendCfg<DP, F8, TEAM>;
+  using C = AttendCfg<DP, F8, ROWS>;
   static int64_t workspace(int64_t spans, int64_t kv_heads, int64_t d, int64_t entries) {
-    return 2 * (int64_t)attend_blocks<DP, F8, TEAM>(spans, kv_heads, entries) * C::kRows * (d + 2) * 4;
+    return 2 * (int64_t)attend_blocks<DP, F8, ROWS>(spans, kv_heads, entries) * C::kRows * (d + 2) * 4;
   }
   static tf_status launch(AttendArgs p, void* workspace, cudaStream_t stream) {
-    auto kernel = paged_attention_kernel<DP, F8, TEAM>;
+    auto kernel = paged_attention_kernel<DP, F8, ROWS>;
     static thread_local int configured_dev = -1;
     int dev = 0;
     TF_CUDA(cudaGetDevice(&dev));
@@ -684,7 +681,7 @@ struct AttendCall {
       TF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
       configured_dev = dev;
     }
-    const int blocks = attend_blocks<DP, F8, TEAM>(p.spans, p.kv_heads, p.entries);
+    const int blocks = attend_blocks<DP, F8, ROWS>(p.spans, p.kv_heads, p.entries);
     p.part_sums = static_cast<float*>(workspace);
     p.part_stats = reinterpret_cast<float2*>(p.part_sums + 2 * (int64_t)blocks * C::kRows * p.d);
     kernel<<<blocks, kAttendThreads, C::kSmem, stream>>>(p);
