@@ -4,13 +4,14 @@
 // keys stream through once. Bound by HBM: a bf16 key and value of 128 elements are 512 bytes for 4 * 128 operations per row, 24 bytes a clock
 // and SM, while 16 rows use about a tenth of the tensor cores and of the issue slots.
 //
-// One pass with a running maximum and sum (base 2, f32). Each warp (or team of 2 or 4 warps with 16 rows each, where there are more than 16
-// rows) has a ring of its own in shared memory, filled by cp.async: a tile's wait is a warp's wait, never the block's. The four warps of a block are
-// joined through shared memory at the end of a segment.
+// One pass with a running maximum and sum (base 2, f32). The workers are single warps, or teams of 2 or 4 warps with 16 rows each where there are
+// more than 16 rows. Each has a ring of its own in shared memory, filled by cp.async, and never waits for another: while one waits for a
+// head's first keys, the others of its SM keep the memory busy.
 //
-// The work is the list of all (sequence, row tile, kv head, unit of keys), cut into as many equal contiguous ranges as there are blocks, whatever
-// the lengths are (they are read on the device, so a captured call follows them). A block writes the result of a head whose keys it has seen
-// all of; of others it leaves its maximum, sum and unnormalised sum of values in the workspace, and paged_attention_join_kernel adds them up in the order of the keys.
+// The work is the list of all (sequence, row tile, kv head), each as long as its tiles of keys and a fixed part for starting it, cut into as many
+// equal contiguous ranges as there are workers, whatever the lengths are (they are read on the device, so a captured call follows them). A worker
+// that has seen all keys of a head writes its result. Else it leaves its maximum, sum and unnormalised sum of values in the workspace, and
+// paged_attention_join_kernel adds them up in the order of the keys.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -42,12 +43,13 @@ struct AttendArgs {
   int queries, q_heads, row_tiles, window;
   Divisor group;
   float scale_log2;
-  float* part_sums;   // [slots][rows][d]
-  float2* part_stats; // [slots][rows]: maximum, sum
+  float* part_sums;    // [2 * workers][rows][d]: of a worker's first head, and of its last
+  float2* part_stats;  // [2 * workers][rows]: maximum, sum
+  int4* shares;        // [spans * kv_heads]: the first and the last worker of a head, and the first one's slot
 };
 
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
-constexpr int kMaxAttendBlocks = 1024;
+constexpr int kHeadCost = 1;  // what starting a head costs a worker, in tiles: about the latency of its first keys
 
 // ROWS query rows of a kv head: 8 or 16 by a warp of its own, 32 or 64 by a team of two or four.
 template <int DP, bool F8, int ROWS>
@@ -57,14 +59,10 @@ struct AttendCfg {
   static constexpr int kRowBytes = DP * (F8 ? 1 : 2);
   static constexpr int kKeys = kRowBytes >= (kTeam == 1 ? 256 : 512) ? 16 : 32;  // of a team's tile
   static constexpr int kLoadRows = kKeys / kTeam;                               // of them, a warp loads
-  static constexpr int kUnit = kKeys * kTeams;
   static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
   static constexpr int kFit = 65536 / (kTeams * 2 * kHalf);
   static constexpr int kStages = kFit < 2 ? 2 : kFit > 4 ? 4 : kFit;
-  static constexpr int kRing = kTeams * kStages * 2 * kHalf;
-  static constexpr int kPitch = DP + 8;  // floats of a row that is joined: rows start in other banks
-  static constexpr int kJoin = kTeams * kRows * kPitch * 4;
-  static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kSmem = kTeams * kStages * 2 * kHalf;
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
   static constexpr int kRowsPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
   static constexpr int kBlocksPerSm = DP <= 128 ? 3 : F8 ? 2 : 1;
@@ -95,11 +93,11 @@ __device__ __forceinline__ void load_matrices_turned(uint32_t (&r)[4], uint32_t 
 template <bool F16>
 __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (F16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -178,46 +176,69 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
   using C = AttendCfg<DP, F8, ROWS>;
   constexpr int TEAM = C::kTeam, kHalves = C::kHalves;
   extern __shared__ __align__(1024) uint8_t smem[];  // rows of the ring start on multiples of their size
-  __shared__ long long s_scratch[kAttendWarps], s_before;
-  __shared__ int s_index;
+  __shared__ long long s_scratch[kAttendWarps], s_before[C::kTeams];
+  __shared__ int s_index[C::kTeams];
   __shared__ uint32_t s_seen[C::kTeams][C::kStages][TEAM];
-  __shared__ float2 s_stats[C::kTeams * C::kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / TEAM, member = warp % TEAM;
+  const int worker = blockIdx.x * C::kTeams + team;
 
-  // this block's range of the list
+  // the workers' ranges of the list, and where in it this block's begin
+  auto cost_of = [](int units) { return units ? units + kHeadCost : 0; };
   long long mine = 0;
-  int first_units = 0;
+  int first_cost = 0;
   for (int i = threadIdx.x; i < p.spans; i += kAttendThreads) {
-    const int u = span_of<C::kRows, C::kUnit>(p, i).units;
-    if (i < kAttendThreads) first_units = u;
-    mine += u;
+    const int c = cost_of(span_of<C::kRows, C::kKeys>(p, i).units);
+    if (i < kAttendThreads) first_cost = c;
+    mine += c;
   }
   const long long total = block_sum(mine, s_scratch) * p.kv_heads;
-  const long long blocks = total < gridDim.x ? total : gridDim.x;  // none of them without a unit: the join relies on it
-  if (blockIdx.x >= blocks) return;
-  const long long u0 = total * blockIdx.x / blocks, u1 = total * (blockIdx.x + 1) / blocks;
-  long long run = 0;  // units of the spans before this chunk
-  for (int at = 0;; at += kAttendThreads) {
-    const int i = at + threadIdx.x;
-    const int u = at == 0 ? first_units : i < p.spans ? span_of<C::kRows, C::kUnit>(p, i).units : 0;
-    long long upto = u;
-    for (int x = 1; x < 32; x <<= 1) {
-      const long long y = __shfl_up_sync(~0u, upto, x);
-      if (lane >= x) upto += y;
+  const long long workers = total < (long long)gridDim.x * C::kTeams ? total : (long long)gridDim.x * C::kTeams;
+  if (total > 0) {
+    long long run = 0;  // cost of the spans before this chunk
+    for (int at = 0;; at += kAttendThreads) {
+      const int i = at + threadIdx.x;
+      const int c = at == 0 ? first_cost : i < p.spans ? cost_of(span_of<C::kRows, C::kKeys>(p, i).units) : 0;
+      long long upto = c;
+      for (int x = 1; x < 32; x <<= 1) {
+        const long long y = __shfl_up_sync(~0u, upto, x);
+        if (lane >= x) upto += y;
+      }
+      __syncthreads();
+      if (lane == 31) s_scratch[warp] = upto;
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) upto += s_scratch[w];
+      upto += run;
+      long long last = 0;  // the last range of the block begins here
+      for (int t = 0; t < C::kTeams; ++t) {
+        const long long w = (long long)blockIdx.x * C::kTeams + t;
+        if (w >= workers) break;
+        const long long begin = last = total * w / workers;
+        if ((upto - c) * p.kv_heads <= begin && begin < upto * p.kv_heads) {
+          s_index[t] = i;
+          s_before[t] = (upto - c) * p.kv_heads;
+        }
+      }
+      run += s_scratch[0] + s_scratch[1] + s_scratch[2] + s_scratch[3];
+      if (last < run * p.kv_heads) break;
     }
-    __syncthreads();
-    if (lane == 31) s_scratch[warp] = upto;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) upto += s_scratch[w];
-    upto += run;
-    if ((upto - u) * p.kv_heads <= u0 && u0 < upto * p.kv_heads) {
-      s_index = i;
-      s_before = (upto - u) * p.kv_heads;
+  }
+  // heads whose rows see nothing
+  for (int i = blockIdx.x; i < p.spans; i += gridDim.x) {
+    if (span_of<C::kRows, C::kKeys>(p, i).units) continue;
+    const int b = p.row_tiles == 1 ? i : i / p.row_tiles, row0 = (i - b * p.row_tiles) * C::kRows;
+    int rows = p.queries * p.group.d - row0;
+    if (rows > C::kRows) rows = C::kRows;
+    for (int x = warp; x < rows * p.kv_heads; x += kAttendWarps) {
+      const int kv = x / rows, r = row0 + x - kv * rows, q = divide(r, p.group), head = kv * p.group.d + r - q * p.group.d;
+      const int64_t token = (int64_t)b * p.queries + q;
+      for (int e = 4 * lane; e < p.d; e += 128) *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = make_uint2(0u, 0u);
+      if (lane == 0 && p.lse) p.lse[token * p.q_heads + head] = -INFINITY;
     }
-    run += s_scratch[0] + s_scratch[1] + s_scratch[2] + s_scratch[3];
-    if (u0 < run * p.kv_heads) break;
+    for (int x = threadIdx.x; x < p.kv_heads; x += kAttendThreads) p.shares[(int64_t)i * p.kv_heads + x] = make_int4(0, 0, 0, 0);
   }
   __syncthreads();
+  if (worker >= workers) return;
+  const long long u0 = total * worker / workers, u1 = total * (worker + 1) / workers;
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + team * C::kStages * 2 * C::kHalf;
   const int chunks = p.d * (F8 ? 1 : 2) / 16;  // of a staged row, that hold data
@@ -230,33 +251,53 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
   const uint32_t k_from = k_row * C::kRowBytes + (((F8 ? lane >> 4 : (lane >> 3) & 1) ^ swizzle(k_row)) << 4);
   const uint32_t v_from = v_row * C::kRowBytes + (((lane >> 4) ^ swizzle(v_row)) << 4);
 
-  int index = s_index;
-  long long before = s_before;
+  if (p.d < DP) {
+    // the products run over DP elements: the keys' others are zero, as the queries' are (the values' give columns that nobody reads)
+    for (int i = lane; i < C::kStages * C::kKeys / TEAM * C::kChunks; i += 32) {
+      const int ch = i % C::kChunks, r = i / C::kChunks * TEAM + member, row = r % C::kKeys;
+      if (ch >= chunks)
+        *reinterpret_cast<uint4*>(smem + team * C::kStages * 2 * C::kHalf + r / C::kKeys * 2 * C::kHalf + row * C::kRowBytes + ((ch ^ swizzle(row)) << 4)) =
+            make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+
+  int index = s_index[team];
+  long long before = s_before[team];
   for (long long u = u0; u < u1;) {
-    const Span sp = span_of<C::kRows, C::kUnit>(p, index);
+    const Span sp = span_of<C::kRows, C::kKeys>(p, index);
     if (sp.units == 0) {
       ++index;
       continue;
     }
-    const int kv = (int)((u - before) / sp.units), unit = (int)((u - before) - (long long)kv * sp.units);
-    const int n = (long long)(sp.units - unit) < u1 - u ? sp.units - unit : (int)(u1 - u);
-    const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row0 = (index - b * p.row_tiles) * C::kRows;
-    const int key0 = sp.start + unit * C::kUnit + team * C::kKeys;  // of this team's first tile; its tiles are a unit apart
-    int tiles = key0 < sp.hi ? (sp.hi - key0 + C::kUnit - 1) / C::kUnit : 0;
-    if (tiles > n) tiles = n;
+    const int cost = cost_of(sp.units), kv = (int)((u - before) / cost), from = (int)((u - before) - (long long)kv * cost);
+    const int to = cost - from < u1 - u ? cost : from + (int)(u1 - u);
+    const int unit = from > kHeadCost ? from - kHeadCost : 0, tiles = to - kHeadCost - unit;
+    const int span = index;
+    const int64_t slot = 2 * (int64_t)worker + (u == u0 ? 0 : 1);
+    const long long head_end = before + (long long)(kv + 1) * cost;
+    u += to - from;
+    if (u == before + (long long)cost * p.kv_heads) {
+      before = u;
+      ++index;
+    }
+    if (tiles <= 0) continue;
+    if (unit == 0 && lane == 0 && member == 0)  // worker w has [w * total / workers, (w + 1) * total / workers): the last whose range begins at or before a position
+      p.shares[(int64_t)span * p.kv_heads + kv] = make_int4(worker, (int)((head_end * workers - 1) / total), (int)slot, 0);
+    const int b = p.row_tiles == 1 ? span : span / p.row_tiles, row0 = (span - b * p.row_tiles) * C::kRows;
+    const int key0 = sp.start + unit * C::kKeys;
 
     // the pages of a tile's rows are asked for a tile ahead of the copies
     const int32_t* table = p.tables + b * p.table_stride;
     const uint8_t* kbase = p.k + kv * p.stride_head;
     const uint8_t* vbase = p.v + kv * p.stride_head;
     auto page_of = [&](int tile) {
-      const int key = key0 + tile * C::kUnit + member * C::kLoadRows + lane;
+      const int key = key0 + tile * C::kKeys + member * C::kLoadRows + lane;
       return tile < tiles && lane < C::kLoadRows && key < sp.hi ? table[divide(key, p.page)] : -1;
     };
     int page = page_of(0);
     auto issue = [&](int tile) {
       if (tile < tiles) {
-        const int key = key0 + tile * C::kUnit + member * C::kLoadRows + lane;
+        const int key = key0 + tile * C::kKeys + member * C::kLoadRows + lane;
         const bool ok = page >= 0 && page < p.pages;
         const int64_t off = ok ? page * p.stride_page + (int64_t)(key - divide(key, p.page) * p.page.d) * p.stride_slot : 0;
         const uint32_t seen = __ballot_sync(~0u, ok);
@@ -279,15 +320,6 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       }
       copy_commit();
     };
-    if (p.d < DP) {
-      // the products run over DP elements: the keys' others are zero, as the queries' are (the values' give columns that nobody reads)
-      for (int i = lane; i < C::kStages * C::kKeys / TEAM * C::kChunks; i += 32) {
-        const int ch = i % C::kChunks, r = i / C::kChunks * TEAM + member, row = r % C::kKeys;
-        if (ch >= chunks)
-          *reinterpret_cast<uint4*>(smem + team * C::kStages * 2 * C::kHalf + r / C::kKeys * 2 * C::kHalf + row * C::kRowBytes + ((ch ^ swizzle(row)) << 4)) =
-              make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
 #pragma unroll
     for (int i = 0; i < C::kStages - 1; ++i) issue(i);
 
@@ -347,7 +379,7 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       copy_wait<C::kStages - 2>();
       team_sync<TEAM>(team);
       issue(tile + C::kStages - 1);
-      const int stage = tile % C::kStages, key = key0 + tile * C::kUnit;
+      const int stage = tile % C::kStages, key = key0 + tile * C::kKeys;
       const uint32_t kt = ring + stage * 2 * C::kHalf, vt = kt + C::kHalf;
       uint32_t seen = 0;
 #pragma unroll
@@ -506,171 +538,135 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       }
     }
 
-    // join the teams, in their order
-    copy_wait<0>();
-    __syncthreads();  // the ring is free
-    float* sums = reinterpret_cast<float*>(smem);
+    // the result, or this worker's part of it
+    const bool all = tiles == sp.units;
+    const float v_scale = p.v_scale ? load_f32(p.v_scale + kv) : 1.0f;
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       l[h] += __shfl_xor_sync(~0u, l[h], 1);
       l[h] += __shfl_xor_sync(~0u, l[h], 2);
-      const int r = team * C::kRows + member * 16 + (lane >> 2) + 8 * h;
-      if ((lane & 3) == 0) s_stats[r] = make_float2(m[h], l[h]);
-      float* row = sums + r * C::kPitch;
+      const int in_tile = member * 16 + (lane >> 2) + 8 * h, r = row0 + in_tile;
+      if (r >= p.queries * p.group.d) continue;
+      if (all) {
+        const int i = divide(r, p.group), head = kv * p.group.d + r - i * p.group.d;
+        const int64_t token = (int64_t)b * p.queries + i;
+        const bool nothing = l[h] == 0.0f || i >= sp.count;  // padding went along unmasked
+        const float finish = v_scale / l[h];
+        __nv_bfloat16* row = p.out + token * p.out_ldt + head * p.out_ldh;
 #pragma unroll
-      for (int j = 0; j < DP / 8; j += F8 ? 2 : 1) {
-        if constexpr (F8)
-          *reinterpret_cast<float4*>(row + j * 8 + 4 * (lane & 3)) = make_float4(o[j][2 * h], o[j + 1][2 * h], o[j][2 * h + 1], o[j + 1][2 * h + 1]);
-        else
-          *reinterpret_cast<float2*>(row + j * 8 + 2 * (lane & 3)) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
-      }
-    }
-    __syncthreads();
-    const bool all = n == sp.units;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (u == u0 ? 0 : 1);
-    int rows = p.queries * p.group.d - row0;
-    if (rows > C::kRows) rows = C::kRows;
-    for (int r = warp; r < rows; r += kAttendWarps) {
-      const int i = divide(row0 + r, p.group), head = kv * p.group.d + row0 + r - i * p.group.d;
-      float top = -INFINITY, sum = 0.0f, w[C::kTeams];
-#pragma unroll
-      for (int t = 0; t < C::kTeams; ++t) top = fmaxf(top, s_stats[t * C::kRows + r].x);
-      const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-      for (int t = 0; t < C::kTeams; ++t) {
-        w[t] = exp2_approx(s_stats[t * C::kRows + r].x - base);
-        sum = fmaf(w[t], s_stats[t * C::kRows + r].y, sum);
-      }
-      if (i >= sp.count) sum = 0.0f;  // padding: it went along unmasked
-      const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
-      const int64_t token = (int64_t)b * p.queries + i;
-      for (int e = 4 * lane; e < p.d; e += 128) {
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int t = 0; t < C::kTeams; ++t) {
-          const float4 y = *reinterpret_cast<const float4*>(sums + (t * C::kRows + r) * C::kPitch + e);
-          x.x = fmaf(w[t], y.x, x.x), x.y = fmaf(w[t], y.y, x.y), x.z = fmaf(w[t], y.z, x.z), x.w = fmaf(w[t], y.w, x.w);
+        for (int j = 0; j < DP / 8; j += F8 ? 2 : 1) {
+          const int e = j * 8 + (F8 ? 4 : 2) * (lane & 3);
+          if (e >= p.d) break;
+          if constexpr (F8) {
+            const uint2 w = make_uint2(pack_bf16x2(o[j][2 * h] * finish, o[j + 1][2 * h] * finish), pack_bf16x2(o[j][2 * h + 1] * finish, o[j + 1][2 * h + 1] * finish));
+            *reinterpret_cast<uint2*>(row + e) = nothing ? make_uint2(0u, 0u) : w;
+          } else {
+            *reinterpret_cast<uint32_t*>(row + e) = nothing ? 0u : pack_bf16x2(o[j][2 * h] * finish, o[j][2 * h + 1] * finish);
+          }
         }
-        if (all) {
-          uint2 pair = make_uint2(pack_bf16x2(x.x * finish, x.y * finish), pack_bf16x2(x.z * finish, x.w * finish));
-          if (sum == 0.0f) pair = make_uint2(0u, 0u);  // a row that sees nothing, whatever the others' values were
-          *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = pair;
-        } else {
-          *reinterpret_cast<float4*>(p.part_sums + (slot * C::kRows + r) * p.d + e) = x;
+        if ((lane & 3) == 0 && p.lse) p.lse[token * p.q_heads + head] = nothing ? -INFINITY : (m[h] + log2f(l[h]) - C::kShift) * 0.6931471805599453f;
+      } else {
+        float* row = p.part_sums + (slot * C::kRows + in_tile) * p.d;
+#pragma unroll
+        for (int j = 0; j < DP / 8; j += F8 ? 2 : 1) {
+          const int e = j * 8 + (F8 ? 4 : 2) * (lane & 3);
+          if (e >= p.d) break;
+          if constexpr (F8)
+            *reinterpret_cast<float4*>(row + e) = make_float4(o[j][2 * h], o[j + 1][2 * h], o[j][2 * h + 1], o[j + 1][2 * h + 1]);
+          else
+            *reinterpret_cast<float2*>(row + e) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
         }
-      }
-      if (lane == 0) {
-        if (!all)
-          p.part_stats[slot * C::kRows + r] = make_float2(top, sum);
-        else if (p.lse)
-          p.lse[token * p.q_heads + head] = sum == 0.0f ? -INFINITY : (base + log2f(sum) - C::kShift) * 0.6931471805599453f;
+        if ((lane & 3) == 0) p.part_stats[slot * C::kRows + in_tile] = make_float2(m[h], l[h]);
       }
     }
-    __syncthreads();  // before the next segment's copies
-    u += n;
-    if (u == before + (long long)sp.units * p.kv_heads) {
-      before = u;
-      ++index;
-    }
+    copy_wait<0>();
+    team_sync<TEAM>(team);  // the ring is free for the next head
   }
 }
 
-// One block per row of a (span, kv head): adds up what the blocks that shared it left, or writes the result of a row that sees nothing.
-template <int ROWS, int UNIT>
-__global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(const AttendArgs p, int grid, float shift) {
-  __shared__ long long s_scratch[kAttendWarps];
-  __shared__ float s_weight[kMaxAttendBlocks], s_part[kAttendWarps];
+// Adds up what the workers that shared a head left. `kWarps` warps take the parts of one row in turn and are joined through shared memory: one
+// where there are many heads and few parts of each, four where few heads are in many parts.
+template <int ROWS, int UNIT, int kWarps>
+__global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(const AttendArgs p, float shift) {
+  constexpr int kGroups = kAttendWarps / kWarps;
   __shared__ float4 s_sum[kAttendThreads];
-  const int index = blockIdx.x / p.kv_heads, kv = blockIdx.x - index * p.kv_heads, r = blockIdx.y;
-  const int b = index / p.row_tiles, row0 = (index - b * p.row_tiles) * ROWS;
-  if (row0 + r >= p.queries * p.group.d) return;
-  const Span sp = span_of<ROWS, UNIT>(p, index);
-  const int units = sp.units, i = divide(row0 + r, p.group), head = kv * p.group.d + row0 + r - i * p.group.d;
-  const int64_t token = (int64_t)b * p.queries + i;
-  __nv_bfloat16* out = p.out + token * p.out_ldt + head * p.out_ldh;
-  if (units == 0 || i >= sp.count) {
-    for (int e = 4 * threadIdx.x; e < p.d; e += 4 * kAttendThreads) *reinterpret_cast<uint2*>(out + e) = make_uint2(0u, 0u);
-    if (threadIdx.x == 0 && p.lse) p.lse[token * p.q_heads + head] = -INFINITY;
-    return;
-  }
-  long long all = 0, front = 0;
-  for (int x = threadIdx.x; x < p.spans; x += kAttendThreads) {
-    const int u = span_of<ROWS, UNIT>(p, x).units;
-    all += u;
-    if (x < index) front += u;
-  }
-  const long long total = block_sum(all, s_scratch) * p.kv_heads;
-  const long long first = block_sum(front, s_scratch) * p.kv_heads + (long long)kv * units, last = first + units - 1;
-  const long long blocks = total < grid ? total : grid;
-  // block c has [c * total / blocks, (c + 1) * total / blocks): the one that holds unit u is the last that begins at or before it
-  const int c0 = (int)(((first + 1) * blocks - 1) / total), c1 = (int)(((last + 1) * blocks - 1) / total);
-  if (c0 == c1) return;
-  const int n = c1 - c0 + 1;
-  auto slot_of = [&](int x) { return 2 * (int64_t)(c0 + x) + (first <= total * (c0 + x) / blocks ? 0 : 1); };
-
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float top = -INFINITY;
-  for (int x = threadIdx.x; x < n; x += kAttendThreads) {
-    s_weight[x] = p.part_stats[slot_of(x) * ROWS + r].x;
-    top = fmaxf(top, s_weight[x]);
-  }
-  for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-  if (lane == 0) s_part[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_part[0], s_part[1]), fmaxf(s_part[2], s_part[3]));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f;
-  for (int x = threadIdx.x; x < n; x += kAttendThreads) {
-    const float w = exp2_approx(s_weight[x] - base);
-    s_weight[x] = w;
-    sum = fmaf(w, p.part_stats[slot_of(x) * ROWS + r].y, sum);
-  }
-  for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
-  __syncthreads();
-  if (lane == 0) s_part[warp] = sum;
-  __syncthreads();
-  sum = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
-
-  const int quads = p.d / 4, groups = kAttendThreads / quads, g = threadIdx.x / quads, e = 4 * (threadIdx.x - g * quads);
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (g < groups) {
-#pragma unroll 4
-    for (int x = g; x < n; x += groups) {
-      const float4 y = *reinterpret_cast<const float4*>(p.part_sums + (slot_of(x) * ROWS + r) * p.d + e);
-      const float w = s_weight[x];
-      acc.x = fmaf(w, y.x, acc.x), acc.y = fmaf(w, y.y, acc.y), acc.z = fmaf(w, y.z, acc.z), acc.w = fmaf(w, y.w, acc.w);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % kWarps;
+  int rows = p.queries * p.group.d;
+  if (rows > ROWS) rows = ROWS;
+  const int64_t items = (int64_t)p.spans * p.kv_heads * rows;
+  for (int64_t first = (int64_t)blockIdx.x * kGroups; first < items; first += (int64_t)gridDim.x * kGroups) {
+    const int64_t item = first + warp / kWarps, at = item / rows;
+    const int r = (int)(item - at * rows), index = (int)(at / p.kv_heads), kv = (int)(at - (int64_t)index * p.kv_heads);
+    const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row = (index - b * p.row_tiles) * ROWS + r;
+    if (kWarps == 1 && (item >= items || row >= p.queries * p.group.d)) continue;  // uniform in the block where it is more than a warp's matter
+    if (kWarps > 1 && row >= p.queries * p.group.d) continue;
+    const int4 sh = p.shares[at];
+    const int n = sh.y - sh.x + 1;
+    if (n <= 1) continue;
+    auto slot_of = [&](int x) { return x == 0 ? (int64_t)sh.z : 2 * (int64_t)(sh.x + x); };  // the others begin with this head
+    float top = -INFINITY, sum = 0.0f;
+    for (int x = lane; x < n; x += 32) top = fmaxf(top, p.part_stats[slot_of(x) * ROWS + r].x);
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+    const float base = top == -INFINITY ? 0.0f : top;
+    const int i = divide(row, p.group), head = kv * p.group.d + row - i * p.group.d;
+    const int64_t token = (int64_t)b * p.queries + i;
+    const bool padding = i >= span_of<ROWS, UNIT>(p, index).count;
+    for (int e0 = 0; e0 < p.d; e0 += 128) {
+      const int e = e0 + 4 * lane;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      sum = 0.0f;
+      for (int x0 = 0; x0 < n; x0 += 32) {
+        const float2 st = x0 + lane < n ? p.part_stats[slot_of(x0 + lane) * ROWS + r] : make_float2(-INFINITY, 0.0f);
+        const float w = exp2_approx(st.x - base);
+        sum += w * st.y;
+        const int many = n - x0 < 32 ? n - x0 : 32;
+#pragma unroll 8
+        for (int y = share; y < many; y += kWarps) {
+          const float wy = __shfl_sync(~0u, w, y);
+          if (e < p.d) {
+            const float4 v = *reinterpret_cast<const float4*>(p.part_sums + (slot_of(x0 + y) * ROWS + r) * p.d + e);
+            acc.x = fmaf(wy, v.x, acc.x), acc.y = fmaf(wy, v.y, acc.y), acc.z = fmaf(wy, v.z, acc.z), acc.w = fmaf(wy, v.w, acc.w);
+          }
+        }
+      }
+      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
+      if constexpr (kWarps > 1) {
+        __syncthreads();
+        s_sum[threadIdx.x] = acc;
+        __syncthreads();
+        if (share == 0)
+          for (int x = 1; x < kWarps; ++x) {
+            const float4 v = s_sum[threadIdx.x + 32 * x];
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+          }
+      }
+      if (share == 0 && e < p.d) {
+        const bool nothing = sum == 0.0f || padding;
+        const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
+        const uint2 w = make_uint2(pack_bf16x2(acc.x * finish, acc.y * finish), pack_bf16x2(acc.z * finish, acc.w * finish));
+        *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = nothing ? make_uint2(0u, 0u) : w;
+      }
     }
-    s_sum[threadIdx.x] = acc;
-  }
-  __syncthreads();
-  if (g == 0) {
-    for (int x = 1; x < groups; ++x) {
-      const float4 y = s_sum[x * quads + threadIdx.x];
-      acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
-    }
-    const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
-    uint2 pair = make_uint2(pack_bf16x2(acc.x * finish, acc.y * finish), pack_bf16x2(acc.z * finish, acc.w * finish));
-    if (sum == 0.0f) pair = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2*>(out + e) = pair;
-    if (threadIdx.x == 0 && p.lse) p.lse[token * p.q_heads + head] = sum == 0.0f ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
+    if (share == 0 && lane == 0 && p.lse) p.lse[token * p.q_heads + head] = sum == 0.0f || padding ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
   }
 }
 
-// Blocks of a call: as many as fit the device at once, or one per unit where the table cannot name more.
+// Blocks of a call: as many as fit the device at once, or as the list can need.
 template <int DP, bool F8, int ROWS>
 static int attend_blocks(int64_t spans, int64_t kv_heads, int64_t entries) {
   using C = AttendCfg<DP, F8, ROWS>;
-  int64_t cap = (int64_t)sm_count() * C::kBlocksPerSm;
-  if (cap > kMaxAttendBlocks) cap = kMaxAttendBlocks;
-  const int64_t heads = spans * kv_heads, each = (entries + C::kUnit - 1) / C::kUnit;
-  return (int)(heads >= cap || each >= cap || heads * each >= cap ? cap : heads * each);
+  const int64_t cap = (int64_t)sm_count() * C::kBlocksPerSm;
+  const int64_t heads = spans * kv_heads, each = (entries + C::kKeys - 1) / C::kKeys + kHeadCost;
+  if (heads >= cap * C::kTeams || each >= cap * C::kTeams || heads * each >= cap * C::kTeams) return (int)cap;
+  return (int)((heads * each + C::kTeams - 1) / C::kTeams);
 }
 
 template <int DP, bool F8, int ROWS>
 struct AttendCall {
   using C = AttendCfg<DP, F8, ROWS>;
+  static int64_t slots(int64_t spans, int64_t kv_heads, int64_t entries) { return 2 * (int64_t)attend_blocks<DP, F8, ROWS>(spans, kv_heads, entries) * C::kTeams; }
   static int64_t workspace(int64_t spans, int64_t kv_heads, int64_t d, int64_t entries) {
-    return 2 * (int64_t)attend_blocks<DP, F8, ROWS>(spans, kv_heads, entries) * C::kRows * (d + 2) * 4;
+    return slots(spans, kv_heads, entries) * C::kRows * (d + 2) * 4 + spans * kv_heads * 16;
   }
   static tf_status launch(AttendArgs p, void* workspace, cudaStream_t stream) {
     auto kernel = paged_attention_kernel<DP, F8, ROWS>;
@@ -682,13 +678,21 @@ struct AttendCall {
       configured_dev = dev;
     }
     const int blocks = attend_blocks<DP, F8, ROWS>(p.spans, p.kv_heads, p.entries);
+    const int64_t parts = 2 * (int64_t)blocks * C::kTeams * C::kRows, heads = (int64_t)p.spans * p.kv_heads;
     p.part_sums = static_cast<float*>(workspace);
-    p.part_stats = reinterpret_cast<float2*>(p.part_sums + 2 * (int64_t)blocks * C::kRows * p.d);
+    p.part_stats = reinterpret_cast<float2*>(p.part_sums + parts * p.d);
+    p.shares = reinterpret_cast<int4*>(p.part_stats + parts);
     kernel<<<blocks, kAttendThreads, C::kSmem, stream>>>(p);
     TF_LAUNCH_CHECK();
-    int rows = p.queries * p.group.d;
-    if (rows > C::kRows) rows = C::kRows;
-    paged_attention_join_kernel<C::kRows, C::kUnit><<<dim3((unsigned)p.spans * (unsigned)p.kv_heads, (unsigned)rows), kAttendThreads, 0, stream>>>(p, blocks, C::kShift);
+    const int64_t rows = (int64_t)p.queries * p.group.d, items = heads * (rows < C::kRows ? rows : C::kRows);
+    // four warps to a row where a head may have more than eight parts
+    const bool few = heads * 8 < (int64_t)blocks * C::kTeams;
+    const int64_t need = few ? items : (items + kAttendWarps - 1) / kAttendWarps, most = (int64_t)sm_count() * 8;
+    const unsigned grid = (unsigned)(need < most ? need : most);
+    if (few)
+      paged_attention_join_kernel<C::kRows, C::kKeys, 4><<<grid, kAttendThreads, 0, stream>>>(p, C::kShift);
+    else
+      paged_attention_join_kernel<C::kRows, C::kKeys, 1><<<grid, kAttendThreads, 0, stream>>>(p, C::kShift);
     TF_LAUNCH_CHECK();
     return TF_OK;
   }
