@@ -162,6 +162,29 @@ __device__ __forceinline__ Span span_of(const AttendArgs& p, int index) {
   return s;
 }
 
+// n / d, with the short division where both fit it.
+__device__ __forceinline__ long long quotient(long long n, long long d) {
+  return ((n | d) >> 32) == 0 ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
+}
+
+// `total` positions dealt out to workers in contiguous ranges that differ by one at most; none of them is empty.
+struct Ranges {
+  long long each, more;  // the first `more` workers have each + 1
+  int workers;
+  __device__ static Ranges of(long long total, int most) {
+    Ranges r;
+    r.workers = total < most ? (int)total : most;
+    r.each = r.workers ? quotient(total, r.workers) : 0;
+    r.more = total - r.each * r.workers;
+    return r;
+  }
+  __device__ long long begin(int w) const { return each * w + (w < more ? w : more); }
+  __device__ int of_position(long long x) const {
+    const long long large = (each + 1) * more;
+    return (int)(x < large ? quotient(x, each + 1) : more + quotient(x - large, each));
+  }
+};
+
 // Sums over a block of 128 threads. `scratch` holds one value per warp; the caller does not touch it without a barrier.
 __device__ __forceinline__ long long block_sum(long long x, long long* scratch) {
   for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(~0u, x, i);
@@ -180,47 +203,52 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
   __shared__ int s_index[C::kTeams];
   __shared__ uint32_t s_seen[C::kTeams][C::kStages][TEAM];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / TEAM, member = warp % TEAM;
+  griddep_wait();
+  griddep_launch_dependents();  // the join: its blocks find room as this kernel's leave
   const int worker = blockIdx.x * C::kTeams + team;
 
   // the workers' ranges of the list, and where in it this block's begin
-  auto cost_of = [](int units) { return units ? units + kHeadCost : 0; };
-  long long mine = 0;
-  int first_cost = 0;
-  for (int i = threadIdx.x; i < p.spans; i += kAttendThreads) {
-    const int c = cost_of(span_of<C::kRows, C::kKeys>(p, i).units);
-    if (i < kAttendThreads) first_cost = c;
-    mine += c;
+  auto cost_of = [&](int i) {
+    const int units = i < p.spans ? span_of<C::kRows, C::kKeys>(p, i).units : 0;
+    return units ? units + kHeadCost : 0;
+  };
+  const int chunk_cost = cost_of(threadIdx.x);
+  long long total = 0;
+  if (p.spans > kAttendThreads) {
+    long long mine = chunk_cost;
+    for (int i = threadIdx.x + kAttendThreads; i < p.spans; i += kAttendThreads) mine += cost_of(i);
+    total = block_sum(mine, s_scratch) * p.kv_heads;
   }
-  const long long total = block_sum(mine, s_scratch) * p.kv_heads;
-  const long long workers = total < (long long)gridDim.x * C::kTeams ? total : (long long)gridDim.x * C::kTeams;
-  if (total > 0) {
-    long long run = 0;  // cost of the spans before this chunk
-    for (int at = 0;; at += kAttendThreads) {
-      const int i = at + threadIdx.x;
-      const int c = at == 0 ? first_cost : i < p.spans ? cost_of(span_of<C::kRows, C::kKeys>(p, i).units) : 0;
-      long long upto = c;
-      for (int x = 1; x < 32; x <<= 1) {
-        const long long y = __shfl_up_sync(~0u, upto, x);
-        if (lane >= x) upto += y;
-      }
-      __syncthreads();
-      if (lane == 31) s_scratch[warp] = upto;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) upto += s_scratch[w];
-      upto += run;
-      long long last = 0;  // the last range of the block begins here
-      for (int t = 0; t < C::kTeams; ++t) {
-        const long long w = (long long)blockIdx.x * C::kTeams + t;
-        if (w >= workers) break;
-        const long long begin = last = total * w / workers;
-        if ((upto - c) * p.kv_heads <= begin && begin < upto * p.kv_heads) {
-          s_index[t] = i;
-          s_before[t] = (upto - c) * p.kv_heads;
-        }
-      }
-      run += s_scratch[0] + s_scratch[1] + s_scratch[2] + s_scratch[3];
-      if (last < run * p.kv_heads) break;
+  Ranges ranges;
+  long long run = 0;  // cost of the spans before this chunk
+  for (int at = 0;; at += kAttendThreads) {
+    const int c = at == 0 ? chunk_cost : cost_of(at + threadIdx.x);
+    long long upto = c;
+    for (int x = 1; x < 32; x <<= 1) {
+      const long long y = __shfl_up_sync(~0u, upto, x);
+      if (lane >= x) upto += y;
     }
+    __syncthreads();
+    if (lane == 31) s_scratch[warp] = upto;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) upto += s_scratch[w];
+    upto += run;
+    run += s_scratch[0] + s_scratch[1] + s_scratch[2] + s_scratch[3];
+    if (at == 0) {
+      if (p.spans <= kAttendThreads) total = run * p.kv_heads;
+      ranges = Ranges::of(total, (int)gridDim.x * C::kTeams);
+    }
+    long long last = -1;  // the last range of the block begins here
+    for (int t = 0; t < C::kTeams; ++t) {
+      const int w = (int)blockIdx.x * C::kTeams + t;
+      if (w >= ranges.workers) break;
+      last = ranges.begin(w);
+      if ((upto - c) * p.kv_heads <= last && last < upto * p.kv_heads) {
+        s_index[t] = at + threadIdx.x;
+        s_before[t] = (upto - c) * p.kv_heads;
+      }
+    }
+    if (last < run * p.kv_heads) break;
   }
   // heads whose rows see nothing
   for (int i = blockIdx.x; i < p.spans; i += gridDim.x) {
@@ -237,8 +265,8 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
     for (int x = threadIdx.x; x < p.kv_heads; x += kAttendThreads) p.shares[(int64_t)i * p.kv_heads + x] = make_int4(0, 0, 0, 0);
   }
   __syncthreads();
-  if (worker >= workers) return;
-  const long long u0 = total * worker / workers, u1 = total * (worker + 1) / workers;
+  if (worker >= ranges.workers) return;
+  const long long u0 = ranges.begin(worker), u1 = ranges.begin(worker + 1);
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + team * C::kStages * 2 * C::kHalf;
   const int chunks = p.d * (F8 ? 1 : 2) / 16;  // of a staged row, that hold data
@@ -269,7 +297,7 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       ++index;
       continue;
     }
-    const int cost = cost_of(sp.units), kv = (int)((u - before) / cost), from = (int)((u - before) - (long long)kv * cost);
+    const int cost = sp.units + kHeadCost, kv = (int)quotient(u - before, cost), from = (int)((u - before) - (long long)kv * cost);
     const int to = cost - from < u1 - u ? cost : from + (int)(u1 - u);
     const int unit = from > kHeadCost ? from - kHeadCost : 0, tiles = to - kHeadCost - unit;
     const int span = index;
@@ -281,8 +309,7 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       ++index;
     }
     if (tiles <= 0) continue;
-    if (unit == 0 && lane == 0 && member == 0)  // worker w has [w * total / workers, (w + 1) * total / workers): the last whose range begins at or before a position
-      p.shares[(int64_t)span * p.kv_heads + kv] = make_int4(worker, (int)((head_end * workers - 1) / total), (int)slot, 0);
+    if (unit == 0 && lane == 0 && member == 0) p.shares[(int64_t)span * p.kv_heads + kv] = make_int4(worker, ranges.of_position(head_end - 1), (int)slot, 0);
     const int b = p.row_tiles == 1 ? span : span / p.row_tiles, row0 = (span - b * p.row_tiles) * C::kRows;
     const int key0 = sp.start + unit * C::kKeys;
 
@@ -591,6 +618,7 @@ __global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(co
   constexpr int kGroups = kAttendWarps / kWarps;
   __shared__ float4 s_sum[kAttendThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % kWarps;
+  griddep_wait();
   int rows = p.queries * p.group.d;
   if (rows > ROWS) rows = ROWS;
   const int64_t items = (int64_t)p.spans * p.kv_heads * rows;
@@ -612,7 +640,7 @@ __global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(co
     const int64_t token = (int64_t)b * p.queries + i;
     const bool padding = i >= span_of<ROWS, UNIT>(p, index).count;
     for (int e0 = 0; e0 < p.d; e0 += 128) {
-      const int e = e0 + 4 * lane;
+      const int e = e0 + 4 * lane, column = e < p.d ? e : 0;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       sum = 0.0f;
       for (int x0 = 0; x0 < n; x0 += 32) {
@@ -620,12 +648,19 @@ __global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(co
         const float w = exp2_approx(st.x - base);
         sum += w * st.y;
         const int many = n - x0 < 32 ? n - x0 : 32;
-#pragma unroll 8
-        for (int y = share; y < many; y += kWarps) {
-          const float wy = __shfl_sync(~0u, w, y);
-          if (e < p.d) {
-            const float4 v = *reinterpret_cast<const float4*>(p.part_sums + (slot_of(x0 + y) * ROWS + r) * p.d + e);
-            acc.x = fmaf(wy, v.x, acc.x), acc.y = fmaf(wy, v.y, acc.y), acc.z = fmaf(wy, v.z, acc.z), acc.w = fmaf(wy, v.w, acc.w);
+        for (int y0 = share; y0 < many; y0 += 8 * kWarps) {  // eight loads in flight
+          float4 v[8];
+          float wy[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            const int z = y0 + y * kWarps, x = z < many ? z : many - 1;
+            wy[y] = __shfl_sync(~0u, w, z & 31);
+            v[y] = *reinterpret_cast<const float4*>(p.part_sums + (slot_of(x0 + x) * ROWS + r) * p.d + column);
+          }
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            if (y0 + y * kWarps >= many) continue;
+            acc.x = fmaf(wy[y], v[y].x, acc.x), acc.y = fmaf(wy[y], v[y].y, acc.y), acc.z = fmaf(wy[y], v[y].z, acc.z), acc.w = fmaf(wy[y], v[y].w, acc.w);
           }
         }
       }
@@ -682,18 +717,14 @@ struct AttendCall {
     p.part_sums = static_cast<float*>(workspace);
     p.part_stats = reinterpret_cast<float2*>(p.part_sums + parts * p.d);
     p.shares = reinterpret_cast<int4*>(p.part_stats + parts);
-    kernel<<<blocks, kAttendThreads, C::kSmem, stream>>>(p);
-    TF_LAUNCH_CHECK();
+    TF_CUDA(launch_dependent(true, kernel, dim3((unsigned)blocks), dim3(kAttendThreads), C::kSmem, stream, p));
     const int64_t rows = (int64_t)p.queries * p.group.d, items = heads * (rows < C::kRows ? rows : C::kRows);
     // four warps to a row where a head may have more than eight parts
     const bool few = heads * 8 < (int64_t)blocks * C::kTeams;
     const int64_t need = few ? items : (items + kAttendWarps - 1) / kAttendWarps, most = (int64_t)sm_count() * 8;
     const unsigned grid = (unsigned)(need < most ? need : most);
-    if (few)
-      paged_attention_join_kernel<C::kRows, C::kKeys, 4><<<grid, kAttendThreads, 0, stream>>>(p, C::kShift);
-    else
-      paged_attention_join_kernel<C::kRows, C::kKeys, 1><<<grid, kAttendThreads, 0, stream>>>(p, C::kShift);
-    TF_LAUNCH_CHECK();
+    auto join = few ? paged_attention_join_kernel<C::kRows, C::kKeys, 4> : paged_attention_join_kernel<C::kRows, C::kKeys, 1>;
+    TF_CUDA(launch_dependent(true, join, dim3(grid), dim3(kAttendThreads), 0, stream, p, C::kShift));
     return TF_OK;
   }
 };
