@@ -83,6 +83,13 @@ def test_attention_refuses(status, change):
 
 
 @needs_library
+def test_attention_refuses_a_small_workspace():
+    need = N.load().tf_paged_attention_workspace_bytes(2, 2, 4, 2, 64, 0, 48)
+    assert need > 0
+    assert attend(workspace_bytes=need - 1) == N.TF_ERR_WORKSPACE and attend(workspace=None) == N.TF_ERR_WORKSPACE and str(need) in N.last_error()
+
+
+@needs_library
 def test_nothing_to_do_is_no_error():
     assert rotary(tokens=0) == append(tokens=0) == attend(seqs=0) == N.TF_OK
     assert N.load().tf_paged_attention_workspace_bytes(0, 0, 4, 2, 64, 0, 16) == -1

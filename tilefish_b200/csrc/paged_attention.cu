@@ -1,7 +1,7 @@
 // The entry points of attention over a paged key-value cache. The kernels are in paged_attention.cuh, built by head size in paged_attention_<type>_d<size>.cu.
 #include <type_traits>
 
-#include "paged_attention.cuh"
+#include "paged_attention.h"
 
 namespace tf {
 
@@ -84,9 +84,6 @@ extern "C" tf_status tf_paged_attention(const tf_paged_cache* cache, const void*
   if (seqs == 0) return TF_OK;
   // a table that names more entries than 2^30 is read up to there: no sequence is that long
   const int64_t most = INT32_MAX / 2, entries = table_cols > most / cache->page_size ? most : table_cols * cache->page_size;
-  const int64_t need = tf_paged_attention_workspace_bytes(seqs, queries, q_heads, cache->kv_heads, cache->head_dim, cache->dtype, entries);
-  if (need > workspace_bytes || (need > 0 && !workspace))
-    return fail(TF_ERR_WORKSPACE, "%s: the workspace needs %lld bytes, %lld were given", __func__, (long long)need, (long long)workspace_bytes);
   const int64_t item = cache->dtype == TF_CACHE_BF16 ? 2 : 1, rows = queries * (q_heads / cache->kv_heads);
   AttendArgs p = {};
   p.k = static_cast<const uint8_t*>(cache->k), p.v = static_cast<const uint8_t*>(cache->v), p.k_scale = cache->k_scale, p.v_scale = cache->v_scale;
@@ -100,5 +97,5 @@ extern "C" tf_status tf_paged_attention(const tf_paged_cache* cache, const void*
   p.window = (int)(window > INT32_MAX / 2 ? 0 : window);
   p.group = divisor((int)(q_heads / cache->kv_heads));
   p.scale_log2 = scale * 1.4426950408889634f;
-  return with_attend_call(rows, p.d, cache->dtype, [&](auto call) { return decltype(call)::launch(p, workspace, (cudaStream_t)stream); });
+  return with_attend_call(rows, p.d, cache->dtype, [&](auto call) { return decltype(call)::launch(p, workspace, workspace_bytes, (cudaStream_t)stream, "tf_paged_attention"); });
 }

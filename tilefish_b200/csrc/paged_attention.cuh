@@ -14,39 +14,11 @@
 // paged_attention_join_kernel adds them up in the order of the keys.
 #pragma once
 
-#include <cuda_bf16.h>
-
 #include <cmath>
 
-#include "paged_cache.h"
+#include "paged_attention.h"
 
 namespace tf {
-
-struct AttendArgs {
-  const uint8_t* k;
-  const uint8_t* v;
-  const float* k_scale;
-  const float* v_scale;
-  int64_t stride_page, stride_head, stride_slot;  // bytes
-  int pages, kv_heads, d;
-  Divisor page;
-  const __nv_bfloat16* q;
-  __nv_bfloat16* out;
-  float* lse;
-  int64_t q_ldt, q_ldh, out_ldt, out_ldh;
-  const int32_t* tables;
-  int64_t table_stride;
-  const int32_t* lengths;
-  const int32_t* counts;
-  int entries;  // what a table can name
-  int spans;    // sequences x row tiles
-  int queries, q_heads, row_tiles, window;
-  Divisor group;
-  float scale_log2;
-  float* part_sums;    // [2 * workers][rows][d]: of a worker's first head, and of its last
-  float2* part_stats;  // [2 * workers][rows]: maximum, sum
-  int4* shares;        // [spans * kv_heads]: the first and the last worker of a head, and the first one's slot
-};
 
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
 constexpr int kHeadCost = 1;  // what starting a head costs a worker, in tiles: about the latency of its first keys
@@ -697,36 +669,38 @@ static int attend_blocks(int64_t spans, int64_t kv_heads, int64_t entries) {
 }
 
 template <int DP, bool F8, int ROWS>
-struct AttendCall {
+int64_t AttendCall<DP, F8, ROWS>::workspace(int64_t spans, int64_t kv_heads, int64_t d, int64_t entries) {
   using C = AttendCfg<DP, F8, ROWS>;
-  static int64_t slots(int64_t spans, int64_t kv_heads, int64_t entries) { return 2 * (int64_t)attend_blocks<DP, F8, ROWS>(spans, kv_heads, entries) * C::kTeams; }
-  static int64_t workspace(int64_t spans, int64_t kv_heads, int64_t d, int64_t entries) {
-    return slots(spans, kv_heads, entries) * C::kRows * (d + 2) * 4 + spans * kv_heads * 16;
+  return 2 * (int64_t)attend_blocks<DP, F8, ROWS>(spans, kv_heads, entries) * C::kTeams * C::kRows * (d + 2) * 4 + spans * kv_heads * 16;
+}
+
+template <int DP, bool F8, int ROWS>
+tf_status AttendCall<DP, F8, ROWS>::launch(AttendArgs p, void* workspace_at, int64_t workspace_bytes, cudaStream_t stream, const char* fn) {
+  using C = AttendCfg<DP, F8, ROWS>;
+  const int64_t need = workspace(p.spans, p.kv_heads, p.d, p.entries);
+  if (need > workspace_bytes || !workspace_at)
+    return fail(TF_ERR_WORKSPACE, "%s: the workspace needs %lld bytes, %lld were given", fn, (long long)need, (long long)workspace_bytes);
+  auto kernel = paged_attention_kernel<DP, F8, ROWS>;
+  static thread_local int configured_dev = -1;
+  int dev = 0;
+  TF_CUDA(cudaGetDevice(&dev));
+  if (configured_dev != dev) {
+    TF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    configured_dev = dev;
   }
-  static tf_status launch(AttendArgs p, void* workspace, cudaStream_t stream) {
-    auto kernel = paged_attention_kernel<DP, F8, ROWS>;
-    static thread_local int configured_dev = -1;
-    int dev = 0;
-    TF_CUDA(cudaGetDevice(&dev));
-    if (configured_dev != dev) {
-      TF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-      configured_dev = dev;
-    }
-    const int blocks = attend_blocks<DP, F8, ROWS>(p.spans, p.kv_heads, p.entries);
-    const int64_t parts = 2 * (int64_t)blocks * C::kTeams * C::kRows, heads = (int64_t)p.spans * p.kv_heads;
-    p.part_sums = static_cast<float*>(workspace);
-    p.part_stats = reinterpret_cast<float2*>(p.part_sums + parts * p.d);
-    p.shares = reinterpret_cast<int4*>(p.part_stats + parts);
-    TF_CUDA(launch_dependent(true, kernel, dim3((unsigned)blocks), dim3(kAttendThreads), C::kSmem, stream, p));
-    const int64_t rows = (int64_t)p.queries * p.group.d, items = heads * (rows < C::kRows ? rows : C::kRows);
-    // four warps to a row where a head may have more than eight parts
-    const bool few = heads * 8 < (int64_t)blocks * C::kTeams;
-    const int64_t need = few ? items : (items + kAttendWarps - 1) / kAttendWarps, most = (int64_t)sm_count() * 8;
-    const unsigned grid = (unsigned)(need < most ? need : most);
-    auto join = few ? paged_attention_join_kernel<C::kRows, C::kKeys, 4> : paged_attention_join_kernel<C::kRows, C::kKeys, 1>;
-    TF_CUDA(launch_dependent(true, join, dim3(grid), dim3(kAttendThreads), 0, stream, p, C::kShift));
-    return TF_OK;
-  }
-};
+  const int blocks = attend_blocks<DP, F8, ROWS>(p.spans, p.kv_heads, p.entries);
+  const int64_t parts = 2 * (int64_t)blocks * C::kTeams * C::kRows, heads = (int64_t)p.spans * p.kv_heads;
+  p.part_sums = static_cast<float*>(workspace_at);
+  p.part_stats = reinterpret_cast<float2*>(p.part_sums + parts * p.d);
+  p.shares = reinterpret_cast<int4*>(p.part_stats + parts);
+  TF_CUDA(launch_dependent(true, kernel, dim3((unsigned)blocks), dim3(kAttendThreads), C::kSmem, stream, p));
+  const int64_t rows = (int64_t)p.queries * p.group.d, items = heads * (rows < C::kRows ? rows : C::kRows);
+  // four warps to a row where a head may have more than eight parts
+  const bool few = heads * 8 < (int64_t)blocks * C::kTeams;
+  const int64_t groups = few ? items : (items + kAttendWarps - 1) / kAttendWarps, most = (int64_t)sm_count() * 8;
+  auto join = few ? paged_attention_join_kernel<C::kRows, C::kKeys, 4> : paged_attention_join_kernel<C::kRows, C::kKeys, 1>;
+  TF_CUDA(launch_dependent(true, join, dim3((unsigned)(groups < most ? groups : most)), dim3(kAttendThreads), 0, stream, p, C::kShift));
+  return TF_OK;
+}
 
 }  // namespace tf
