@@ -32,12 +32,14 @@ struct AttendCfg {
   static constexpr int kKeys = kRowBytes >= (kTeam == 1 ? 256 : 512) ? 16 : 32;  // of a team's tile
   static constexpr int kLoadRows = kKeys / kTeam;                               // of them, a warp loads
   static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
-  static constexpr int kFit = 65536 / (kTeams * 2 * kHalf);
-  static constexpr int kStages = kFit < 2 ? 2 : kFit > 4 ? 4 : kFit;
+  // Two blocks an SM with rings of 96 KB, without spilled registers, keep more in flight than three with 64 KB (64 x 8192 bf16 195 -> 189 us, e4m3 122 -> 113); heads of up
+  // to 64 elements have registers for three, and little calls gain by the warps (a window of 1024: 21.3 us, 23.0 with two).
+  static constexpr int kBlocksPerSm = DP <= 64 ? 3 : DP <= 128 || F8 ? 2 : 1;
+  static constexpr int kFit = (kBlocksPerSm == 3 ? 65536 : kBlocksPerSm == 2 ? 98304 : 196608) / (kTeams * 2 * kHalf);
+  static constexpr int kStages = kFit < 2 ? 2 : kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kTeams * kStages * 2 * kHalf;
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
   static constexpr int kRowsPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
-  static constexpr int kBlocksPerSm = DP <= 128 ? 3 : F8 ? 2 : 1;
   // an e4m3 entry is multiplied as f16: weights are scaled by 2^15 (the largest is 2^15), so that small ones keep their bits
   static constexpr float kShift = F8 ? 15.0f : 0.0f;
 };
@@ -293,16 +295,16 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       const int key = key0 + tile * C::kKeys + member * C::kLoadRows + lane;
       return tile < tiles && lane < C::kLoadRows && key < sp.hi ? table[divide(key, p.page)] : -1;
     };
-    int page = page_of(0);
+    int page = page_of(0), fill = 0, stage = 0;  // the ring's places that are filled and read next
     auto issue = [&](int tile) {
       if (tile < tiles) {
         const int key = key0 + tile * C::kKeys + member * C::kLoadRows + lane;
         const bool ok = page >= 0 && page < p.pages;
         const int64_t off = ok ? page * p.stride_page + (int64_t)(key - divide(key, p.page) * p.page.d) * p.stride_slot : 0;
         const uint32_t seen = __ballot_sync(~0u, ok);
-        const int stage = tile % C::kStages;
-        if (lane == 0) s_seen[team][stage][member] = seen;
-        const uint32_t to = ring + stage * 2 * C::kHalf + copy_to;
+        if (lane == 0) s_seen[team][fill][member] = seen;
+        const uint32_t to = ring + fill * 2 * C::kHalf + copy_to;
+        fill = fill + 1 == C::kStages ? 0 : fill + 1;
 #pragma unroll
         for (int i = 0; i < (C::kLoadRows + C::kRowsPerCopy - 1) / C::kRowsPerCopy; ++i) {
           const int r = i * C::kRowsPerCopy + copy_row;  // of this warp's rows
@@ -378,11 +380,12 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       copy_wait<C::kStages - 2>();
       team_sync<TEAM>(team);
       issue(tile + C::kStages - 1);
-      const int stage = tile % C::kStages, key = key0 + tile * C::kKeys;
+      const int key = key0 + tile * C::kKeys;
       const uint32_t kt = ring + stage * 2 * C::kHalf, vt = kt + C::kHalf;
       uint32_t seen = 0;
 #pragma unroll
       for (int w = 0; w < TEAM; ++w) seen |= s_seen[team][stage][w] << (w * C::kLoadRows);
+      stage = stage + 1 == C::kStages ? 0 : stage + 1;
 
       float s[C::kKeys / 8][4];
 #pragma unroll
@@ -583,78 +586,156 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
   }
 }
 
-// Adds up what the workers that shared a head left. `kWarps` warps take the parts of one row in turn and are joined through shared memory: one
-// where there are many heads and few parts of each, four where few heads are in many parts.
-template <int ROWS, int UNIT, int kWarps>
+// Adds up what the workers that shared a head left: for row r of head `at` the parts of workers sh.x to sh.y. The first part's slot is sh.z; the others
+// begin their range with this head.
+__device__ __forceinline__ int64_t part_of(const int4& sh, int x) { return x == 0 ? (int64_t)sh.z : 2 * (int64_t)(sh.x + x); }
+
+// A warp per row, where a head has few parts.
+template <int ROWS, int UNIT>
 __global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(const AttendArgs p, float shift) {
-  constexpr int kGroups = kAttendWarps / kWarps;
-  __shared__ float4 s_sum[kAttendThreads];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % kWarps;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_wait();
   int rows = p.queries * p.group.d;
   if (rows > ROWS) rows = ROWS;
   const int64_t items = (int64_t)p.spans * p.kv_heads * rows;
-  for (int64_t first = (int64_t)blockIdx.x * kGroups; first < items; first += (int64_t)gridDim.x * kGroups) {
-    const int64_t item = first + warp / kWarps, at = item / rows;
+  for (int64_t item = (int64_t)blockIdx.x * kAttendWarps + warp; item < items; item += (int64_t)gridDim.x * kAttendWarps) {
+    const int64_t at = item / rows;
     const int r = (int)(item - at * rows), index = (int)(at / p.kv_heads), kv = (int)(at - (int64_t)index * p.kv_heads);
     const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row = (index - b * p.row_tiles) * ROWS + r;
-    if (kWarps == 1 && (item >= items || row >= p.queries * p.group.d)) continue;  // uniform in the block where it is more than a warp's matter
-    if (kWarps > 1 && row >= p.queries * p.group.d) continue;
+    if (row >= p.queries * p.group.d) continue;
     const int4 sh = p.shares[at];
     const int n = sh.y - sh.x + 1;
     if (n <= 1) continue;
-    auto slot_of = [&](int x) { return x == 0 ? (int64_t)sh.z : 2 * (int64_t)(sh.x + x); };  // the others begin with this head
-    float top = -INFINITY, sum = 0.0f;
-    for (int x = lane; x < n; x += 32) top = fmaxf(top, p.part_stats[slot_of(x) * ROWS + r].x);
+    float top = -INFINITY;
+    for (int x = lane; x < n; x += 32) top = fmaxf(top, p.part_stats[part_of(sh, x) * ROWS + r].x);
     for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
     const float base = top == -INFINITY ? 0.0f : top;
     const int i = divide(row, p.group), head = kv * p.group.d + row - i * p.group.d;
     const int64_t token = (int64_t)b * p.queries + i;
     const bool padding = i >= span_of<ROWS, UNIT>(p, index).count;
+    float sum = 0.0f;
     for (int e0 = 0; e0 < p.d; e0 += 128) {
       const int e = e0 + 4 * lane, column = e < p.d ? e : 0;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       sum = 0.0f;
       for (int x0 = 0; x0 < n; x0 += 32) {
-        const float2 st = x0 + lane < n ? p.part_stats[slot_of(x0 + lane) * ROWS + r] : make_float2(-INFINITY, 0.0f);
+        const float2 st = x0 + lane < n ? p.part_stats[part_of(sh, x0 + lane) * ROWS + r] : make_float2(-INFINITY, 0.0f);
         const float w = exp2_approx(st.x - base);
         sum += w * st.y;
         const int many = n - x0 < 32 ? n - x0 : 32;
-        for (int y0 = share; y0 < many; y0 += 8 * kWarps) {  // eight loads in flight
+        for (int y0 = 0; y0 < many; y0 += 8) {  // eight loads in flight
           float4 v[8];
           float wy[8];
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
-            const int z = y0 + y * kWarps, x = z < many ? z : many - 1;
-            wy[y] = __shfl_sync(~0u, w, z & 31);
-            v[y] = *reinterpret_cast<const float4*>(p.part_sums + (slot_of(x0 + x) * ROWS + r) * p.d + column);
+            const int x = y0 + y < many ? y0 + y : many - 1;
+            wy[y] = __shfl_sync(~0u, w, x);
+            v[y] = *reinterpret_cast<const float4*>(p.part_sums + (part_of(sh, x0 + x) * ROWS + r) * p.d + column);
           }
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
-            if (y0 + y * kWarps >= many) continue;
+            if (y0 + y >= many) continue;
             acc.x = fmaf(wy[y], v[y].x, acc.x), acc.y = fmaf(wy[y], v[y].y, acc.y), acc.z = fmaf(wy[y], v[y].z, acc.z), acc.w = fmaf(wy[y], v[y].w, acc.w);
           }
         }
       }
       for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
-      if constexpr (kWarps > 1) {
-        __syncthreads();
-        s_sum[threadIdx.x] = acc;
-        __syncthreads();
-        if (share == 0)
-          for (int x = 1; x < kWarps; ++x) {
-            const float4 v = s_sum[threadIdx.x + 32 * x];
-            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-          }
-      }
-      if (share == 0 && e < p.d) {
+      if (e < p.d) {
         const bool nothing = sum == 0.0f || padding;
         const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
         const uint2 w = make_uint2(pack_bf16x2(acc.x * finish, acc.y * finish), pack_bf16x2(acc.z * finish, acc.w * finish));
         *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = nothing ? make_uint2(0u, 0u) : w;
       }
     }
-    if (share == 0 && lane == 0 && p.lse) p.lse[token * p.q_heads + head] = sum == 0.0f || padding ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
+    if (lane == 0 && p.lse) p.lse[token * p.q_heads + head] = sum == 0.0f || padding ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
+  }
+}
+
+// A block per row, where few heads are in many parts: its warps take the parts in turn.
+constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32, kJoinMost = 2048;  // parts whose weights shared memory holds: all workers'
+
+__device__ __forceinline__ float2 join_all(float2 x, bool largest, float2* scratch) {  // .x: maximum or sum over the block
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = 16; i; i >>= 1) {
+    const float y = __shfl_xor_sync(~0u, x.x, i);
+    x.x = largest ? fmaxf(x.x, y) : x.x + y;
+  }
+  __syncthreads();
+  if (lane == 0) scratch[warp] = x;
+  __syncthreads();
+  float2 all = scratch[0];
+  for (int w = 1; w < kJoinWarps; ++w) all.x = largest ? fmaxf(all.x, scratch[w].x) : all.x + scratch[w].x;
+  return all;
+}
+
+template <int ROWS, int UNIT>
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_wide_kernel(const AttendArgs p, float shift) {
+  __shared__ float s_weight[kJoinMost];
+  __shared__ float2 s_scratch[kJoinWarps];
+  __shared__ float4 s_sum[kJoinThreads];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  griddep_wait();
+  int rows = p.queries * p.group.d;
+  if (rows > ROWS) rows = ROWS;
+  const int64_t items = (int64_t)p.spans * p.kv_heads * rows;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t at = item / rows;
+    const int r = (int)(item - at * rows), index = (int)(at / p.kv_heads), kv = (int)(at - (int64_t)index * p.kv_heads);
+    const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row = (index - b * p.row_tiles) * ROWS + r;
+    if (row >= p.queries * p.group.d) continue;
+    const int4 sh = p.shares[at];
+    const int n = sh.y - sh.x + 1;
+    if (n <= 1) continue;
+    float top = -INFINITY, sum = 0.0f;
+    float2 first = make_float2(-INFINITY, 0.0f);  // this thread's first statistics, of n <= 512 parts all
+    for (int x = threadIdx.x; x < n; x += kJoinThreads) {
+      const float2 st = p.part_stats[part_of(sh, x) * ROWS + r];
+      if (x == threadIdx.x) first = st;
+      top = fmaxf(top, st.x);
+    }
+    top = join_all(make_float2(top, 0.0f), true, s_scratch).x;
+    const float base = top == -INFINITY ? 0.0f : top;
+    for (int x = threadIdx.x; x < n; x += kJoinThreads) {
+      const float2 st = x == threadIdx.x ? first : p.part_stats[part_of(sh, x) * ROWS + r];
+      const float w = exp2_approx(st.x - base);
+      s_weight[x] = w;
+      sum = fmaf(w, st.y, sum);
+    }
+    sum = join_all(make_float2(sum, 0.0f), false, s_scratch).x;
+    const int i = divide(row, p.group), head = kv * p.group.d + row - i * p.group.d;
+    const int64_t token = (int64_t)b * p.queries + i;
+    const bool nothing = sum == 0.0f || i >= span_of<ROWS, UNIT>(p, index).count;
+    for (int e0 = 0; e0 < p.d; e0 += 128) {
+      const int e = e0 + 4 * lane, column = e < p.d ? e : 0;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int y0 = warp; y0 < n; y0 += 8 * kJoinWarps) {  // eight loads in flight
+        float4 v[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const int x = y0 + y * kJoinWarps < n ? y0 + y * kJoinWarps : y0;
+          v[y] = *reinterpret_cast<const float4*>(p.part_sums + (part_of(sh, x) * ROWS + r) * p.d + column);
+        }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          if (y0 + y * kJoinWarps >= n) continue;
+          const float w = s_weight[y0 + y * kJoinWarps];
+          acc.x = fmaf(w, v[y].x, acc.x), acc.y = fmaf(w, v[y].y, acc.y), acc.z = fmaf(w, v[y].z, acc.z), acc.w = fmaf(w, v[y].w, acc.w);
+        }
+      }
+      s_sum[threadIdx.x] = acc;
+      __syncthreads();
+      if (warp == 0 && e < p.d) {
+        for (int x = 1; x < kJoinWarps; ++x) {
+          const float4 v = s_sum[lane + 32 * x];
+          acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        }
+        const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
+        const uint2 w = make_uint2(pack_bf16x2(acc.x * finish, acc.y * finish), pack_bf16x2(acc.z * finish, acc.w * finish));
+        *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = nothing ? make_uint2(0u, 0u) : w;
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0 && p.lse) p.lse[token * p.q_heads + head] = nothing ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
   }
 }
 
@@ -695,11 +776,15 @@ tf_status AttendCall<DP, F8, ROWS>::launch(AttendArgs p, void* workspace_at, int
   p.shares = reinterpret_cast<int4*>(p.part_stats + parts);
   TF_CUDA(launch_dependent(true, kernel, dim3((unsigned)blocks), dim3(kAttendThreads), C::kSmem, stream, p));
   const int64_t rows = (int64_t)p.queries * p.group.d, items = heads * (rows < C::kRows ? rows : C::kRows);
-  // four warps to a row where a head may have more than eight parts
-  const bool few = heads * 8 < (int64_t)blocks * C::kTeams;
-  const int64_t groups = few ? items : (items + kAttendWarps - 1) / kAttendWarps, most = (int64_t)sm_count() * 8;
-  auto join = few ? paged_attention_join_kernel<C::kRows, C::kKeys, 4> : paged_attention_join_kernel<C::kRows, C::kKeys, 1>;
-  TF_CUDA(launch_dependent(true, join, dim3((unsigned)(groups < most ? groups : most)), dim3(kAttendThreads), 0, stream, p, C::kShift));
+  // a block to a row where a head has more than eight parts on average
+  const int workers = blocks * C::kTeams;
+  if (heads * 8 < workers && workers <= kJoinMost) {
+    const int64_t most = (int64_t)sm_count() * 4;
+    TF_CUDA(launch_dependent(true, paged_attention_join_wide_kernel<C::kRows, C::kKeys>, dim3((unsigned)(items < most ? items : most)), dim3(kJoinThreads), 0, stream, p, C::kShift));
+  } else {
+    const int64_t groups = (items + kAttendWarps - 1) / kAttendWarps, most = (int64_t)sm_count() * 8;
+    TF_CUDA(launch_dependent(true, paged_attention_join_kernel<C::kRows, C::kKeys>, dim3((unsigned)(groups < most ? groups : most)), dim3(kAttendThreads), 0, stream, p, C::kShift));
+  }
   return TF_OK;
 }
 
