@@ -7,19 +7,27 @@ namespace tf {
 
 extern template struct AttendCall<64, false, 8>;
 extern template struct AttendCall<64, false, 16>;
+extern template struct AttendCall<64, false, 24>;
 extern template struct AttendCall<64, false, 32>;
+extern template struct AttendCall<64, false, 48>;
 extern template struct AttendCall<64, false, 64>;
 extern template struct AttendCall<64, true, 8>;
 extern template struct AttendCall<64, true, 16>;
+extern template struct AttendCall<64, true, 24>;
 extern template struct AttendCall<64, true, 32>;
+extern template struct AttendCall<64, true, 48>;
 extern template struct AttendCall<64, true, 64>;
 extern template struct AttendCall<128, false, 8>;
 extern template struct AttendCall<128, false, 16>;
+extern template struct AttendCall<128, false, 24>;
 extern template struct AttendCall<128, false, 32>;
+extern template struct AttendCall<128, false, 48>;
 extern template struct AttendCall<128, false, 64>;
 extern template struct AttendCall<128, true, 8>;
 extern template struct AttendCall<128, true, 16>;
+extern template struct AttendCall<128, true, 24>;
 extern template struct AttendCall<128, true, 32>;
+extern template struct AttendCall<128, true, 48>;
 extern template struct AttendCall<128, true, 64>;
 extern template struct AttendCall<256, false, 8>;
 extern template struct AttendCall<256, false, 16>;
@@ -36,7 +44,13 @@ static auto with_attend_call(int64_t rows, int64_t d, int32_t dtype, Use use) {
   auto by_rows = [&](auto dp, auto f8) {
     constexpr int kDP = decltype(dp)::value;
     constexpr bool kF8 = decltype(f8)::value;
-    return rows <= 8 ? use(AttendCall<kDP, kF8, 8>{}) : rows <= 16 ? use(AttendCall<kDP, kF8, 16>{}) : rows <= 32 ? use(AttendCall<kDP, kF8, 32>{}) : use(AttendCall<kDP, kF8, 64>{});
+    if (rows <= 8) return use(AttendCall<kDP, kF8, 8>{});
+    if (rows <= 16) return use(AttendCall<kDP, kF8, 16>{});
+    if constexpr (kDP < 256) {
+      if (rows <= 24) return use(AttendCall<kDP, kF8, 24>{});
+      if (rows > 32 && rows <= 48) return use(AttendCall<kDP, kF8, 48>{});
+    }
+    return rows <= 32 ? use(AttendCall<kDP, kF8, 32>{}) : use(AttendCall<kDP, kF8, 64>{});
   };
   auto by_dim = [&](auto f8) {
     return d <= 64 ? by_rows(std::integral_constant<int, 64>{}, f8) : d <= 128 ? by_rows(std::integral_constant<int, 128>{}, f8) : by_rows(std::integral_constant<int, 256>{}, f8);

@@ -1,11 +1,12 @@
 // Attention of new tokens over a paged key-value cache, split over its length and joined.
 //
-// The rows of one kv head (its query heads times the new tokens) read the same keys, so they are the 16-row operand of mma.sync m16n8k16 and
-// keys stream through once. Bound by HBM: a bf16 key and value of 128 elements are 512 bytes for 4 * 128 operations per row, 24 bytes a clock
-// and SM, while 16 rows use about a tenth of the tensor cores and of the issue slots.
+// The rows of one kv head (its query heads times the new tokens) read the same keys, so keys stream through once, as the 16-row operand of
+// mma.sync m16n8k16: S^T = K Q^T and O^T = V^T P^T, rows in eights. (Rows as the 16-row operand took twice the products and accumulators for the
+// eight rows that most models have.) Bound by HBM: a bf16 key and value of 128 elements are 512 bytes for 512 operations per row, while eight
+// rows use about a twentieth of the tensor cores.
 //
-// One pass with a running maximum and sum (base 2, f32). The workers are single warps, or teams of 2 or 4 warps with 16 rows each where there are
-// more than 16 rows. Each has a ring of its own in shared memory, filled by cp.async, and never waits for another: while one waits for a
+// One pass with a running maximum and sum (base 2, f32). The workers are single warps, or teams of 2 or 4 warps with rows of their own where
+// one warp's registers do not hold them. Each has a ring of its own in shared memory, filled by cp.async, and never waits for another: while one waits for a
 // head's first keys, the others of its SM keep the memory busy.
 //
 // The work is the list of all (sequence, row tile, kv head), each as long as its tiles of keys and a fixed part for starting it, cut into as many
@@ -22,20 +23,24 @@ namespace tf {
 
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
 constexpr int kHeadCost = 1;  // what starting a head costs a worker, in tiles: about the latency of its first keys
+#ifndef ATT_KEYS
+#define ATT_KEYS (kRowBytes <= 128 && kEights == 1 ? 32 : 16)
+#define ATT_BPS (kEights * DP <= 128 ? 3 : 2)
+#define ATT_RING 196608
+#endif
 
-// ROWS query rows of a kv head: 8 or 16 by a warp of its own, 32 or 64 by a team of two or four.
+// ROWS query rows of a kv head, in eights: as many of them to a warp as its registers hold (an accumulator of DP x 8 takes DP / 4 of them), the rest to
+// a team of warps that share the keys' tiles.
 template <int DP, bool F8, int ROWS>
 struct AttendCfg {
-  static constexpr int kTeam = ROWS <= 16 ? 1 : ROWS / 16, kTeams = kAttendWarps / kTeam, kRows = ROWS;
-  static constexpr int kHalves = ROWS == 8 ? 1 : 2;  // a thread has rows r and r + 8 of the 16; with 8 rows the operand's other half is zero
+  static constexpr int kEights = DP == 256 ? (ROWS > 8 ? 2 : 1) : ROWS <= 32 ? ROWS / 8 : ROWS / 16, kTeam = ROWS / (8 * kEights);
+  static constexpr int kTeams = kAttendWarps / kTeam, kRows = ROWS;
   static constexpr int kRowBytes = DP * (F8 ? 1 : 2);
-  static constexpr int kKeys = kRowBytes >= (kTeam == 1 ? 256 : 512) ? 16 : 32;  // of a team's tile
-  static constexpr int kLoadRows = kKeys / kTeam;                               // of them, a warp loads
+  static constexpr int kKeys = ATT_KEYS;          // of a team's tile
+  static constexpr int kLoadRows = kKeys / kTeam;  // of them, a warp loads
   static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
-  // Two blocks an SM with rings of 96 KB, without spilled registers, keep more in flight than three with 64 KB (64 x 8192 bf16 195 -> 189 us, e4m3 122 -> 113); heads of up
-  // to 64 elements have registers for three, and little calls gain by the warps (a window of 1024: 21.3 us, 23.0 with two).
-  static constexpr int kBlocksPerSm = DP <= 64 ? 3 : DP <= 128 || F8 ? 2 : 1;
-  static constexpr int kFit = (kBlocksPerSm == 3 ? 65536 : kBlocksPerSm == 2 ? 98304 : 196608) / (kTeams * 2 * kHalf);
+  static constexpr int kBlocksPerSm = ATT_BPS;
+  static constexpr int kFit = (ATT_RING) / (kBlocksPerSm * kTeams * 2 * kHalf);
   static constexpr int kStages = kFit < 2 ? 2 : kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kTeams * kStages * 2 * kHalf;
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
@@ -74,6 +79,12 @@ __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of 16-bit elements, two neighbours of a row per thread, turned
+__device__ __forceinline__ uint32_t turn_matrix(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
@@ -171,7 +182,7 @@ __device__ __forceinline__ long long block_sum(long long x, long long* scratch) 
 template <int DP, bool F8, int ROWS>
 __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlocksPerSm)) paged_attention_kernel(const AttendArgs p) {
   using C = AttendCfg<DP, F8, ROWS>;
-  constexpr int TEAM = C::kTeam, kHalves = C::kHalves;
+  constexpr int TEAM = C::kTeam, NR = C::kEights, KT = C::kKeys / 16;
   extern __shared__ __align__(1024) uint8_t smem[];  // rows of the ring start on multiples of their size
   __shared__ long long s_scratch[kAttendWarps], s_before[C::kTeams];
   __shared__ int s_index[C::kTeams];
@@ -249,9 +260,10 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
   // step to another chunk, and to a row of the same instruction's series, is an exclusive or with a constant.
   auto swizzle = [](int row) { return C::kRowBytes >= 128 ? row & 7 : (row >> 1) & 3; };
   const uint32_t copy_to = (member * C::kLoadRows + copy_row) * C::kRowBytes + ((copy_chunk ^ swizzle(member * C::kLoadRows + copy_row)) << 4);
-  const int k_row = F8 ? (lane & 7) + (lane & 8) : (lane & 7) + ((lane >> 4) << 3), v_row = (lane & 7) + (lane & 8);
-  const uint32_t k_from = k_row * C::kRowBytes + (((F8 ? lane >> 4 : (lane >> 3) & 1) ^ swizzle(k_row)) << 4);
-  const uint32_t v_from = v_row * C::kRowBytes + (((lane >> 4) ^ swizzle(v_row)) << 4);
+  // matrix loads of four 8 x 8 blocks: K by (keys, keys + 8) x (chunk, chunk + 1), V in the same order for codes, turned and chunks first for bf16
+  const int k_row = (lane & 7) + (lane & 8), v_row = F8 ? k_row : (lane & 7) + ((lane >> 4) << 3);
+  const uint32_t k_from = k_row * C::kRowBytes + (((lane >> 4) ^ swizzle(k_row)) << 4);
+  const uint32_t v_from = v_row * C::kRowBytes + (((F8 ? lane >> 4 : (lane >> 3) & 1) ^ swizzle(v_row)) << 4);
 
   if (p.d < DP) {
     // the products run over DP elements: the keys' others are zero, as the queries' are (the values' give columns that nobody reads)
@@ -324,20 +336,14 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
 #pragma unroll
     for (int i = 0; i < C::kStages - 1; ++i) issue(i);
 
-    // this thread's two rows: the query operand, scale and limits
-    uint32_t qf[DP / 16][4];
-    float row_scale[kHalves];
-    int limit[kHalves], lowest[kHalves];
-    if constexpr (kHalves == 1) {
+    // The query operand: row lane / 4 of each eight. Scores and sums are of rows 2c and 2c + 1, c = lane % 4.
+    uint32_t qf[DP / 16][NR][2];
+    float row_scale[NR][2];
+    int limit[NR][2], lowest[NR][2];
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) qf[kk][1] = qf[kk][3] = 0u;
-    }
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const int r = row0 + member * 16 + (lane >> 2) + 8 * h, i = divide(r, p.group);
+    for (int n = 0; n < NR; ++n) {
+      const int r = row0 + member * 8 * NR + 8 * n + (lane >> 2), i = divide(r, p.group);
       const bool real = r < p.queries * p.group.d;
-      limit[h] = real && i < sp.count ? sp.length - sp.count + 1 + i : 0;
-      lowest[h] = p.window > 0 && limit[h] > p.window ? limit[h] - p.window : 0;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((int64_t)b * p.queries + i) * p.q_ldt + ((int64_t)kv * p.group.d + r - i * p.group.d) * p.q_ldh);
       float top = 0.0f;
 #pragma unroll
@@ -347,11 +353,11 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
           // a matrix load of e4m3 codes leaves four neighbours in a thread: elements 4c .. 4c + 3 stand at k = 2c, 2c + 1, 2c + 8, 2c + 9
           const int at = F8 ? kk * 8 + (lane & 3) * 2 + x : kk * 8 + (lane & 3) + 4 * x;
           const uint32_t w = real && kk * 16 < p.d ? src[at] : 0u;
-          qf[kk][h + 2 * x] = w;
+          qf[kk][n][x] = w;
           if constexpr (F8) top = fmaxf(top, fmaxf(fabsf(bf16lo_to_f32(w)), fabsf(bf16hi_to_f32(w))));
         }
       }
-      row_scale[h] = p.scale_log2;
+      row_scale[n][0] = row_scale[n][1] = p.scale_log2;
       if constexpr (F8) {
         // bf16 -> f16 without loss: the row is scaled by a power of two that puts its largest element into [2^14, 2^15)
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
@@ -363,18 +369,29 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const uint32_t w = qf[kk][h + 2 * x];
-            qf[kk][h + 2 * x] = pack_f16x2(bf16lo_to_f32(w) * a * c, bf16hi_to_f32(w) * a * c);
+            const uint32_t w = qf[kk][n][x];
+            qf[kk][n][x] = pack_f16x2(bf16lo_to_f32(w) * a * c, bf16hi_to_f32(w) * a * c);
           }
         const float ia = __uint_as_float((uint32_t)(127 - (up >> 1)) << 23), ic = __uint_as_float((uint32_t)(127 - (up - (up >> 1))) << 23);
-        row_scale[h] = row_scale[h] * (p.k_scale ? load_f32(p.k_scale + kv) : 1.0f) * ia * ic;
+        const float mine = p.scale_log2 * (p.k_scale ? load_f32(p.k_scale + kv) : 1.0f) * ia * ic;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) row_scale[n][h] = __shfl_sync(~0u, mine, (2 * (lane & 3) + h) * 4);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r2 = row0 + member * 8 * NR + 8 * n + 2 * (lane & 3) + h, i2 = divide(r2, p.group);
+        limit[n][h] = r2 < p.queries * p.group.d && i2 < sp.count ? sp.length - sp.count + 1 + i2 : 0;
+        lowest[n][h] = p.window > 0 && limit[n][h] > p.window ? limit[n][h] - p.window : 0;
       }
     }
-    float o[DP / 8][4], m[kHalves], l[kHalves];
+    float o[DP / 16][NR][4], m[NR][2], l[NR][2];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) m[h] = -INFINITY, l[h] = 0.0f;
+    for (int n = 0; n < NR; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < DP / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+      for (int t = 0; t < DP / 16; ++t) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.0f;
+    }
 
     for (int tile = 0; tile < tiles; ++tile) {
       copy_wait<C::kStages - 2>();
@@ -387,78 +404,93 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       for (int w = 0; w < TEAM; ++w) seen |= s_seen[team][stage][w] << (w * C::kLoadRows);
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
 
-      float s[C::kKeys / 8][4];
+      float s[KT][NR][4];  // keys 16 j + lane / 4 (+ 8 for the upper two) of rows 2c, 2c + 1
 #pragma unroll
-      for (int j = 0; j < C::kKeys / 8; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+      for (int j = 0; j < KT; ++j)
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.0f;
 #pragma unroll
       for (int kk = 0; kk < DP / 16; kk += F8 ? 2 : 1)
 #pragma unroll
-        for (int j = 0; j < C::kKeys / 16; ++j) {
+        for (int j = 0; j < KT; ++j) {
           uint32_t r[4];
           load_matrices(r, ((kt + k_from) ^ (kk << (F8 ? 4 : 5))) + j * 16 * C::kRowBytes);
           if constexpr (F8) {
-            multiply<true>(s[2 * j], qf[kk], codes_to_f16x2(r[0], false), codes_to_f16x2(r[0], true));
-            multiply<true>(s[2 * j + 1], qf[kk], codes_to_f16x2(r[1], false), codes_to_f16x2(r[1], true));
-            multiply<true>(s[2 * j], qf[kk + 1], codes_to_f16x2(r[2], false), codes_to_f16x2(r[2], true));
-            multiply<true>(s[2 * j + 1], qf[kk + 1], codes_to_f16x2(r[3], false), codes_to_f16x2(r[3], true));
+            const uint32_t a0[4] = {codes_to_f16x2(r[0], false), codes_to_f16x2(r[1], false), codes_to_f16x2(r[0], true), codes_to_f16x2(r[1], true)};
+            const uint32_t a1[4] = {codes_to_f16x2(r[2], false), codes_to_f16x2(r[3], false), codes_to_f16x2(r[2], true), codes_to_f16x2(r[3], true)};
+#pragma unroll
+            for (int n = 0; n < NR; ++n) multiply<true>(s[j][n], a0, qf[kk][n][0], qf[kk][n][1]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) multiply<true>(s[j][n], a1, qf[kk + 1][n][0], qf[kk + 1][n][1]);
           } else {
-            multiply<false>(s[2 * j], qf[kk], r[0], r[1]);
-            multiply<false>(s[2 * j + 1], qf[kk], r[2], r[3]);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) multiply<false>(s[j][n], r, qf[kk][n][0], qf[kk][n][1]);
           }
         }
 
       const bool whole = seen == (uint32_t)((1ull << C::kKeys) - 1);
       const bool inside = key >= sp.last_lo && key + C::kKeys <= sp.first;  // every row sees all of the tile's keys that anyone sees
 #pragma unroll
-      for (int j = 0; j < C::kKeys / 8; ++j)
+      for (int j = 0; j < KT; ++j)
 #pragma unroll
-        for (int x = 0; x < 2 * kHalves; ++x) s[j][x] *= row_scale[x >> 1];
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[j][n][x] *= row_scale[n][x & 1];
       if (!(whole && inside)) {
 #pragma unroll
-        for (int j = 0; j < C::kKeys / 8; ++j)
+        for (int j = 0; j < KT; ++j)
 #pragma unroll
-          for (int x = 0; x < 2 * kHalves; ++x) {
-            const int c = 8 * j + 2 * (lane & 3) + (x & 1), e = key + c;
-            if (!((seen >> c) & 1) || e < lowest[x >> 1] || e >= limit[x >> 1]) s[j][x] = -INFINITY;
-          }
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int c = 16 * j + (lane >> 2) + 8 * (x >> 1), e = key + c;
+              if (!((seen >> c) & 1) || e < lowest[n][x & 1] || e >= limit[n][x & 1]) s[j][n][x] = -INFINITY;
+            }
       }
-      float top[kHalves], base[kHalves];
+      float top[NR][2], base[NR][2];
       bool moved = false;
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        top[h] = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int j = 1; j < C::kKeys / 8; ++j) top[h] = fmaxf(top[h], fmaxf(s[j][2 * h], s[j][2 * h + 1]));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
-        top[h] = fmaxf(top[h], m[h]);
-        base[h] = top[h] == -INFINITY ? 0.0f : top[h];
-        moved |= top[h] != m[h];
-      }
+        for (int h = 0; h < 2; ++h) {
+          float t = fmaxf(s[0][n][h], s[0][n][2 + h]);
+#pragma unroll
+          for (int j = 1; j < KT; ++j) t = fmaxf(t, fmaxf(s[j][n][h], s[j][n][2 + h]));
+          t = fmaxf(t, __shfl_xor_sync(~0u, t, 4));
+          t = fmaxf(t, __shfl_xor_sync(~0u, t, 8));
+          t = fmaxf(t, __shfl_xor_sync(~0u, t, 16));
+          top[n][h] = t = fmaxf(t, m[n][h]);
+          base[n][h] = t == -INFINITY ? 0.0f : t;
+          moved |= t != m[n][h];
+        }
       if (__any_sync(~0u, moved)) {
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const float keep = exp2_approx(m[h] - base[h]);
-          l[h] *= keep;
-          m[h] = top[h];
+        for (int n = 0; n < NR; ++n)
 #pragma unroll
-          for (int j = 0; j < DP / 8; ++j) o[j][2 * h] *= keep, o[j][2 * h + 1] *= keep;
-        }
+          for (int h = 0; h < 2; ++h) {
+            const float keep = exp2_approx(m[n][h] - base[n][h]);
+            l[n][h] *= keep;
+            m[n][h] = top[n][h];
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) o[t][n][h] *= keep, o[t][n][2 + h] *= keep;
+          }
       }
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const float shift = C::kShift - base[h];
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int j = 0; j < C::kKeys / 8; ++j) {
-          s[j][2 * h] = exp2_approx(s[j][2 * h] + shift), s[j][2 * h + 1] = exp2_approx(s[j][2 * h + 1] + shift);
-          l[h] += s[j][2 * h] + s[j][2 * h + 1];
+        for (int h = 0; h < 2; ++h) {
+          const float shift = C::kShift - base[n][h];
+#pragma unroll
+          for (int j = 0; j < KT; ++j) {
+            s[j][n][h] = exp2_approx(s[j][n][h] + shift), s[j][n][2 + h] = exp2_approx(s[j][n][2 + h] + shift);
+            l[n][h] += s[j][n][h] + s[j][n][2 + h];
+          }
         }
-      }
 
       // A value that some rows see and others do not reaches both through the product, the latter with weight 0: harmless unless it is not finite.
       bool odd = false;
+      const uint8_t* values = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
       if (!inside) {
-        const uint8_t* values = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
         for (int i = lane; i < C::kKeys * chunks; i += 32) {
           const int row = i / chunks, ch = i - row * chunks;
           const uint4 w = *reinterpret_cast<const uint4*>(values + row * C::kRowBytes + ((ch ^ swizzle(row)) << 4));
@@ -475,21 +507,23 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       }
       if (!odd) {
 #pragma unroll
-        for (int j = 0; j < C::kKeys / 16; ++j) {
-          uint32_t hi[4] = {0u, 0u, 0u, 0u};
-          [[maybe_unused]] uint32_t lo[4] = {0u, 0u, 0u, 0u};
+        for (int j = 0; j < KT; ++j) {
+          uint32_t hi[NR][2];
+          [[maybe_unused]] uint32_t lo[NR][2];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {  // the scores' registers are the weights' operand: keys 2c, 2c + 1 and 2c + 8, 2c + 9 of rows r and r + 8
-            if (kHalves == 1 && (x & 1)) continue;
-            const float a = s[2 * j + (x >> 1)][2 * (x & 1)], c = s[2 * j + (x >> 1)][2 * (x & 1) + 1];
-            if constexpr (F8) {
-              hi[x] = pack_f16x2(a, c);
-            } else {
-              // 16 bits of a weight in two products: one of 8 bits would add an error as large as the result's own rounding
-              hi[x] = pack_bf16x2(a, c);
-              lo[x] = pack_bf16x2(a - bf16lo_to_f32(hi[x]), c - bf16hi_to_f32(hi[x]));
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // scores are (key, rows); the weights' operand wants (row, keys)
+              const float a = s[j][n][2 * x], c = s[j][n][2 * x + 1];
+              if constexpr (F8) {
+                hi[n][x] = turn_matrix(pack_f16x2(a, c));
+              } else {
+                // 16 bits of a weight in two products: one of 8 bits would add an error as large as the result's own rounding
+                const uint32_t w = pack_bf16x2(a, c);
+                hi[n][x] = turn_matrix(w);
+                lo[n][x] = turn_matrix(pack_bf16x2(a - bf16lo_to_f32(w), c - bf16hi_to_f32(w)));
+              }
             }
-          }
 #pragma unroll
           for (int t = 0; t < DP / 16; t += F8 ? 2 : 1) {
             uint32_t r[4];
@@ -497,44 +531,41 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
             if constexpr (F8) {
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                // a thread holds elements (2c', 2c' + 1) of two keys: bytes to (key, key + 1) pairs, the even elements in one product, the odd ones in another
+                // a thread holds elements (2i, 2i + 1), i = lane / 4, of two keys: bytes to (key, key + 1) pairs; the even elements are the operand's rows i, the odd ones 8 + i
                 const uint32_t w0 = __byte_perm(r[2 * x], 0, 0x3120), w1 = __byte_perm(r[2 * x + 1], 0, 0x3120);
-                multiply<true>(o[2 * (t + x)], hi, codes_to_f16x2(w0, false), codes_to_f16x2(w1, false));
-                multiply<true>(o[2 * (t + x) + 1], hi, codes_to_f16x2(w0, true), codes_to_f16x2(w1, true));
+                const uint32_t a[4] = {codes_to_f16x2(w0, false), codes_to_f16x2(w0, true), codes_to_f16x2(w1, false), codes_to_f16x2(w1, true)};
+#pragma unroll
+                for (int n = 0; n < NR; ++n) multiply<true>(o[t + x][n], a, hi[n][0], hi[n][1]);
               }
             } else {
-              multiply<false>(o[2 * t], hi, r[0], r[1]);
-              multiply<false>(o[2 * t + 1], hi, r[2], r[3]);
-              multiply<false>(o[2 * t], lo, r[0], r[1]);
-              multiply<false>(o[2 * t + 1], lo, r[2], r[3]);
+#pragma unroll
+              for (int n = 0; n < NR; ++n) multiply<false>(o[t][n], r, hi[n][0], hi[n][1]);
+#pragma unroll
+              for (int n = 0; n < NR; ++n) multiply<false>(o[t][n], r, lo[n][0], lo[n][1]);
             }
           }
         }
       } else {
-        const uint8_t* values = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
 #pragma unroll
-        for (int eight = 0; eight < C::kKeys / 8; ++eight)
+        for (int j = 0; j < 2 * KT; ++j)  // eight keys
 #pragma unroll 1
           for (int x8 = 0; x8 < 8; ++x8) {
-            const int c = 8 * eight + x8;
-            float w[kHalves];
-            bool sees[kHalves];
+            const int c = 8 * j + x8;
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-              const float w0 = s[eight][2 * h], w1 = s[eight][2 * h + 1];
-              w[h] = __shfl_sync(~0u, x8 & 1 ? w1 : w0, (lane & ~3) | (x8 >> 1));
-              sees[h] = ((seen >> c) & 1) && key + c >= lowest[h] && key + c < limit[h];
-            }
+            for (int n = 0; n < NR; ++n)
 #pragma unroll
-            for (int j = 0; j < DP / 8; ++j)
+              for (int h = 0; h < 2; ++h) {
+                const float w = __shfl_sync(~0u, s[j / 2][n][2 * (j & 1) + h], 4 * x8 + (lane & 3));
+                if (!((seen >> c) & 1) || key + c < lowest[n][h] || key + c >= limit[n][h]) continue;
 #pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int e = F8 ? (j >> 1) * 16 + 4 * (lane & 3) + 2 * x + (j & 1) : j * 8 + 2 * (lane & 3) + x, byte = F8 ? e : 2 * e;
-                const uint8_t* from = values + c * C::kRowBytes + (((byte >> 4) ^ swizzle(c)) << 4) + (byte & 15);
-                const float y = F8 ? e4m3_to_f32(*from) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(from));
+                for (int t = 0; t < DP / 16; ++t)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h)
-                  if (sees[h]) o[j][2 * h + x] = fmaf(w[h], y, o[j][2 * h + x]);
+                  for (int x = 0; x < 2; ++x) {
+                    const int e = 16 * t + (F8 ? 2 * (lane >> 2) + x : (lane >> 2) + 8 * x), byte = F8 ? e : 2 * e;
+                    const uint8_t* at = values + c * C::kRowBytes + (((byte >> 4) ^ swizzle(c)) << 4) + (byte & 15);
+                    const float y = F8 ? e4m3_to_f32(*at) : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(at));
+                    o[t][n][2 * x + h] = fmaf(w, y, o[t][n][2 * x + h]);
+                  }
               }
           }
       }
@@ -544,41 +575,59 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
     const bool all = tiles == sp.units;
     const float v_scale = p.v_scale ? load_f32(p.v_scale + kv) : 1.0f;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      l[h] += __shfl_xor_sync(~0u, l[h], 1);
-      l[h] += __shfl_xor_sync(~0u, l[h], 2);
-      const int in_tile = member * 16 + (lane >> 2) + 8 * h, r = row0 + in_tile;
-      if (r >= p.queries * p.group.d) continue;
-      if (all) {
-        const int i = divide(r, p.group), head = kv * p.group.d + r - i * p.group.d;
-        const int64_t token = (int64_t)b * p.queries + i;
-        const bool nothing = l[h] == 0.0f || i >= sp.count;  // padding went along unmasked
-        const float finish = v_scale / l[h];
-        __nv_bfloat16* row = p.out + token * p.out_ldt + head * p.out_ldh;
+    for (int n = 0; n < NR; ++n) {
+      const int in_tile = member * 8 * NR + 8 * n;
+      float finish[2];
+      bool nothing[2];
 #pragma unroll
-        for (int j = 0; j < DP / 8; j += F8 ? 2 : 1) {
-          const int e = j * 8 + (F8 ? 4 : 2) * (lane & 3);
-          if (e >= p.d) break;
-          if constexpr (F8) {
-            const uint2 w = make_uint2(pack_bf16x2(o[j][2 * h] * finish, o[j + 1][2 * h] * finish), pack_bf16x2(o[j][2 * h + 1] * finish, o[j + 1][2 * h + 1] * finish));
-            *reinterpret_cast<uint2*>(row + e) = nothing ? make_uint2(0u, 0u) : w;
+      for (int h = 0; h < 2; ++h) {
+        for (int x = 4; x < 32; x <<= 1) l[n][h] += __shfl_xor_sync(~0u, l[n][h], x);
+        const int r = row0 + in_tile + 2 * (lane & 3) + h, i = divide(r, p.group);
+        nothing[h] = l[n][h] == 0.0f || i >= sp.count;  // padding went along unmasked
+        finish[h] = v_scale / l[n][h];
+        if (lane < 4 && r < p.queries * p.group.d) {
+          if (!all)
+            p.part_stats[slot * C::kRows + r - row0] = make_float2(m[n][h], l[n][h]);
+          else if (p.lse)
+            p.lse[((int64_t)b * p.queries + i) * p.q_heads + kv * p.group.d + r - i * p.group.d] =
+                nothing[h] ? -INFINITY : (m[n][h] + log2f(l[n][h]) - C::kShift) * 0.6931471805599453f;
+        }
+      }
+      if (all) {
+        const int r = row0 + in_tile + (lane >> 2), i = divide(r, p.group);
+        __nv_bfloat16* row = p.out + ((int64_t)b * p.queries + i) * p.out_ldt + ((int64_t)kv * p.group.d + r - i * p.group.d) * p.out_ldh;
+        const bool real = r < p.queries * p.group.d;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+          uint32_t w[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            w[x] = turn_matrix(pack_bf16x2(nothing[0] ? 0.0f : o[t][n][2 * x] * finish[0], nothing[1] ? 0.0f : o[t][n][2 * x + 1] * finish[1]));
+          if (!real || 16 * t >= p.d) continue;
+          if constexpr (F8) {  // even and odd elements 4c, 4c + 2 and 4c + 1, 4c + 3
+            *reinterpret_cast<uint2*>(row + 16 * t + 4 * (lane & 3)) = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[0], w[1], 0x7632));
           } else {
-            *reinterpret_cast<uint32_t*>(row + e) = nothing ? 0u : pack_bf16x2(o[j][2 * h] * finish, o[j][2 * h + 1] * finish);
+            *reinterpret_cast<uint32_t*>(row + 16 * t + 2 * (lane & 3)) = w[0];
+            *reinterpret_cast<uint32_t*>(row + 16 * t + 8 + 2 * (lane & 3)) = w[1];
           }
         }
-        if ((lane & 3) == 0 && p.lse) p.lse[token * p.q_heads + head] = nothing ? -INFINITY : (m[h] + log2f(l[h]) - C::kShift) * 0.6931471805599453f;
       } else {
-        float* row = p.part_sums + (slot * C::kRows + in_tile) * p.d;
 #pragma unroll
-        for (int j = 0; j < DP / 8; j += F8 ? 2 : 1) {
-          const int e = j * 8 + (F8 ? 4 : 2) * (lane & 3);
-          if (e >= p.d) break;
-          if constexpr (F8)
-            *reinterpret_cast<float4*>(row + e) = make_float4(o[j][2 * h], o[j + 1][2 * h], o[j][2 * h + 1], o[j + 1][2 * h + 1]);
-          else
-            *reinterpret_cast<float2*>(row + e) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) {
+          const int r = in_tile + 2 * (lane & 3) + h;
+          if (row0 + r >= p.queries * p.group.d) continue;
+          float* row = p.part_sums + (slot * C::kRows + r) * p.d;
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) {
+            if (16 * t >= p.d) break;
+            if constexpr (F8) {
+              *reinterpret_cast<float2*>(row + 16 * t + 2 * (lane >> 2)) = make_float2(o[t][n][h], o[t][n][2 + h]);
+            } else {
+              row[16 * t + (lane >> 2)] = o[t][n][h];
+              row[16 * t + 8 + (lane >> 2)] = o[t][n][2 + h];
+            }
+          }
         }
-        if ((lane & 3) == 0) p.part_stats[slot * C::kRows + in_tile] = make_float2(m[h], l[h]);
       }
     }
     copy_wait<0>();

@@ -5,7 +5,9 @@ namespace tf {
 
 template struct AttendCall<128, false, 8>;
 template struct AttendCall<128, false, 16>;
+template struct AttendCall<128, false, 24>;
 template struct AttendCall<128, false, 32>;
+template struct AttendCall<128, false, 48>;
 template struct AttendCall<128, false, 64>;
 
 }  // namespace tf

@@ -5,7 +5,9 @@ namespace tf {
 
 template struct AttendCall<128, true, 8>;
 template struct AttendCall<128, true, 16>;
+template struct AttendCall<128, true, 24>;
 template struct AttendCall<128, true, 32>;
+template struct AttendCall<128, true, 48>;
 template struct AttendCall<128, true, 64>;
 
 }  // namespace tf
