@@ -45,8 +45,9 @@ struct AttendCfg {
   static constexpr int kSmem = kTeams * kStages * 2 * kHalf;
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
   static constexpr int kRowsPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
-  // an e4m3 entry is multiplied as f16: weights are scaled by 2^15 (the largest is 2^15), so that small ones keep their bits
-  static constexpr float kShift = F8 ? 15.0f : 0.0f;
+  // An e4m3 entry is multiplied as f16: weights are scaled by 2^kShift, so that the largest is 2^15 and small ones keep their bits.
+  static constexpr float kSlack = 8.0f;
+  static constexpr float kShift = F8 ? 15.0f - kSlack : 0.0f;
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -428,14 +429,22 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
           }
         }
 
+      // Exponents relative to the row's reference. It is a maximum of earlier keys and moves only when a key passes it by 2^kSlack (or is the first that
+      // is seen): weights up to that are as exact, and most tiles need neither the maximum over the warp nor the accumulators' rescaling.
       const bool whole = seen == (uint32_t)((1ull << C::kKeys) - 1);
       const bool inside = key >= sp.last_lo && key + C::kKeys <= sp.first;  // every row sees all of the tile's keys that anyone sees
+      float offset[NR][2];
+      bool moved = false;
 #pragma unroll
-      for (int j = 0; j < KT; ++j)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
+        for (int h = 0; h < 2; ++h) {
+          offset[n][h] = m[n][h] == -INFINITY ? 0.0f : C::kShift - m[n][h];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[j][n][x] *= row_scale[n][x & 1];
+          for (int j = 0; j < KT; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; x += 2) s[j][n][x + h] = fmaf(s[j][n][x + h], row_scale[n][h], offset[n][h]);
+        }
       if (!(whole && inside)) {
 #pragma unroll
         for (int j = 0; j < KT; ++j)
@@ -447,8 +456,7 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
               if (!((seen >> c) & 1) || e < lowest[n][x & 1] || e >= limit[n][x & 1]) s[j][n][x] = -INFINITY;
             }
       }
-      float top[NR][2], base[NR][2];
-      bool moved = false;
+      float top[NR][2];
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -456,36 +464,38 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
           float t = fmaxf(s[0][n][h], s[0][n][2 + h]);
 #pragma unroll
           for (int j = 1; j < KT; ++j) t = fmaxf(t, fmaxf(s[j][n][h], s[j][n][2 + h]));
-          t = fmaxf(t, __shfl_xor_sync(~0u, t, 4));
-          t = fmaxf(t, __shfl_xor_sync(~0u, t, 8));
-          t = fmaxf(t, __shfl_xor_sync(~0u, t, 16));
-          top[n][h] = t = fmaxf(t, m[n][h]);
-          base[n][h] = t == -INFINITY ? 0.0f : t;
-          moved |= t != m[n][h];
+          top[n][h] = t;
+          moved |= t > (m[n][h] == -INFINITY ? -INFINITY : C::kShift + C::kSlack);
         }
       if (__any_sync(~0u, moved)) {
 #pragma unroll
         for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float keep = exp2_approx(m[n][h] - base[n][h]);
+            float t = top[n][h];
+            t = fmaxf(t, __shfl_xor_sync(~0u, t, 4));
+            t = fmaxf(t, __shfl_xor_sync(~0u, t, 8));
+            t = fmaxf(t, __shfl_xor_sync(~0u, t, 16));
+            const float now = fmaxf(m[n][h], t - offset[n][h]);  // what was unset has offset 0
+            const float next = now == -INFINITY ? 0.0f : C::kShift - now;
+            const float keep = exp2_approx(m[n][h] - (now == -INFINITY ? 0.0f : now));
             l[n][h] *= keep;
-            m[n][h] = top[n][h];
+            m[n][h] = now;
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) o[t][n][h] *= keep, o[t][n][2 + h] *= keep;
+            for (int x = 0; x < DP / 16; ++x) o[x][n][h] *= keep, o[x][n][2 + h] *= keep;
+#pragma unroll
+            for (int j = 0; j < KT; ++j) s[j][n][h] += next - offset[n][h], s[j][n][2 + h] += next - offset[n][h];
           }
       }
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float shift = C::kShift - base[n][h];
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < KT; ++j) {
-            s[j][n][h] = exp2_approx(s[j][n][h] + shift), s[j][n][2 + h] = exp2_approx(s[j][n][2 + h] + shift);
+            s[j][n][h] = exp2_approx(s[j][n][h]), s[j][n][2 + h] = exp2_approx(s[j][n][2 + h]);
             l[n][h] += s[j][n][h] + s[j][n][2 + h];
           }
-        }
 
       // A value that some rows see and others do not reaches both through the product, the latter with weight 0: harmless unless it is not finite.
       bool odd = false;
