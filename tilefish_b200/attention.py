@@ -28,15 +28,43 @@ LAYOUTS = {"half": N.ROTARY_HALF, "interleaved": N.ROTARY_INTERLEAVED}
 _PI = Fraction("3.14159265358979323846264338327950288419716939937510")
 
 
-def _here(device) -> None:
+# A call's checks run in front of launches of a few microseconds: shape, strides and address of a tensor are asked for once and device indexes are
+# compared, and only a check that fails looks for what to say (a rotation of four tokens 14 -> 12 us a call).
+
+
+def _strides(shape, strides):
+    """The first two axes' strides, 0 for one that is never stepped along (its stride says nothing then)."""
+    return strides[0] if shape[0] > 1 else 0, strides[1] if shape[1] > 1 else 0
+
+
+def _here(index: int) -> None:
     current = _torch()._C._cuda_getDevice()
-    if device.index != current:
-        _pre(False, f"the tensors are on {device}, the current device is cuda:{current}: make it current (with torch.cuda.device(...))", "device")
+    if index != current:
+        _pre(False, f"the tensors are on cuda:{index}, the current device is cuda:{current}: make it current (with torch.cuda.device(...))", "device")
 
 
-def _stride(t, axis: int) -> int:
-    """An axis' stride, 0 for one that is never stepped along (its stride says nothing then)."""
-    return t.stride(axis) if t.shape[axis] > 1 else 0
+def _rows(t, name: str, dtype, index: Optional[int], unit: int, align: int):
+    """(shape, token stride, head stride, address) of a [tokens, heads, dim] tensor of ``dtype`` on device ``index`` (None: any): the last axis dense, the
+    others at strides that are multiples of ``unit`` elements."""
+    if not (isinstance(t, _torch().Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == 3 and (index is None or t.get_device() == index)):
+        _check(t, name, dtype, 3, None if index is None else _torch().device("cuda", index), align)
+    shape, strides, at = t.shape, t.stride(), t.data_ptr()
+    st, sh = _strides(shape, strides)
+    if (strides[2] != 1 and shape[2] > 1) or st % unit or sh % unit or at % align:
+        _pre(shape[2] <= 1 or strides[2] == 1, f"{name}: the last axis must be dense (strides {tuple(strides)})", "contiguous", name)
+        _pre(st % unit == 0 and sh % unit == 0, f"{name}: strides {tuple(strides)} must be multiples of {unit} elements", "alignment", name)
+        _pre(t.numel() == 0 or at % align == 0, f"{name}: the data pointer is not {align}-byte aligned", "pointer_alignment", name)
+    return shape, st, sh, at
+
+
+def _ints(t, name: str, n: Optional[int], index: int) -> int:
+    """The address of a dense int32 [n] tensor."""
+    torch = _torch()
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.get_device() == index and t.shape[0] == n and (n <= 1 or t.stride(0) == 1)):
+        _check(t, name, torch.int32, 1, torch.device("cuda", index), align=4)
+        _pre(t.shape[0] == n, f"{name}: {t.shape[0]} of them, expected {n}", "shape", name)
+        _dense(t, name)
+    return t.data_ptr()
 
 
 def _overlap(a, b) -> bool:
@@ -45,14 +73,6 @@ def _overlap(a, b) -> bool:
 
     (a0, a1), (b0, b1) = span(a), span(b)
     return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
-
-
-def _dense_inner(t, name: str, unit: int) -> None:
-    """The last axis dense, the others at any stride that is a multiple of ``unit`` elements."""
-    if t.stride(2) == 1 and _stride(t, 0) % unit == 0 and _stride(t, 1) % unit == 0:
-        return
-    _pre(t.shape[2] <= 1 or t.stride(2) == 1, f"{name}: the last axis must be dense (strides {tuple(t.stride())})", "contiguous", name)
-    _pre(_stride(t, 0) % unit == 0 and _stride(t, 1) % unit == 0, f"{name}: strides {tuple(t.stride())} must be multiples of {unit} elements", "alignment", name)
 
 
 def _result(t, name: str) -> None:
@@ -80,7 +100,7 @@ class RotaryTable:
     ``magnitude``  factor of the turned elements (long-context scalings use it); elements from rot on are left alone
     """
 
-    __slots__ = ("rot", "layout", "magnitude", "turns", "_layout")
+    __slots__ = ("rot", "layout", "magnitude", "turns", "index", "_layout")
 
     def __init__(self, inv_freq, *, layout: str = "half", magnitude: float = 1.0, device=None) -> None:
         torch = _torch()
@@ -96,6 +116,7 @@ class RotaryTable:
         _pre(all(math.isfinite(f) for f in values), "inv_freq: not finite", "argument", "inv_freq")
         self.rot, self.layout, self.magnitude, self._layout = 2 * len(values), layout, float(magnitude), LAYOUTS[layout]
         self.turns = torch.tensor(_turns(values), dtype=torch.int64, device=device if device is not None else "cuda")
+        self.index = self.turns.get_device()
 
     def __repr__(self) -> str:
         return f"RotaryTable(rot={self.rot}, {self.layout}, magnitude={self.magnitude:g})"
@@ -137,20 +158,23 @@ def rotary_frequencies(rot: int, *, base: float = 10000.0, scaling: Optional[str
     return [f * (k + (1 - k) / factor) for f, k in zip(inv, keep)], 0.1 * math.log(factor) + 1.0
 
 
-def _check_positions(positions, tokens: int, device) -> int:
+def _check_positions(positions, tokens: int, index: int):
+    """(address, 32 or 64)"""
     torch = _torch()
-    wide = isinstance(positions, torch.Tensor) and positions.dtype == torch.int64
-    _check(positions, "positions", torch.int64 if wide else torch.int32, 1, device, align=8 if wide else 4)
-    if positions.shape[0] != tokens:
-        _pre(False, f"positions: {positions.shape[0]} of them for {tokens} tokens", "shape", "positions")
-    _dense(positions, "positions")
-    return 64 if wide else 32
+    if isinstance(positions, torch.Tensor) and positions.dtype == torch.int64:
+        if not (positions.dim() == 1 and positions.get_device() == index and positions.shape[0] == tokens and (tokens <= 1 or positions.stride(0) == 1)):
+            _check(positions, "positions", torch.int64, 1, torch.device("cuda", index), align=8)
+            _pre(positions.shape[0] == tokens, f"positions: {positions.shape[0]} of them for {tokens} tokens", "shape", "positions")
+            _dense(positions, "positions")
+        return positions.data_ptr(), 64
+    return _ints(positions, "positions", tokens, index), 32
 
 
-def _check_table(table, dim: int, device) -> None:
-    _pre(isinstance(table, RotaryTable), f"expected a RotaryTable, got {type(table).__name__}", "dtype", "table")
-    if table.turns.device != device:
-        _pre(False, f"the table is on {table.turns.device}, the other arguments are on {device}", "device", "table")
+def _check_table(table, dim: int, index: int) -> None:
+    if not isinstance(table, RotaryTable):
+        _pre(False, f"expected a RotaryTable, got {type(table).__name__}", "dtype", "table")
+    if table.index != index:
+        _pre(False, f"the table is on {table.turns.device}, the other arguments are on cuda:{index}", "device", "table")
     if table.rot > dim:
         _pre(False, f"the table turns {table.rot} elements of a head of {dim}", "shape", "table")
 
@@ -161,30 +185,27 @@ def rotary(x, positions, table: RotaryTable, *, out=None, inverse: bool = False,
     Positions are int32 or int64 of any size: an angle is exact to 2^-65 turns times the position."""
     torch = _torch()
     f32 = isinstance(x, torch.Tensor) and x.dtype == torch.float32
-    dtype = torch.float32 if f32 else torch.bfloat16
-    item = 4 if f32 else 2
-    _check(x, "x", dtype, 3, align=item)
-    device = x.device
-    _here(device)
-    tokens, heads, dim = x.shape
-    _check_table(table, dim, device)
-    bits = _check_positions(positions, tokens, device)
-    _dense_inner(x, "x", 1)
-    _pre(dim <= 1024, f"x: head_dim {dim} is more than 1024", "unsupported", "x")
+    dtype, item = (torch.float32, 4) if f32 else (torch.bfloat16, 2)
+    shape, st, sh, xp = _rows(x, "x", dtype, None, 1, item)
+    tokens, heads, dim = shape
+    index = x.get_device()
+    _here(index)
+    _check_table(table, dim, index)
+    pp, bits = _check_positions(positions, tokens, index)
+    if dim > 1024:
+        _pre(False, f"x: head_dim {dim} is more than 1024", "unsupported", "x")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+        out = torch.empty_strided(shape, (heads * dim, dim, 1), dtype=dtype, device=x.device)
+        ot, oh, op = heads * dim, dim, out.data_ptr()
     else:
-        _check(out, "out", dtype, 3, device, align=item)
-        _pre(tuple(out.shape) == (tokens, heads, dim), f"out: shape {tuple(out.shape)}, expected {(tokens, heads, dim)}", "shape", "out")
-        _dense_inner(out, "out", 1)
+        oshape, ot, oh, op = _rows(out, "out", dtype, index, 1, item)
+        _pre(oshape == shape, f"out: shape {tuple(oshape)}, expected {tuple(shape)}", "shape", "out")
         _result(out, "out")
-        same = out.data_ptr() == x.data_ptr() and all(_stride(out, i) == _stride(x, i) for i in range(2))
-        _pre(same or not _overlap(out, x), "out overlaps x without being x", "alias", "out")
+        _pre((op == xp and ot == st and oh == sh) or not _overlap(out, x), "out overlaps x without being x", "alias", "out")
     if tokens == 0 or heads == 0:
         return out
-    N.check(N.load().tf_rotary(x.data_ptr(), N.TYPE_F32 if f32 else N.TYPE_BF16, tokens, heads, dim, _stride(x, 0), _stride(x, 1), positions.data_ptr(), bits,
-                               table.turns.data_ptr(), table.rot, table._layout, table.magnitude, 1 if inverse else 0, out.data_ptr(), _stride(out, 0),
-                               _stride(out, 1), _stream(stream)), "tf_rotary")
+    N.check(N.load().tf_rotary(xp, N.TYPE_F32 if f32 else N.TYPE_BF16, tokens, heads, dim, st, sh, pp, bits, table.turns.data_ptr(), table.rot, table._layout,
+                               table.magnitude, 1 if inverse else 0, op, ot, oh, _stream(stream)), "tf_rotary")
     return out
 
 
@@ -201,7 +222,7 @@ class PagedCache:
     Which pages belong to which sequence stands in the int32 [sequences, width] tables that the operators take, not here.
     """
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "_desc", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "index", "_desc", "_ref")
 
     def __init__(self, k, v, k_scale=None, v_scale=None) -> None:
         torch = _torch()
@@ -214,8 +235,8 @@ class PagedCache:
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         _pre(self.head_dim % 16 == 0 and self.head_dim <= 256, f"k: head_dim {self.head_dim} is not a multiple of 16 up to 256", "divisible", "k")
         _pre(k.stride(3) == 1 and v.stride(3) == 1, "k, v: the last axis must be dense", "contiguous", "k")
-        strides = [_stride(k, i) for i in range(3)]
-        _pre(strides == [_stride(v, i) for i in range(3)], f"v: strides {tuple(v.stride())}, expected those of k, {tuple(k.stride())}", "contiguous", "v")
+        strides = [k.stride(i) if k.shape[i] > 1 else 0 for i in range(3)]
+        _pre(strides == [v.stride(i) if v.shape[i] > 1 else 0 for i in range(3)], f"v: strides {tuple(v.stride())}, expected those of k, {tuple(k.stride())}", "contiguous", "v")
         _pre(all(s % unit == 0 for s in strides), f"k: strides {tuple(k.stride())} must be multiples of {unit} elements", "alignment", "k")
         axes = sorted((st, n) for st, n in zip(strides, k.shape[:3]) if n > 1)
         reach = self.head_dim
@@ -230,6 +251,7 @@ class PagedCache:
                 _dense(s, name)
                 _pre(s.shape[0] == self.kv_heads, f"{name}: {s.shape[0]} of them for {self.kv_heads} heads", "shape", name)
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
+        self.index = k.get_device()
         self._desc = N.PagedCacheDescriptor(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
                                             v_scale.data_ptr() if v_scale is not None else None, self.pages, self.page_size, self.kv_heads, self.head_dim,
                                             strides[0], strides[1], strides[2], N.CACHE_E4M3 if codes else N.CACHE_BF16, 0)
@@ -251,24 +273,30 @@ class PagedCache:
         return f"PagedCache({self.dtype}, pages={self.pages}, page_size={self.page_size}, kv_heads={self.kv_heads}, head_dim={self.head_dim})"
 
 
-def _check_tables(tables, device) -> None:
-    _check(tables, "tables", _torch().int32, 2, device, align=4)
-    _pre(tables.shape[1] > 0 and (tables.stride(1) == 1 or tables.shape[1] == 1), f"tables: rows must be dense and not empty (shape {tuple(tables.shape)})", "contiguous",
-         "tables")
+def _check_tables(tables, index: int):
+    """(rows, columns, row stride, address) of int32 page tables."""
+    torch = _torch()
+    if not (isinstance(tables, torch.Tensor) and tables.dtype == torch.int32 and tables.dim() == 2 and tables.get_device() == index):
+        _check(tables, "tables", torch.int32, 2, torch.device("cuda", index), align=4)
+    rows, cols = tables.shape
+    stride, inner = tables.stride()
+    if cols == 0 or (inner != 1 and cols > 1):
+        _pre(False, f"tables: rows must be dense and not empty (shape {tuple(tables.shape)})", "contiguous", "tables")
+    return rows, cols, stride if rows > 1 else 0, tables.data_ptr()
 
 
-def _check_int32(t, name: str, n: int, device) -> None:
-    _check(t, name, _torch().int32, 1, device, align=4)
-    _dense(t, name)
-    if t.shape[0] != n:
-        _pre(False, f"{name}: {t.shape[0]} of them, expected {n}", "shape", name)
+def _check_cache(cache) -> None:
+    if not isinstance(cache, PagedCache):
+        _pre(False, f"cache: expected a PagedCache, got {type(cache).__name__}", "dtype", "cache")
 
 
-def _check_heads(t, name: str, tokens: Optional[int], heads: Optional[int], dim: int, device) -> None:
-    _check(t, name, _torch().bfloat16, 3, device)
-    if (tokens is not None and t.shape[0] != tokens) or (heads is not None and t.shape[1] != heads) or t.shape[2] != dim:
-        _pre(False, f"{name}: shape {tuple(t.shape)}, expected [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, {dim}]", "shape", name)
-    _dense_inner(t, name, 8)
+def _heads(t, name: str, tokens: Optional[int], heads: Optional[int], dim: int, index: int):
+    """``_rows`` of bf16 queries, keys, values or results of that many tokens and heads (None: any)."""
+    got = _rows(t, name, _torch().bfloat16, index, 8, 16)
+    shape = got[0]
+    if (tokens is not None and shape[0] != tokens) or (heads is not None and shape[1] != heads) or shape[2] != dim:
+        _pre(False, f"{name}: shape {tuple(shape)}, expected [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, {dim}]", "shape", name)
+    return got
 
 
 def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=None, rotary: Optional[RotaryTable] = None, q_out=None, stream=None):
@@ -280,45 +308,46 @@ def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=Non
 
     A token with a negative position (padding), one beyond its table, a row outside the tables or a page outside the cache is not written. Two tokens
     for one entry: which of them stays is not specified."""
-    torch = _torch()
-    _pre(isinstance(cache, PagedCache), f"cache: expected a PagedCache, got {type(cache).__name__}", "dtype", "cache")
-    device, dim = cache.device, cache.head_dim
-    _here(device)
-    _check_heads(k, "k", None, cache.kv_heads, dim, device)
-    tokens = k.shape[0]
-    _check_heads(v, "v", tokens, cache.kv_heads, dim, device)
-    _check_tables(tables, device)
-    bits = _check_positions(positions, tokens, device)
+    _check_cache(cache)
+    index, dim = cache.index, cache.head_dim
+    _here(index)
+    kshape, kt, kh, kp = _heads(k, "k", None, cache.kv_heads, dim, index)
+    tokens = kshape[0]
+    _, vt, vh, vp = _heads(v, "v", tokens, cache.kv_heads, dim, index)
+    seqs, cols, table_stride, tp = _check_tables(tables, index)
+    pp, bits = _check_positions(positions, tokens, index)
     if rows is not None:
-        _check_int32(rows, "rows", tokens, device)
+        rp = _ints(rows, "rows", tokens, index)
     else:
-        _pre(tokens == 0 or (tables.shape[0] > 0 and tokens % tables.shape[0] == 0),
-             f"k: {tokens} tokens cannot be dealt out evenly to {tables.shape[0]} sequences; give rows", "divisible", "k")
+        rp = None
+        if tokens and (seqs == 0 or tokens % seqs):
+            _pre(False, f"k: {tokens} tokens cannot be dealt out evenly to {seqs} sequences; give rows", "divisible", "k")
     if rotary is not None:
-        _check_table(rotary, dim, device)
-    q_heads, qp, qs, qop, qos = 0, None, (0, 0), None, (0, 0)
-    if q is not None:
-        _check_heads(q, "q", tokens, None, dim, device)
-        q_heads = q.shape[1]
-        if q_out is None:
-            q_out = torch.empty((tokens, q_heads, dim), dtype=torch.bfloat16, device=device)
-        else:
-            _check_heads(q_out, "q_out", tokens, q_heads, dim, device)
-            _result(q_out, "q_out")
-            same = q_out.data_ptr() == q.data_ptr() and all(_stride(q_out, i) == _stride(q, i) for i in range(2))
-            _pre(same or not _overlap(q_out, q), "q_out overlaps q without being q", "alias", "q_out")
-        if q_heads:
-            qp, qs, qop, qos = q.data_ptr(), (_stride(q, 0), _stride(q, 1)), q_out.data_ptr(), (_stride(q_out, 0), _stride(q_out, 1))
+        _check_table(rotary, dim, index)
+        turns, rot, layout, magnitude = rotary.turns.data_ptr(), rotary.rot, rotary._layout, rotary.magnitude
     else:
-        _pre(q_out is None, "q_out without q", "argument", "q_out")
-    if tokens == 0 or tables.shape[0] == 0:
-        _pre(tokens == 0, "tables: no sequences", "shape", "tables")
+        turns, rot, layout, magnitude = None, 0, 0, 1.0
+    q_heads, qp, qt, qh, op, ot, oh = 0, None, 0, 0, None, 0, 0
+    if q is not None:
+        qshape, qt, qh, qp = _heads(q, "q", tokens, None, dim, index)
+        q_heads = qshape[1]
+        if q_out is None:
+            q_out = _torch().empty_strided(qshape, (q_heads * dim, dim, 1), dtype=q.dtype, device=cache.device)
+            ot, oh, op = q_heads * dim, dim, q_out.data_ptr()
+        else:
+            _, ot, oh, op = _heads(q_out, "q_out", tokens, q_heads, dim, index)
+            _result(q_out, "q_out")
+            _pre((op == qp and ot == qt and oh == qh) or not _overlap(q_out, q), "q_out overlaps q without being q", "alias", "q_out")
+        if q_heads == 0:
+            qp = op = None
+    elif q_out is not None:
+        _pre(False, "q_out without q", "argument", "q_out")
+    if tokens == 0:
         return q_out
-    N.check(N.load().tf_cache_append(cache._ref, k.data_ptr(), _stride(k, 0), _stride(k, 1), v.data_ptr(), _stride(v, 0), _stride(v, 1), tokens, tables.data_ptr(),
-                                     tables.shape[0], tables.shape[1], _stride(tables, 0), positions.data_ptr(), bits, rows.data_ptr() if rows is not None else None,
-                                     qp, q_heads, qs[0], qs[1], qop, qos[0], qos[1], rotary.turns.data_ptr() if rotary is not None else None,
-                                     rotary.rot if rotary is not None else 0, rotary._layout if rotary is not None else 0,
-                                     rotary.magnitude if rotary is not None else 1.0, _stream(stream)), "tf_cache_append")
+    if seqs == 0:
+        _pre(False, "tables: no sequences", "shape", "tables")
+    N.check(N.load().tf_cache_append(cache._ref, kp, kt, kh, vp, vt, vh, tokens, tp, seqs, cols, table_stride, pp, bits, rp, qp, q_heads, qt, qh, op, ot, oh, turns, rot,
+                                     layout, magnitude, _stream(stream)), "tf_cache_append")
     return q_out
 
 
@@ -344,18 +373,16 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
     exp(scale * q . k). A query that sees nothing (padding, an empty sequence) gets 0 and -inf. Entries on pages outside the cache are seen by nobody, and
     what is not seen does not matter, infinities and NaN included."""
     torch = _torch()
-    _pre(isinstance(cache, PagedCache), f"cache: expected a PagedCache, got {type(cache).__name__}", "dtype", "cache")
-    device, dim = cache.device, cache.head_dim
-    _here(device)
-    _check_heads(q, "q", None, None, dim, device)
-    _check_tables(tables, device)
-    tokens, heads = q.shape[0], q.shape[1]
-    seqs, width = tables.shape
-    _check_int32(lengths, "lengths", seqs, device)
-    if counts is not None:
-        _check_int32(counts, "counts", seqs, device)
-    if heads == 0 or heads % cache.kv_heads:
-        _pre(False, f"q: {heads} heads are not a multiple of the cache's {cache.kv_heads}", "divisible", "q")
+    _check_cache(cache)
+    index, dim, kv_heads = cache.index, cache.head_dim, cache.kv_heads
+    _here(index)
+    shape, qt, qh, qp = _heads(q, "q", None, None, dim, index)
+    tokens, heads = shape[0], shape[1]
+    seqs, width, table_stride, tp = _check_tables(tables, index)
+    lp = _ints(lengths, "lengths", seqs, index)
+    cp = _ints(counts, "counts", seqs, index) if counts is not None else None
+    if heads == 0 or heads % kv_heads:
+        _pre(False, f"q: {heads} heads are not a multiple of the cache's {kv_heads}", "divisible", "q")
     if tokens and (seqs == 0 or tokens % seqs):
         _pre(False, f"q: {tokens} tokens cannot be dealt out evenly to {seqs} sequences", "divisible", "q")
     if scale is None:
@@ -365,40 +392,39 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
     if window < 0:
         _pre(False, f"window: {window} is negative", "argument", "window")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=torch.bfloat16, device=device)
+        out = torch.empty_strided(shape, (heads * dim, dim, 1), dtype=q.dtype, device=cache.device)
+        ot, oh, op = heads * dim, dim, out.data_ptr()
     else:
-        _check_heads(out, "out", tokens, heads, dim, device)
+        _, ot, oh, op = _heads(out, "out", tokens, heads, dim, index)
         _result(out, "out")
         _pre(not _overlap(out, q), "out overlaps q", "alias", "out")
     if lse is not None:
-        _check(lse, "lse", torch.float32, 2, device, align=4)
+        _check(lse, "lse", torch.float32, 2, cache.device, align=4)
         _pre(tuple(lse.shape) == (tokens, heads), f"lse: shape {tuple(lse.shape)}, expected {(tokens, heads)}", "shape", "lse")
         _dense(lse, "lse")
         return_lse = True
     elif return_lse:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
+        lse = torch.empty_strided((tokens, heads), (heads, 1), dtype=torch.float32, device=cache.device)
     if tokens:
         queries = tokens // seqs
-        need = _workspace_bytes(device.index, seqs, queries, heads, cache.kv_heads, dim, cache._desc.dtype, width * cache.page_size)
+        need = _workspace_bytes(index, seqs, queries, heads, kv_heads, dim, cache._desc.dtype, width * cache.page_size)
         if need < 0:
             _pre(False, f"q: {seqs} sequences of {queries} queries are more than this operator takes", "unsupported", "q")
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            workspace, have = torch.empty(need, dtype=torch.uint8, device=cache.device), need
         else:
-            _check(workspace, "workspace", torch.uint8, 1, device)
+            _check(workspace, "workspace", torch.uint8, 1, cache.device)
             _dense(workspace, "workspace")
-            _pre(workspace.numel() >= need, f"workspace: {need} bytes needed", "workspace", "workspace")
-        N.check(N.load().tf_paged_attention(cache._ref, q.data_ptr(), _stride(q, 0), _stride(q, 1), seqs, queries, heads, tables.data_ptr(), width,
-                                            _stride(tables, 0), lengths.data_ptr(), counts.data_ptr() if counts is not None else None, scale, window, out.data_ptr(),
-                                            _stride(out, 0), _stride(out, 1), lse.data_ptr() if lse is not None else None,
-                                            workspace.data_ptr() if workspace is not None else None, workspace.numel() if workspace is not None else 0,
-                                            _stream(stream)), "tf_paged_attention")
+            have = workspace.numel()
+            _pre(have >= need, f"workspace: {need} bytes needed", "workspace", "workspace")
+        N.check(N.load().tf_paged_attention(cache._ref, qp, qt, qh, seqs, queries, heads, tp, width, table_stride, lp, cp, scale, window, op, ot, oh,
+                                            lse.data_ptr() if return_lse else None, workspace.data_ptr(), have, _stream(stream)), "tf_paged_attention")
     return (out, lse) if return_lse else out
 
 
 def attention_workspace_bytes(cache: PagedCache, sequences: int, queries: int, q_heads: int, width: int) -> int:
     """Bytes of the ``workspace`` that ``paged_attention`` takes for tables of ``width`` pages (for callers that keep one; it must not serve two calls at once)."""
-    return _workspace_bytes(cache.device.index, sequences, queries, q_heads, cache.kv_heads, cache.head_dim, cache._desc.dtype, width * cache.page_size)
+    return _workspace_bytes(cache.index, sequences, queries, q_heads, cache.kv_heads, cache.head_dim, cache._desc.dtype, width * cache.page_size)
 
 
 # ---- the block ------------------------------------------------------------------------------------------------------------------

@@ -23,12 +23,6 @@ namespace tf {
 
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
 constexpr int kHeadCost = 1;  // what starting a head costs a worker, in tiles: about the latency of its first keys
-#ifndef ATT_KEYS
-#define ATT_KEYS (kRowBytes <= 128 && kEights == 1 ? 32 : 16)
-#define ATT_BPS (kEights * DP <= 128 ? 3 : 2)
-#define ATT_RING 196608
-#endif
-
 // ROWS query rows of a kv head, in eights: as many of them to a warp as its registers hold (an accumulator of DP x 8 takes DP / 4 of them), the rest to
 // a team of warps that share the keys' tiles.
 template <int DP, bool F8, int ROWS>
@@ -36,11 +30,13 @@ struct AttendCfg {
   static constexpr int kEights = DP == 256 ? (ROWS > 8 ? 2 : 1) : ROWS <= 32 ? ROWS / 8 : ROWS / 16, kTeam = ROWS / (8 * kEights);
   static constexpr int kTeams = kAttendWarps / kTeam, kRows = ROWS;
   static constexpr int kRowBytes = DP * (F8 ? 1 : 2);
-  static constexpr int kKeys = ATT_KEYS;          // of a team's tile
+  // keys of a team's tile: a tile costs what ten copies do besides its keys, so 32 where two stages of them fit (e4m3 32 x 16384: 103 us, 116 with 16)
+  static constexpr int kKeys = kRowBytes <= 128 && kEights == 1 ? 32 : 16;
   static constexpr int kLoadRows = kKeys / kTeam;  // of them, a warp loads
   static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
-  static constexpr int kBlocksPerSm = ATT_BPS;
-  static constexpr int kFit = (ATT_RING) / (kBlocksPerSm * kTeams * 2 * kHalf);
+  // three blocks an SM where the registers allow it without spilling (64 x 8192 bf16 183 us, 187 with two and a third stage)
+  static constexpr int kBlocksPerSm = kEights * DP <= 128 ? 3 : 2;
+  static constexpr int kFit = 196608 / (kBlocksPerSm * kTeams * 2 * kHalf);
   static constexpr int kStages = kFit < 2 ? 2 : kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kTeams * kStages * 2 * kHalf;
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
@@ -55,9 +51,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 16 bytes global -> shared without registers; zeros where `bytes` is 0 (the address is then not read).
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// 16 bytes global -> shared without registers, where `on`; zeros where `bytes` is 0 (the address is then not read).
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes, bool on) {
+  asm volatile("{ .reg .pred p;\n setp.ne.s32 p, %3, 0;\n @p cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2; }" ::"r"(dst), "l"(src), "r"(bytes), "r"((int)on) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -302,8 +298,8 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
 
     // the pages of a tile's rows are asked for a tile ahead of the copies
     const int32_t* table = p.tables + b * p.table_stride;
-    const uint8_t* kbase = p.k + kv * p.stride_head;
-    const uint8_t* vbase = p.v + kv * p.stride_head;
+    const uint8_t* kbase = p.k + kv * p.stride_head + copy_chunk * 16;
+    const uint8_t* vbase = p.v + kv * p.stride_head + copy_chunk * 16;
     auto page_of = [&](int tile) {
       const int key = key0 + tile * C::kKeys + member * C::kLoadRows + lane;
       return tile < tiles && lane < C::kLoadRows && key < sp.hi ? table[divide(key, p.page)] : -1;
@@ -323,12 +319,10 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
           const int r = i * C::kRowsPerCopy + copy_row;  // of this warp's rows
           const int64_t o = __shfl_sync(~0u, off, r & 31);
           const int bytes = (seen >> (r & 31)) & 1 ? 16 : 0;
-          if (C::kLoadRows % C::kRowsPerCopy && r >= C::kLoadRows) continue;
-          if (copy_chunk < chunks) {
-            const uint32_t dst = (to ^ (swizzle(i * C::kRowsPerCopy) << 4)) + i * C::kRowsPerCopy * C::kRowBytes;
-            copy_async(dst, kbase + o + copy_chunk * 16, bytes);
-            copy_async(dst + C::kHalf, vbase + o + copy_chunk * 16, bytes);
-          }
+          const bool on = copy_chunk < chunks && (C::kLoadRows % C::kRowsPerCopy == 0 || r < C::kLoadRows);
+          const uint32_t dst = (to ^ (swizzle(i * C::kRowsPerCopy) << 4)) + i * C::kRowsPerCopy * C::kRowBytes;
+          copy_async(dst, kbase + o, bytes, on);
+          copy_async(dst + C::kHalf, vbase + o, bytes, on);
         }
         page = page_of(tile + 1);
       }
