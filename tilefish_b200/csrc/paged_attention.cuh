@@ -296,35 +296,60 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
     const int b = p.row_tiles == 1 ? span : span / p.row_tiles, row0 = (span - b * p.row_tiles) * C::kRows;
     const int key0 = sp.start + unit * C::kKeys;
 
-    // the pages of a tile's rows are asked for a tile ahead of the copies
+    // The lanes hold 64 neighbouring entries of the table, asked for long before they are used.
     const int32_t* table = p.tables + b * p.table_stride;
+    const int last_column = divide(sp.hi - 1, p.page);
+    auto entries_at = [&](int column) { return column + lane <= last_column ? table[column + lane] : -1; };
+    int column0 = divide(key0, p.page), entries0 = entries_at(column0), entries1 = entries_at(column0 + 32);
     const uint8_t* kbase = p.k + kv * p.stride_head + copy_chunk * 16;
     const uint8_t* vbase = p.v + kv * p.stride_head + copy_chunk * 16;
-    auto page_of = [&](int tile) {
-      const int key = key0 + tile * C::kKeys + member * C::kLoadRows + lane;
-      return tile < tiles && lane < C::kLoadRows && key < sp.hi ? table[divide(key, p.page)] : -1;
-    };
-    int page = page_of(0), fill = 0, stage = 0;  // the ring's places that are filled and read next
+    int fill = 0, stage = 0;  // the ring's places that are filled and read next
     auto issue = [&](int tile) {
       if (tile < tiles) {
-        const int key = key0 + tile * C::kKeys + member * C::kLoadRows + lane;
-        const bool ok = page >= 0 && page < p.pages;
-        const int64_t off = ok ? page * p.stride_page + (int64_t)(key - divide(key, p.page) * p.page.d) * p.stride_slot : 0;
-        const uint32_t seen = __ballot_sync(~0u, ok);
-        if (lane == 0) s_seen[team][fill][member] = seen;
-        const uint32_t to = ring + fill * 2 * C::kHalf + copy_to;
-        fill = fill + 1 == C::kStages ? 0 : fill + 1;
-#pragma unroll
-        for (int i = 0; i < (C::kLoadRows + C::kRowsPerCopy - 1) / C::kRowsPerCopy; ++i) {
-          const int r = i * C::kRowsPerCopy + copy_row;  // of this warp's rows
-          const int64_t o = __shfl_sync(~0u, off, r & 31);
-          const int bytes = (seen >> (r & 31)) & 1 ? 16 : 0;
-          const bool on = copy_chunk < chunks && (C::kLoadRows % C::kRowsPerCopy == 0 || r < C::kLoadRows);
-          const uint32_t dst = (to ^ (swizzle(i * C::kRowsPerCopy) << 4)) + i * C::kRowsPerCopy * C::kRowBytes;
-          copy_async(dst, kbase + o, bytes, on);
-          copy_async(dst + C::kHalf, vbase + o, bytes, on);
+        const int first = key0 + tile * C::kKeys, column = divide(first, p.page);
+        if (column - column0 >= 32) {  // a tile has at most 32 pages
+          column0 += 32;
+          entries0 = entries1;
+          entries1 = entries_at(column0 + 32);
         }
-        page = page_of(tile + 1);
+        const uint32_t to = ring + fill * 2 * C::kHalf + copy_to;
+        uint32_t seen;
+        if (p.whole_tiles) {  // pages hold whole tiles: one page for all rows
+          const int page = __shfl_sync(~0u, entries0, column - column0), many = sp.hi - first < C::kKeys ? sp.hi - first : C::kKeys;
+          const bool ok = page >= 0 && page < p.pages;
+          seen = ok ? (uint32_t)((1ull << many) - 1) : 0u;
+          int64_t o = ok ? page * p.stride_page + (int64_t)(first - column * p.page.d + member * C::kLoadRows + copy_row) * p.stride_slot : 0;
+          const int left = ok ? many - member * C::kLoadRows - copy_row : 0;
+#pragma unroll
+          for (int i = 0; i < (C::kLoadRows + C::kRowsPerCopy - 1) / C::kRowsPerCopy; ++i) {
+            const bool on = copy_chunk < chunks && (C::kLoadRows % C::kRowsPerCopy == 0 || i * C::kRowsPerCopy + copy_row < C::kLoadRows);
+            const uint32_t dst = (to ^ (swizzle(i * C::kRowsPerCopy) << 4)) + i * C::kRowsPerCopy * C::kRowBytes;
+            const bool have = i * C::kRowsPerCopy < left;
+            const int64_t at = have ? o : 0;
+            copy_async(dst, kbase + at, have ? 16 : 0, on);
+            copy_async(dst + C::kHalf, vbase + at, have ? 16 : 0, on);
+            o += (int64_t)C::kRowsPerCopy * p.stride_slot;
+          }
+        } else {
+          const int key = first + member * C::kLoadRows + lane, col = divide(key, p.page), at = col - column0;
+          const int e0 = __shfl_sync(~0u, entries0, at & 31), e1 = __shfl_sync(~0u, entries1, at & 31), page = at < 32 ? e0 : e1;
+          const bool ok = lane < C::kLoadRows && key < sp.hi && page >= 0 && page < p.pages;
+          const int64_t off = ok ? page * p.stride_page + (int64_t)(key - col * p.page.d) * p.stride_slot : 0;
+          seen = __ballot_sync(~0u, ok);
+#pragma unroll
+          for (int i = 0; i < (C::kLoadRows + C::kRowsPerCopy - 1) / C::kRowsPerCopy; ++i) {
+            const int r = i * C::kRowsPerCopy + copy_row;  // of this warp's rows
+            const int64_t o = __shfl_sync(~0u, off, r & 31);
+            const int bytes = (seen >> (r & 31)) & 1 ? 16 : 0;
+            const bool on = copy_chunk < chunks && (C::kLoadRows % C::kRowsPerCopy == 0 || r < C::kLoadRows);
+            const uint32_t dst = (to ^ (swizzle(i * C::kRowsPerCopy) << 4)) + i * C::kRowsPerCopy * C::kRowBytes;
+            copy_async(dst, kbase + o, bytes, on);
+            copy_async(dst + C::kHalf, vbase + o, bytes, on);
+          }
+          seen <<= member * C::kLoadRows;
+        }
+        if (lane == 0) s_seen[team][fill][member] = seen;
+        fill = fill + 1 == C::kStages ? 0 : fill + 1;
       }
       copy_commit();
     };
@@ -396,7 +421,7 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       const uint32_t kt = ring + stage * 2 * C::kHalf, vt = kt + C::kHalf;
       uint32_t seen = 0;
 #pragma unroll
-      for (int w = 0; w < TEAM; ++w) seen |= s_seen[team][stage][w] << (w * C::kLoadRows);
+      for (int w = 0; w < TEAM; ++w) seen |= s_seen[team][stage][w];
       stage = stage + 1 == C::kStages ? 0 : stage + 1;
 
       float s[KT][NR][4];  // keys 16 j + lane / 4 (+ 8 for the upper two) of rows 2c, 2c + 1
@@ -822,6 +847,7 @@ tf_status AttendCall<DP, F8, ROWS>::launch(AttendArgs p, void* workspace_at, int
     TF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     configured_dev = dev;
   }
+  p.whole_tiles = p.page.d % C::kKeys == 0;
   const int blocks = attend_blocks<DP, F8, ROWS>(p.spans, p.kv_heads, p.entries);
   const int64_t parts = 2 * (int64_t)blocks * C::kTeams * C::kRows, heads = (int64_t)p.spans * p.kv_heads;
   p.part_sums = static_cast<float*>(workspace_at);

@@ -15,6 +15,7 @@ struct AttendArgs {
   int64_t stride_page, stride_head, stride_slot;  // bytes
   int pages, kv_heads, d;
   Divisor page;
+  bool whole_tiles;  // the page size is a multiple of the kernel's tile
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
   float* lse;
