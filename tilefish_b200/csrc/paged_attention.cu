@@ -9,14 +9,30 @@ extern template struct AttendCall<64, false, 8>;
 extern template struct AttendCall<64, false, 16>;
 extern template struct AttendCall<64, false, 24>;
 extern template struct AttendCall<64, false, 32>;
+extern template struct AttendCall<64, false, 40>;
 extern template struct AttendCall<64, false, 48>;
 extern template struct AttendCall<64, false, 64>;
 extern template struct AttendCall<64, true, 8>;
 extern template struct AttendCall<64, true, 16>;
 extern template struct AttendCall<64, true, 24>;
 extern template struct AttendCall<64, true, 32>;
+extern template struct AttendCall<64, true, 40>;
 extern template struct AttendCall<64, true, 48>;
 extern template struct AttendCall<64, true, 64>;
+extern template struct AttendCall<96, false, 8>;
+extern template struct AttendCall<96, false, 16>;
+extern template struct AttendCall<96, false, 24>;
+extern template struct AttendCall<96, false, 32>;
+extern template struct AttendCall<96, false, 40>;
+extern template struct AttendCall<96, false, 48>;
+extern template struct AttendCall<96, false, 64>;
+extern template struct AttendCall<96, true, 8>;
+extern template struct AttendCall<96, true, 16>;
+extern template struct AttendCall<96, true, 24>;
+extern template struct AttendCall<96, true, 32>;
+extern template struct AttendCall<96, true, 40>;
+extern template struct AttendCall<96, true, 48>;
+extern template struct AttendCall<96, true, 64>;
 extern template struct AttendCall<128, false, 8>;
 extern template struct AttendCall<128, false, 16>;
 extern template struct AttendCall<128, false, 24>;
@@ -48,12 +64,14 @@ static auto with_attend_call(int64_t rows, int64_t d, int32_t dtype, Use use) {
     if (rows <= 16) return use(AttendCall<kDP, kF8, 16>{});
     if constexpr (kDP < 256) {
       if (rows <= 24) return use(AttendCall<kDP, kF8, 24>{});
+      if constexpr (kDP < 128)  // 40 rows of 128 elements are more than a warp's registers
+        if (rows > 32 && rows <= 40) return use(AttendCall<kDP, kF8, 40>{});
       if (rows > 32 && rows <= 48) return use(AttendCall<kDP, kF8, 48>{});
     }
     return rows <= 32 ? use(AttendCall<kDP, kF8, 32>{}) : use(AttendCall<kDP, kF8, 64>{});
   };
   auto by_dim = [&](auto f8) {
-    return d <= 64 ? by_rows(std::integral_constant<int, 64>{}, f8) : d <= 128 ? by_rows(std::integral_constant<int, 128>{}, f8) : by_rows(std::integral_constant<int, 256>{}, f8);
+    return d <= 64 ? by_rows(std::integral_constant<int, 64>{}, f8) : d <= 96 ? by_rows(std::integral_constant<int, 96>{}, f8) : d <= 128 ? by_rows(std::integral_constant<int, 128>{}, f8) : by_rows(std::integral_constant<int, 256>{}, f8);
   };
   return dtype == TF_CACHE_E4M3 ? by_dim(std::true_type{}) : by_dim(std::false_type{});
 }
@@ -77,7 +95,7 @@ extern "C" int64_t tf_paged_attention_workspace_bytes(int64_t seqs, int64_t quer
   if (!attend_sizes_ok(seqs, queries, q_heads, kv_heads) || head_dim < 16 || head_dim > 256 || head_dim % 16 || max_entries < 1 || cache_dtype < 0 || cache_dtype > 1) return -1;
   const int64_t rows = queries * (q_heads / kv_heads), entries = max_entries > INT32_MAX / 2 ? INT32_MAX / 2 : max_entries;
   if (seqs == 0) return 0;
-  return with_attend_call(rows, head_dim, cache_dtype, [&](auto call) { return decltype(call)::workspace(seqs * attend_row_tiles(rows), kv_heads, head_dim, entries); });
+  return with_attend_call(rows, head_dim, cache_dtype, [&](auto call) { return decltype(call)::workspace(seqs * attend_row_tiles(rows), kv_heads, entries); });
 }
 
 extern "C" tf_status tf_paged_attention(const tf_paged_cache* cache, const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t seqs, int64_t queries,

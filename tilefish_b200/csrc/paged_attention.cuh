@@ -22,25 +22,29 @@
 namespace tf {
 
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
-constexpr int kHeadCost = 1;  // what starting a head costs a worker, in tiles: about the latency of its first keys
+constexpr int kHeadCost = 3;  // what starting a head costs a worker, in tiles: 3 to 4 us to its first keys, a tile 1 to 2
 // ROWS query rows of a kv head, in eights: as many of them to a warp as its registers hold (an accumulator of DP x 8 takes DP / 4 of them), the rest to
 // a team of warps that share the keys' tiles.
 template <int DP, bool F8, int ROWS>
 struct AttendCfg {
-  static constexpr int kEights = DP == 256 ? (ROWS > 8 ? 2 : 1) : ROWS <= 32 ? ROWS / 8 : ROWS / 16, kTeam = ROWS / (8 * kEights);
+  static constexpr int kEights = DP == 256 ? (ROWS > 8 ? 2 : 1) : ROWS <= 40 ? ROWS / 8 : ROWS / 16, kTeam = ROWS / (8 * kEights);
   static constexpr int kTeams = kAttendWarps / kTeam, kRows = ROWS;
-  static constexpr int kRowBytes = DP * (F8 ? 1 : 2);
+  static constexpr int kItem = F8 ? 1 : 2, kRowBytes = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) * kItem;  // of a staged row: a power of two
+  // The query operand takes half the accumulators' registers. Where both do not fit it is read from shared memory with every tile.
+  static constexpr bool kQueriesInRegisters = kEights * DP <= 384;
+  static constexpr int kQueryBytes = kQueriesInRegisters ? 0 : 8 * kEights * (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) * 2;  // of a warp
   // keys of a team's tile: a tile costs what ten copies do besides its keys, so 32 where two stages of them fit (e4m3 32 x 16384: 103 us, 116 with 16)
   static constexpr int kKeys = kRowBytes <= 128 && kEights == 1 ? 32 : 16;
   static constexpr int kLoadRows = kKeys / kTeam;  // of them, a warp loads
   static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
   // three blocks an SM where the registers allow it without spilling (64 x 8192 bf16 183 us, 187 with two and a third stage)
-  static constexpr int kBlocksPerSm = kEights * DP <= 128 ? 3 : 2;
-  static constexpr int kFit = 196608 / (kBlocksPerSm * kTeams * 2 * kHalf);
+  static constexpr int kBlocksPerSm = DP == 256 && !F8 ? 1 : kEights * DP <= 128 ? 3 : 2;
+  static constexpr int kFit = (200704 - kBlocksPerSm * kAttendWarps * kQueryBytes) / (kBlocksPerSm * kTeams * 2 * kHalf);
   static constexpr int kStages = kFit < 2 ? 2 : kFit > 6 ? 6 : kFit;
-  static constexpr int kSmem = kTeams * kStages * 2 * kHalf;
+  static constexpr int kRing = kTeams * kStages * 2 * kHalf, kSmem = kRing + kAttendWarps * kQueryBytes;
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
   static constexpr int kRowsPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
+  static_assert(kBlocksPerSm * (kSmem + 2560) <= 228 * 1024 && kSmem <= 225 * 1024, "the grid counts on so many blocks an SM");
   // An e4m3 entry is multiplied as f16: weights are scaled by 2^kShift, so that the largest is 2^15 and small ones keep their bits.
   static constexpr float kSlack = 8.0f;
   static constexpr float kShift = F8 ? 15.0f - kSlack : 0.0f;
@@ -167,91 +171,87 @@ struct Ranges {
   }
 };
 
-// Sums over a block of 128 threads. `scratch` holds one value per warp; the caller does not touch it without a barrier.
-__device__ __forceinline__ long long block_sum(long long x, long long* scratch) {
-  for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(~0u, x, i);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-  __syncthreads();
-  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
-}
+// Writes the results of eight rows, from `row` on, whose sums are in the registers' order: a thread has rows 2c and 2c + 1, c = lane % 4, of elements
+// 16 t + lane / 4 and 8 more, or, of e4m3 values, 16 t + 2 (lane / 4) and one more.
+template <bool F8>
+struct Finish {
+  float scale[2];
+  bool nothing[2];
+  __nv_bfloat16* out;  // of row lane / 4
+  int64_t lse[2];      // -1: there is no such row
+  bool real;
+  __device__ __forceinline__ Finish(const AttendArgs& p, const Span& sp, int b, int kv, int row, float v_scale, float2 sum) {
+    const int lane = threadIdx.x & 31, rows = p.queries * p.group.d;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row + 2 * (lane & 3) + h, i = divide(r, p.group);
+      const float l = h ? sum.y : sum.x;
+      nothing[h] = l == 0.0f || i >= sp.count;  // padding goes along unmasked
+      scale[h] = v_scale / l;
+      lse[h] = r < rows ? ((int64_t)b * p.queries + i) * p.q_heads + kv * p.group.d + r - i * p.group.d : -1;
+    }
+    const int r = row + (lane >> 2), i = divide(r, p.group);
+    real = r < rows;
+    out = p.out + ((int64_t)b * p.queries + i) * p.out_ldt + ((int64_t)kv * p.group.d + r - i * p.group.d) * p.out_ldh;
+  }
+  __device__ __forceinline__ void write_lse(const AttendArgs& p, float2 top, float2 sum, float shift) const {
+    if (!p.lse) return;
+    if (lse[0] >= 0) p.lse[lse[0]] = nothing[0] ? -INFINITY : (top.x + log2f(sum.x) - shift) * 0.6931471805599453f;
+    if (lse[1] >= 0) p.lse[lse[1]] = nothing[1] ? -INFINITY : (top.y + log2f(sum.y) - shift) * 0.6931471805599453f;
+  }
+  __device__ __forceinline__ void write(const AttendArgs& p, int t, float4 x) const {
+    const int c = threadIdx.x & 3;
+    const uint32_t w0 = turn_matrix(pack_bf16x2(nothing[0] ? 0.0f : x.x * scale[0], nothing[1] ? 0.0f : x.y * scale[1]));
+    const uint32_t w1 = turn_matrix(pack_bf16x2(nothing[0] ? 0.0f : x.z * scale[0], nothing[1] ? 0.0f : x.w * scale[1]));
+    if (!real || 16 * t >= p.d) return;
+    if constexpr (F8) {  // even and odd elements 4c, 4c + 2 and 4c + 1, 4c + 3
+      *reinterpret_cast<uint2*>(out + 16 * t + 4 * c) = make_uint2(__byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632));
+    } else {
+      *reinterpret_cast<uint32_t*>(out + 16 * t + 2 * c) = w0;
+      *reinterpret_cast<uint32_t*>(out + 16 * t + 8 + 2 * c) = w1;
+    }
+  }
+};
 
 template <int DP, bool F8, int ROWS>
 __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlocksPerSm)) paged_attention_kernel(const AttendArgs p) {
   using C = AttendCfg<DP, F8, ROWS>;
   constexpr int TEAM = C::kTeam, NR = C::kEights, KT = C::kKeys / 16;
+  constexpr bool kInRegisters = C::kQueriesInRegisters;
   extern __shared__ __align__(1024) uint8_t smem[];  // rows of the ring start on multiples of their size
-  __shared__ long long s_scratch[kAttendWarps], s_before[C::kTeams];
-  __shared__ int s_index[C::kTeams];
   __shared__ uint32_t s_seen[C::kTeams][C::kStages][TEAM];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, team = warp / TEAM, member = warp % TEAM;
   griddep_wait();
   griddep_launch_dependents();  // the join: its blocks find room as this kernel's leave
   const int worker = blockIdx.x * C::kTeams + team;
 
-  // the workers' ranges of the list, and where in it this block's begin
+  // The workers' ranges of the list, and where in it this one's begins: every lane takes a few neighbouring spans, every warp for itself.
   auto cost_of = [&](int i) {
     const int units = i < p.spans ? span_of<C::kRows, C::kKeys>(p, i).units : 0;
     return units ? units + kHeadCost : 0;
   };
-  const int chunk_cost = cost_of(threadIdx.x);
-  long long total = 0;
-  if (p.spans > kAttendThreads) {
-    long long mine = chunk_cost;
-    for (int i = threadIdx.x + kAttendThreads; i < p.spans; i += kAttendThreads) mine += cost_of(i);
-    total = block_sum(mine, s_scratch) * p.kv_heads;
+  const int share = (p.spans + 31) / 32;
+  long long cost = cost_of(lane * share);
+#pragma unroll 8
+  for (int i = 1; i < share; ++i) cost += cost_of(lane * share + i);
+  long long upto = cost;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const long long y = __shfl_up_sync(~0u, upto, x);
+    if (lane >= x) upto += y;
   }
-  Ranges ranges;
-  long long run = 0;  // cost of the spans before this chunk
-  for (int at = 0;; at += kAttendThreads) {
-    const int c = at == 0 ? chunk_cost : cost_of(at + threadIdx.x);
-    long long upto = c;
-    for (int x = 1; x < 32; x <<= 1) {
-      const long long y = __shfl_up_sync(~0u, upto, x);
-      if (lane >= x) upto += y;
-    }
-    __syncthreads();
-    if (lane == 31) s_scratch[warp] = upto;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) upto += s_scratch[w];
-    upto += run;
-    run += s_scratch[0] + s_scratch[1] + s_scratch[2] + s_scratch[3];
-    if (at == 0) {
-      if (p.spans <= kAttendThreads) total = run * p.kv_heads;
-      ranges = Ranges::of(total, (int)gridDim.x * C::kTeams);
-    }
-    long long last = -1;  // the last range of the block begins here
-    for (int t = 0; t < C::kTeams; ++t) {
-      const int w = (int)blockIdx.x * C::kTeams + t;
-      if (w >= ranges.workers) break;
-      last = ranges.begin(w);
-      if ((upto - c) * p.kv_heads <= last && last < upto * p.kv_heads) {
-        s_index[t] = at + threadIdx.x;
-        s_before[t] = (upto - c) * p.kv_heads;
-      }
-    }
-    if (last < run * p.kv_heads) break;
-  }
-  // heads whose rows see nothing
-  for (int i = blockIdx.x; i < p.spans; i += gridDim.x) {
-    if (span_of<C::kRows, C::kKeys>(p, i).units) continue;
-    const int b = p.row_tiles == 1 ? i : i / p.row_tiles, row0 = (i - b * p.row_tiles) * C::kRows;
-    int rows = p.queries * p.group.d - row0;
-    if (rows > C::kRows) rows = C::kRows;
-    for (int x = warp; x < rows * p.kv_heads; x += kAttendWarps) {
-      const int kv = x / rows, r = row0 + x - kv * rows, q = divide(r, p.group), head = kv * p.group.d + r - q * p.group.d;
-      const int64_t token = (int64_t)b * p.queries + q;
-      for (int e = 4 * lane; e < p.d; e += 128) *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = make_uint2(0u, 0u);
-      if (lane == 0 && p.lse) p.lse[token * p.q_heads + head] = -INFINITY;
-    }
-    for (int x = threadIdx.x; x < p.kv_heads; x += kAttendThreads) p.shares[(int64_t)i * p.kv_heads + x] = make_int4(0, 0, 0, 0);
-  }
-  __syncthreads();
+  const Ranges ranges = Ranges::of(__shfl_sync(~0u, upto, 31) * p.kv_heads, (int)gridDim.x * C::kTeams);
   if (worker >= ranges.workers) return;
   const long long u0 = ranges.begin(worker), u1 = ranges.begin(worker + 1);
+  const int owner = __popc(__ballot_sync(~0u, upto * p.kv_heads <= u0));  // the lane whose spans u0 falls into
+  int index = owner * share;
+  long long before = __shfl_sync(~0u, upto - cost, owner) * p.kv_heads;  // where span `index` begins
+  if (share > 1)
+    for (long long c = (long long)cost_of(index) * p.kv_heads; u0 >= before + c; c = (long long)cost_of(index) * p.kv_heads) before += c, ++index;
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + team * C::kStages * 2 * C::kHalf;
-  const int chunks = p.d * (F8 ? 1 : 2) / 16;  // of a staged row, that hold data
+  [[maybe_unused]] uint8_t* queries = smem + C::kRing + warp * C::kQueryBytes;  // this warp's, written and read by the same threads
+  const int chunks = p.d * C::kItem / 16;  // of a staged row, that hold data
   const int copy_row = lane / C::kChunks, copy_chunk = lane % C::kChunks;
   // Chunk c of row r lies at c ^ swizzle(r): the eight rows of a matrix load are in other banks. Rows start on multiples of their size, so a
   // step to another chunk, and to a row of the same instruction's series, is an exclusive or with a constant.
@@ -272,8 +272,6 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
     }
   }
 
-  int index = s_index[team];
-  long long before = s_before[team];
   for (long long u = u0; u < u1;) {
     const Span sp = span_of<C::kRows, C::kKeys>(p, index);
     if (sp.units == 0) {
@@ -357,7 +355,7 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
     for (int i = 0; i < C::kStages - 1; ++i) issue(i);
 
     // The query operand: row lane / 4 of each eight. Scores and sums are of rows 2c and 2c + 1, c = lane % 4.
-    uint32_t qf[DP / 16][NR][2];
+    uint32_t qf[kInRegisters ? DP / 16 : 1][NR][2];
     float row_scale[NR][2];
     int limit[NR][2], lowest[NR][2];
 #pragma unroll
@@ -366,15 +364,15 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       const bool real = r < p.queries * p.group.d;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((int64_t)b * p.queries + i) * p.q_ldt + ((int64_t)kv * p.group.d + r - i * p.group.d) * p.q_ldh);
       float top = 0.0f;
+      uint32_t w[DP / 16][2];
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           // a matrix load of e4m3 codes leaves four neighbours in a thread: elements 4c .. 4c + 3 stand at k = 2c, 2c + 1, 2c + 8, 2c + 9
           const int at = F8 ? kk * 8 + (lane & 3) * 2 + x : kk * 8 + (lane & 3) + 4 * x;
-          const uint32_t w = real && kk * 16 < p.d ? src[at] : 0u;
-          qf[kk][n][x] = w;
-          if constexpr (F8) top = fmaxf(top, fmaxf(fabsf(bf16lo_to_f32(w)), fabsf(bf16hi_to_f32(w))));
+          w[kk][x] = real && kk * 16 < p.d ? src[at] : 0u;
+          if constexpr (F8) top = fmaxf(top, fmaxf(fabsf(bf16lo_to_f32(w[kk][x])), fabsf(bf16hi_to_f32(w[kk][x]))));
         }
       }
       row_scale[n][0] = row_scale[n][1] = p.scale_log2;
@@ -388,14 +386,18 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t w = qf[kk][n][x];
-            qf[kk][n][x] = pack_f16x2(bf16lo_to_f32(w) * a * c, bf16hi_to_f32(w) * a * c);
-          }
+          for (int x = 0; x < 2; ++x) w[kk][x] = pack_f16x2(bf16lo_to_f32(w[kk][x]) * a * c, bf16hi_to_f32(w[kk][x]) * a * c);
         const float ia = __uint_as_float((uint32_t)(127 - (up >> 1)) << 23), ic = __uint_as_float((uint32_t)(127 - (up - (up >> 1))) << 23);
         const float mine = p.scale_log2 * (p.k_scale ? load_f32(p.k_scale + kv) : 1.0f) * ia * ic;
 #pragma unroll
         for (int h = 0; h < 2; ++h) row_scale[n][h] = __shfl_sync(~0u, mine, (2 * (lane & 3) + h) * 4);
+      }
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        if constexpr (kInRegisters)
+          qf[kk][n][0] = w[kk][0], qf[kk][n][1] = w[kk][1];
+        else  // in the order of use: a thread's two words of a step, neighbours' behind one another
+          *reinterpret_cast<uint2*>(queries + ((kk * NR + n) * 32 + lane) * 8) = make_uint2(w[kk][0], w[kk][1]);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -430,7 +432,19 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
 #pragma unroll
         for (int n = 0; n < NR; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.0f;
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; kk += F8 ? 2 : 1)
+      for (int kk = 0; kk < DP / 16; kk += F8 ? 2 : 1) {
+        uint32_t q[F8 ? 2 : 1][NR][2];
+#pragma unroll
+        for (int y = 0; y < (F8 ? 2 : 1); ++y)
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            if constexpr (kInRegisters) {
+              q[y][n][0] = qf[kk + y][n][0], q[y][n][1] = qf[kk + y][n][1];
+            } else {
+              const uint2 w = *reinterpret_cast<const uint2*>(queries + (((kk + y) * NR + n) * 32 + lane) * 8);
+              q[y][n][0] = w.x, q[y][n][1] = w.y;
+            }
+          }
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
           uint32_t r[4];
@@ -439,14 +453,15 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
             const uint32_t a0[4] = {codes_to_f16x2(r[0], false), codes_to_f16x2(r[1], false), codes_to_f16x2(r[0], true), codes_to_f16x2(r[1], true)};
             const uint32_t a1[4] = {codes_to_f16x2(r[2], false), codes_to_f16x2(r[3], false), codes_to_f16x2(r[2], true), codes_to_f16x2(r[3], true)};
 #pragma unroll
-            for (int n = 0; n < NR; ++n) multiply<true>(s[j][n], a0, qf[kk][n][0], qf[kk][n][1]);
+            for (int n = 0; n < NR; ++n) multiply<true>(s[j][n], a0, q[0][n][0], q[0][n][1]);
 #pragma unroll
-            for (int n = 0; n < NR; ++n) multiply<true>(s[j][n], a1, qf[kk + 1][n][0], qf[kk + 1][n][1]);
+            for (int n = 0; n < NR; ++n) multiply<true>(s[j][n], a1, q[1][n][0], q[1][n][1]);
           } else {
 #pragma unroll
-            for (int n = 0; n < NR; ++n) multiply<false>(s[j][n], r, qf[kk][n][0], qf[kk][n][1]);
+            for (int n = 0; n < NR; ++n) multiply<false>(s[j][n], r, q[0][n][0], q[0][n][1]);
           }
         }
+      }
 
       // Exponents relative to the row's reference. It is a maximum of earlier keys and moves only when a key passes it by 2^kSlack (or is the first that
       // is seen): weights up to that are as exact, and most tiles need neither the maximum over the warp nor the accumulators' rescaling.
@@ -600,63 +615,26 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       }
     }
 
-    // the result, or this worker's part of it
+    // the result, or this worker's part of it: its registers in their order
     const bool all = tiles == sp.units;
     const float v_scale = p.v_scale ? load_f32(p.v_scale + kv) : 1.0f;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const int in_tile = member * 8 * NR + 8 * n;
-      float finish[2];
-      bool nothing[2];
+      const int eight = member * NR + n;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h)
         for (int x = 4; x < 32; x <<= 1) l[n][h] += __shfl_xor_sync(~0u, l[n][h], x);
-        const int r = row0 + in_tile + 2 * (lane & 3) + h, i = divide(r, p.group);
-        nothing[h] = l[n][h] == 0.0f || i >= sp.count;  // padding went along unmasked
-        finish[h] = v_scale / l[n][h];
-        if (lane < 4 && r < p.queries * p.group.d) {
-          if (!all)
-            p.part_stats[slot * C::kRows + r - row0] = make_float2(m[n][h], l[n][h]);
-          else if (p.lse)
-            p.lse[((int64_t)b * p.queries + i) * p.q_heads + kv * p.group.d + r - i * p.group.d] =
-                nothing[h] ? -INFINITY : (m[n][h] + log2f(l[n][h]) - C::kShift) * 0.6931471805599453f;
-        }
-      }
       if (all) {
-        const int r = row0 + in_tile + (lane >> 2), i = divide(r, p.group);
-        __nv_bfloat16* row = p.out + ((int64_t)b * p.queries + i) * p.out_ldt + ((int64_t)kv * p.group.d + r - i * p.group.d) * p.out_ldh;
-        const bool real = r < p.queries * p.group.d;
+        const Finish<F8> to(p, sp, b, kv, row0 + 8 * eight, v_scale, make_float2(l[n][0], l[n][1]));
+        if (lane < 4) to.write_lse(p, make_float2(m[n][0], m[n][1]), make_float2(l[n][0], l[n][1]), C::kShift);
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t) {
-          uint32_t w[2];
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            w[x] = turn_matrix(pack_bf16x2(nothing[0] ? 0.0f : o[t][n][2 * x] * finish[0], nothing[1] ? 0.0f : o[t][n][2 * x + 1] * finish[1]));
-          if (!real || 16 * t >= p.d) continue;
-          if constexpr (F8) {  // even and odd elements 4c, 4c + 2 and 4c + 1, 4c + 3
-            *reinterpret_cast<uint2*>(row + 16 * t + 4 * (lane & 3)) = make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[0], w[1], 0x7632));
-          } else {
-            *reinterpret_cast<uint32_t*>(row + 16 * t + 2 * (lane & 3)) = w[0];
-            *reinterpret_cast<uint32_t*>(row + 16 * t + 8 + 2 * (lane & 3)) = w[1];
-          }
-        }
+        for (int t = 0; t < DP / 16; ++t) to.write(p, t, make_float4(o[t][n][0], o[t][n][1], o[t][n][2], o[t][n][3]));
       } else {
+        float4* part = p.part_sums + ((slot * (C::kRows / 8) + eight) * (DP / 16)) * 32 + lane;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = in_tile + 2 * (lane & 3) + h;
-          if (row0 + r >= p.queries * p.group.d) continue;
-          float* row = p.part_sums + (slot * C::kRows + r) * p.d;
-#pragma unroll
-          for (int t = 0; t < DP / 16; ++t) {
-            if (16 * t >= p.d) break;
-            if constexpr (F8) {
-              *reinterpret_cast<float2*>(row + 16 * t + 2 * (lane >> 2)) = make_float2(o[t][n][h], o[t][n][2 + h]);
-            } else {
-              row[16 * t + (lane >> 2)] = o[t][n][h];
-              row[16 * t + 8 + (lane >> 2)] = o[t][n][2 + h];
-            }
-          }
-        }
+        for (int t = 0; t < DP / 16; ++t)
+          if (16 * t < p.d) part[t * 32] = make_float4(o[t][n][0], o[t][n][1], o[t][n][2], o[t][n][3]);
+        if (lane < 4) p.part_stats[(slot * (C::kRows / 8) + eight) * 4 + lane] = make_float4(m[n][0], m[n][1], l[n][0], l[n][1]);
       }
     }
     copy_wait<0>();
@@ -664,156 +642,96 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
   }
 }
 
-// Adds up what the workers that shared a head left: for row r of head `at` the parts of workers sh.x to sh.y. The first part's slot is sh.z; the others
-// begin their range with this head.
-__device__ __forceinline__ int64_t part_of(const int4& sh, int x) { return x == 0 ? (int64_t)sh.z : 2 * (int64_t)(sh.x + x); }
+// Adds up what the workers that shared a head left, and writes the rows that see nothing. A group of kWarps warps has one eight of rows and 32 of their
+// elements; its warps take the parts in turn, each with a maximum of its own, and are joined through shared memory: one warp where a head has few parts, eight
+// where few heads are in many.
+constexpr int kJoinThreads = 256, kJoinColumns = 2;  // of 16 elements
 
-// A warp per row, where a head has few parts.
-template <int ROWS, int UNIT>
-__global__ void __launch_bounds__(kAttendThreads) paged_attention_join_kernel(const AttendArgs p, float shift) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+template <int DP, bool F8, int ROWS, int UNIT, int kWarps>
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const AttendArgs p, float shift) {
+  constexpr int kEights = ROWS / 8, kSteps = DP / 16, kGroups = kJoinThreads / 32 / kWarps, kTake = 4;
+  __shared__ float4 s_stats[kJoinThreads / 32][4], s_sums[kWarps > 1 ? kJoinThreads / 32 : 1][kJoinColumns][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % kWarps;
   griddep_wait();
-  int rows = p.queries * p.group.d;
-  if (rows > ROWS) rows = ROWS;
-  const int64_t items = (int64_t)p.spans * p.kv_heads * rows;
-  for (int64_t item = (int64_t)blockIdx.x * kAttendWarps + warp; item < items; item += (int64_t)gridDim.x * kAttendWarps) {
-    const int64_t at = item / rows;
-    const int r = (int)(item - at * rows), index = (int)(at / p.kv_heads), kv = (int)(at - (int64_t)index * p.kv_heads);
-    const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row = (index - b * p.row_tiles) * ROWS + r;
-    if (row >= p.queries * p.group.d) continue;
-    const int4 sh = p.shares[at];
-    const int n = sh.y - sh.x + 1;
-    if (n <= 1) continue;
-    float top = -INFINITY;
-    for (int x = lane; x < n; x += 32) top = fmaxf(top, p.part_stats[part_of(sh, x) * ROWS + r].x);
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-    const float base = top == -INFINITY ? 0.0f : top;
-    const int i = divide(row, p.group), head = kv * p.group.d + row - i * p.group.d;
-    const int64_t token = (int64_t)b * p.queries + i;
-    const bool padding = i >= span_of<ROWS, UNIT>(p, index).count;
-    float sum = 0.0f;
-    for (int e0 = 0; e0 < p.d; e0 += 128) {
-      const int e = e0 + 4 * lane, column = e < p.d ? e : 0;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      sum = 0.0f;
-      for (int x0 = 0; x0 < n; x0 += 32) {
-        const float2 st = x0 + lane < n ? p.part_stats[part_of(sh, x0 + lane) * ROWS + r] : make_float2(-INFINITY, 0.0f);
-        const float w = exp2_approx(st.x - base);
-        sum += w * st.y;
-        const int many = n - x0 < 32 ? n - x0 : 32;
-        for (int y0 = 0; y0 < many; y0 += 8) {  // eight loads in flight
-          float4 v[8];
-          float wy[8];
+  const int rows = p.queries * p.group.d, eights = rows < ROWS ? (rows + 7) / 8 : kEights, columns = (p.d + 16 * kJoinColumns - 1) / (16 * kJoinColumns);
+  const int64_t items = (int64_t)p.spans * p.kv_heads * eights * columns;
+  for (int64_t first = (int64_t)blockIdx.x * kGroups; first < items; first += (int64_t)gridDim.x * kGroups) {
+    const int64_t item = first + warp / kWarps;
+    if (item >= items) continue;  // a group is a warp, or the block
+    const int64_t x0 = item / columns, at = x0 / eights;
+    const int t0 = (int)(item - x0 * columns) * kJoinColumns, eight = (int)(x0 - at * eights), index = (int)(at / p.kv_heads), kv = (int)(at - (int64_t)index * p.kv_heads);
+    const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row0 = (index - b * p.row_tiles) * ROWS + 8 * eight;
+    const Span sp = span_of<ROWS, UNIT>(p, index);
+    const int4 sh = sp.units ? p.shares[at] : make_int4(0, 1, 0, 0);
+    const int n = sp.units ? sh.y - sh.x + 1 : 0;  // parts
+    if (row0 >= rows || n == 1) continue;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float4 acc[kJoinColumns];
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            const int x = y0 + y < many ? y0 + y : many - 1;
-            wy[y] = __shfl_sync(~0u, w, x);
-            v[y] = *reinterpret_cast<const float4*>(p.part_sums + (part_of(sh, x0 + x) * ROWS + r) * p.d + column);
-          }
+    for (int t = 0; t < kJoinColumns; ++t) acc[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int x = member; x < n; x += kTake * kWarps) {
+      float4 st[kTake], v[kTake][kJoinColumns];
 #pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            if (y0 + y >= many) continue;
-            acc.x = fmaf(wy[y], v[y].x, acc.x), acc.y = fmaf(wy[y], v[y].y, acc.y), acc.z = fmaf(wy[y], v[y].z, acc.z), acc.w = fmaf(wy[y], v[y].w, acc.w);
-          }
+      for (int y = 0; y < kTake; ++y) {  // all loads before the first use; those behind the last part read it again
+        const int z = x + y * kWarps < n ? x + y * kWarps : x;
+        const int64_t slot = z == 0 ? (int64_t)sh.z : 2 * (int64_t)(sh.x + z);  // all but the first worker of a head begin with it
+        st[y] = p.part_stats[(slot * kEights + eight) * 4 + (lane & 3)];
+#pragma unroll
+        for (int t = 0; t < kJoinColumns; ++t) v[y][t] = p.part_sums[((slot * kEights + eight) * kSteps + (16 * (t0 + t) < p.d ? t0 + t : t0)) * 32 + lane];
+      }
+      float top[2] = {m[0], m[1]};
+#pragma unroll
+      for (int y = 0; y < kTake; ++y) {
+        if (x + y * kWarps >= n) continue;
+        top[0] = fmaxf(top[0], st[y].x), top[1] = fmaxf(top[1], st[y].y);
+      }
+      const float base[2] = {top[0] == -INFINITY ? 0.0f : top[0], top[1] == -INFINITY ? 0.0f : top[1]};
+      const float keep[2] = {exp2_approx(m[0] - base[0]), exp2_approx(m[1] - base[1])};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) l[h] *= keep[h], m[h] = top[h];
+#pragma unroll
+      for (int t = 0; t < kJoinColumns; ++t) acc[t].x *= keep[0], acc[t].y *= keep[1], acc[t].z *= keep[0], acc[t].w *= keep[1];
+#pragma unroll
+      for (int y = 0; y < kTake; ++y) {
+        if (x + y * kWarps >= n) continue;
+        const float w[2] = {exp2_approx(st[y].x - base[0]), exp2_approx(st[y].y - base[1])};
+        l[0] = fmaf(w[0], st[y].z, l[0]), l[1] = fmaf(w[1], st[y].w, l[1]);
+#pragma unroll
+        for (int t = 0; t < kJoinColumns; ++t) {
+          acc[t].x = fmaf(w[0], v[y][t].x, acc[t].x), acc[t].y = fmaf(w[1], v[y][t].y, acc[t].y);
+          acc[t].z = fmaf(w[0], v[y][t].z, acc[t].z), acc[t].w = fmaf(w[1], v[y][t].w, acc[t].w);
         }
       }
-      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(~0u, sum, x);
-      if (e < p.d) {
-        const bool nothing = sum == 0.0f || padding;
-        const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
-        const uint2 w = make_uint2(pack_bf16x2(acc.x * finish, acc.y * finish), pack_bf16x2(acc.z * finish, acc.w * finish));
-        *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = nothing ? make_uint2(0u, 0u) : w;
-      }
     }
-    if (lane == 0 && p.lse) p.lse[token * p.q_heads + head] = sum == 0.0f || padding ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
-  }
-}
-
-// A block per row, where few heads are in many parts: its warps take the parts in turn.
-constexpr int kJoinThreads = 512, kJoinWarps = kJoinThreads / 32, kJoinMost = 2048;  // parts whose weights shared memory holds: all workers'
-
-__device__ __forceinline__ float2 join_all(float2 x, bool largest, float2* scratch) {  // .x: maximum or sum over the block
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = 16; i; i >>= 1) {
-    const float y = __shfl_xor_sync(~0u, x.x, i);
-    x.x = largest ? fmaxf(x.x, y) : x.x + y;
-  }
-  __syncthreads();
-  if (lane == 0) scratch[warp] = x;
-  __syncthreads();
-  float2 all = scratch[0];
-  for (int w = 1; w < kJoinWarps; ++w) all.x = largest ? fmaxf(all.x, scratch[w].x) : all.x + scratch[w].x;
-  return all;
-}
-
-template <int ROWS, int UNIT>
-__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_wide_kernel(const AttendArgs p, float shift) {
-  __shared__ float s_weight[kJoinMost];
-  __shared__ float2 s_scratch[kJoinWarps];
-  __shared__ float4 s_sum[kJoinThreads];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  griddep_wait();
-  int rows = p.queries * p.group.d;
-  if (rows > ROWS) rows = ROWS;
-  const int64_t items = (int64_t)p.spans * p.kv_heads * rows;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t at = item / rows;
-    const int r = (int)(item - at * rows), index = (int)(at / p.kv_heads), kv = (int)(at - (int64_t)index * p.kv_heads);
-    const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row = (index - b * p.row_tiles) * ROWS + r;
-    if (row >= p.queries * p.group.d) continue;
-    const int4 sh = p.shares[at];
-    const int n = sh.y - sh.x + 1;
-    if (n <= 1) continue;
-    float top = -INFINITY, sum = 0.0f;
-    float2 first = make_float2(-INFINITY, 0.0f);  // this thread's first statistics, of n <= 512 parts all
-    for (int x = threadIdx.x; x < n; x += kJoinThreads) {
-      const float2 st = p.part_stats[part_of(sh, x) * ROWS + r];
-      if (x == threadIdx.x) first = st;
-      top = fmaxf(top, st.x);
-    }
-    top = join_all(make_float2(top, 0.0f), true, s_scratch).x;
-    const float base = top == -INFINITY ? 0.0f : top;
-    for (int x = threadIdx.x; x < n; x += kJoinThreads) {
-      const float2 st = x == threadIdx.x ? first : p.part_stats[part_of(sh, x) * ROWS + r];
-      const float w = exp2_approx(st.x - base);
-      s_weight[x] = w;
-      sum = fmaf(w, st.y, sum);
-    }
-    sum = join_all(make_float2(sum, 0.0f), false, s_scratch).x;
-    const int i = divide(row, p.group), head = kv * p.group.d + row - i * p.group.d;
-    const int64_t token = (int64_t)b * p.queries + i;
-    const bool nothing = sum == 0.0f || i >= span_of<ROWS, UNIT>(p, index).count;
-    for (int e0 = 0; e0 < p.d; e0 += 128) {
-      const int e = e0 + 4 * lane, column = e < p.d ? e : 0;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int y0 = warp; y0 < n; y0 += 8 * kJoinWarps) {  // eight loads in flight
-        float4 v[8];
-#pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const int x = y0 + y * kJoinWarps < n ? y0 + y * kJoinWarps : y0;
-          v[y] = *reinterpret_cast<const float4*>(p.part_sums + (part_of(sh, x) * ROWS + r) * p.d + column);
-        }
-#pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          if (y0 + y * kJoinWarps >= n) continue;
-          const float w = s_weight[y0 + y * kJoinWarps];
-          acc.x = fmaf(w, v[y].x, acc.x), acc.y = fmaf(w, v[y].y, acc.y), acc.z = fmaf(w, v[y].z, acc.z), acc.w = fmaf(w, v[y].w, acc.w);
-        }
-      }
-      s_sum[threadIdx.x] = acc;
+    if constexpr (kWarps > 1) {
       __syncthreads();
-      if (warp == 0 && e < p.d) {
-        for (int x = 1; x < kJoinWarps; ++x) {
-          const float4 v = s_sum[lane + 32 * x];
-          acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-        }
-        const float finish = (p.v_scale ? load_f32(p.v_scale + kv) : 1.0f) / sum;
-        const uint2 w = make_uint2(pack_bf16x2(acc.x * finish, acc.y * finish), pack_bf16x2(acc.z * finish, acc.w * finish));
-        *reinterpret_cast<uint2*>(p.out + token * p.out_ldt + head * p.out_ldh + e) = nothing ? make_uint2(0u, 0u) : w;
-      }
+      if (lane < 4) s_stats[warp][lane] = make_float4(m[0], m[1], l[0], l[1]);
+#pragma unroll
+      for (int t = 0; t < kJoinColumns; ++t) s_sums[warp][t][lane] = acc[t];
       __syncthreads();
+      if (member >= kJoinColumns) continue;  // a warp per 16 elements adds the warps up, in their order
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top[0] = fmaxf(top[0], s_stats[w][lane & 3].x), top[1] = fmaxf(top[1], s_stats[w][lane & 3].y);
+      acc[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      l[0] = l[1] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 st = s_stats[w][lane & 3], v = s_sums[w][member][lane];
+        const float a = exp2_approx(st.x - (top[0] == -INFINITY ? 0.0f : top[0])), c = exp2_approx(st.y - (top[1] == -INFINITY ? 0.0f : top[1]));
+        l[0] = fmaf(a, st.z, l[0]), l[1] = fmaf(c, st.w, l[1]);
+        acc[0].x = fmaf(a, v.x, acc[0].x), acc[0].y = fmaf(c, v.y, acc[0].y), acc[0].z = fmaf(a, v.z, acc[0].z), acc[0].w = fmaf(c, v.w, acc[0].w);
+      }
+      m[0] = top[0], m[1] = top[1];
     }
-    if (threadIdx.x == 0 && p.lse) p.lse[token * p.q_heads + head] = nothing ? -INFINITY : (base + log2f(sum) - shift) * 0.6931471805599453f;
+    const Finish<F8> to(p, sp, b, kv, row0, p.v_scale ? load_f32(p.v_scale + kv) : 1.0f, make_float2(l[0], l[1]));
+    if (lane < 4 && t0 == 0 && member == 0) to.write_lse(p, make_float2(m[0], m[1]), make_float2(l[0], l[1]), shift);
+    if constexpr (kWarps > 1) {
+      to.write(p, t0 + member, acc[0]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < kJoinColumns; ++t) to.write(p, t0 + t, acc[t]);
+    }
   }
 }
 
@@ -828,15 +746,15 @@ static int attend_blocks(int64_t spans, int64_t kv_heads, int64_t entries) {
 }
 
 template <int DP, bool F8, int ROWS>
-int64_t AttendCall<DP, F8, ROWS>::workspace(int64_t spans, int64_t kv_heads, int64_t d, int64_t entries) {
+int64_t AttendCall<DP, F8, ROWS>::workspace(int64_t spans, int64_t kv_heads, int64_t entries) {
   using C = AttendCfg<DP, F8, ROWS>;
-  return 2 * (int64_t)attend_blocks<DP, F8, ROWS>(spans, kv_heads, entries) * C::kTeams * C::kRows * (d + 2) * 4 + spans * kv_heads * 16;
+  return 2 * (int64_t)attend_blocks<DP, F8, ROWS>(spans, kv_heads, entries) * C::kTeams * C::kRows * (DP + 2) * 4 + spans * kv_heads * 16;
 }
 
 template <int DP, bool F8, int ROWS>
 tf_status AttendCall<DP, F8, ROWS>::launch(AttendArgs p, void* workspace_at, int64_t workspace_bytes, cudaStream_t stream, const char* fn) {
   using C = AttendCfg<DP, F8, ROWS>;
-  const int64_t need = workspace(p.spans, p.kv_heads, p.d, p.entries);
+  const int64_t need = workspace(p.spans, p.kv_heads, p.entries);
   if (need > workspace_bytes || !workspace_at)
     return fail(TF_ERR_WORKSPACE, "%s: the workspace needs %lld bytes, %lld were given", fn, (long long)need, (long long)workspace_bytes);
   auto kernel = paged_attention_kernel<DP, F8, ROWS>;
@@ -849,20 +767,19 @@ tf_status AttendCall<DP, F8, ROWS>::launch(AttendArgs p, void* workspace_at, int
   }
   p.whole_tiles = p.page.d % C::kKeys == 0;
   const int blocks = attend_blocks<DP, F8, ROWS>(p.spans, p.kv_heads, p.entries);
-  const int64_t parts = 2 * (int64_t)blocks * C::kTeams * C::kRows, heads = (int64_t)p.spans * p.kv_heads;
-  p.part_sums = static_cast<float*>(workspace_at);
-  p.part_stats = reinterpret_cast<float2*>(p.part_sums + parts * p.d);
-  p.shares = reinterpret_cast<int4*>(p.part_stats + parts);
+  const int64_t slots = 2 * (int64_t)blocks * C::kTeams, heads = (int64_t)p.spans * p.kv_heads;
+  p.part_sums = static_cast<float4*>(workspace_at);
+  p.part_stats = p.part_sums + slots * C::kRows * DP / 4;
+  p.shares = reinterpret_cast<int4*>(p.part_stats + slots * C::kRows / 2);
   TF_CUDA(launch_dependent(true, kernel, dim3((unsigned)blocks), dim3(kAttendThreads), C::kSmem, stream, p));
-  const int64_t rows = (int64_t)p.queries * p.group.d, items = heads * (rows < C::kRows ? rows : C::kRows);
-  // a block to a row where a head has more than eight parts on average
-  const int workers = blocks * C::kTeams;
-  if (heads * 8 < workers && workers <= kJoinMost) {
-    const int64_t most = (int64_t)sm_count() * 4;
-    TF_CUDA(launch_dependent(true, paged_attention_join_wide_kernel<C::kRows, C::kKeys>, dim3((unsigned)(items < most ? items : most)), dim3(kJoinThreads), 0, stream, p, C::kShift));
+  const int64_t rows = (int64_t)p.queries * p.group.d, eights = ((rows < C::kRows ? rows : C::kRows) + 7) / 8;
+  const int64_t items = heads * eights * ((p.d + 16 * kJoinColumns - 1) / (16 * kJoinColumns)), most = (int64_t)sm_count() * 8;
+  if (heads * 8 < (int64_t)blocks * C::kTeams && items <= most) {  // more than eight parts of a head on average
+    TF_CUDA(launch_dependent(true, paged_attention_join_kernel<DP, F8, C::kRows, C::kKeys, 8>, dim3((unsigned)items), dim3(kJoinThreads), 0, stream, p, C::kShift));
   } else {
-    const int64_t groups = (items + kAttendWarps - 1) / kAttendWarps, most = (int64_t)sm_count() * 8;
-    TF_CUDA(launch_dependent(true, paged_attention_join_kernel<C::kRows, C::kKeys>, dim3((unsigned)(groups < most ? groups : most)), dim3(kAttendThreads), 0, stream, p, C::kShift));
+    const int64_t groups = (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+    TF_CUDA(launch_dependent(true, paged_attention_join_kernel<DP, F8, C::kRows, C::kKeys, 1>, dim3((unsigned)(groups < most ? groups : most)), dim3(kJoinThreads), 0, stream, p,
+                             C::kShift));
   }
   return TF_OK;
 }

@@ -29,8 +29,8 @@ struct AttendArgs {
   int queries, q_heads, row_tiles, window;
   Divisor group;
   float scale_log2;
-  float* part_sums;    // [2 * workers][rows][d]: of a worker's first head, and of its last
-  float2* part_stats;  // [2 * workers][rows]: maximum, sum
+  float4* part_sums;   // [2 * workers][rows / 8][elements / 16][32 lanes]: of a worker's first head, and of its last
+  float4* part_stats;  // [2 * workers][rows / 8][4]: two rows' maxima and sums
   int4* shares;        // [spans * kv_heads]: the first and the last worker of a head, and the first one's slot
 };
 
@@ -38,7 +38,7 @@ struct AttendArgs {
 // launch have to agree.
 template <int DP, bool F8, int ROWS>
 struct AttendCall {
-  static int64_t workspace(int64_t spans, int64_t kv_heads, int64_t d, int64_t entries);
+  static int64_t workspace(int64_t spans, int64_t kv_heads, int64_t entries);
   static tf_status launch(AttendArgs p, void* workspace, int64_t workspace_bytes, cudaStream_t stream, const char* fn);
 };
 

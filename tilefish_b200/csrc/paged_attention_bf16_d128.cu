@@ -1,4 +1,4 @@
-// Attention over a paged bf16 cache, heads of 65 to 128 elements.
+// Attention over a paged bf16 cache, heads of 97 to 128 elements.
 #include "paged_attention.cuh"
 
 namespace tf {
