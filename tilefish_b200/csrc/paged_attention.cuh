@@ -123,12 +123,14 @@ __device__ __forceinline__ Span span_of(const AttendArgs& p, int index) {
   const int len = p.lengths[b], cnt = p.counts ? p.counts[b] : p.queries;
   s.length = len < 0 ? 0 : len > p.entries ? p.entries : len;
   s.count = cnt < 0 ? 0 : cnt > p.queries ? p.queries : cnt;
-  const int r0 = tile * ROWS;
-  int r1 = p.queries * p.group.d - 1;
-  if (r1 > r0 + ROWS - 1) r1 = r0 + ROWS - 1;
-  const int i0 = divide(r0, p.group);
-  int i1 = divide(r1, p.group);
-  if (i1 > s.count - 1) i1 = s.count - 1;
+  int i0 = 0, i1 = s.count - 1;  // the tile's first and last real query
+  if (p.row_tiles > 1) {
+    const int r0 = tile * ROWS;
+    int r1 = p.queries * p.group.d - 1;
+    if (r1 > r0 + ROWS - 1) r1 = r0 + ROWS - 1;
+    i0 = divide(r0, p.group);
+    if (i1 > divide(r1, p.group)) i1 = divide(r1, p.group);
+  }
   s.start = s.hi = s.units = s.first = s.last_lo = 0;
   if (i0 > i1) return s;
   const int base = s.length - s.count + 1;
@@ -351,53 +353,57 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
       }
       copy_commit();
     };
-#pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) issue(i);
-
-    // The query operand: row lane / 4 of each eight. Scores and sums are of rows 2c and 2c + 1, c = lane % 4.
-    uint32_t qf[kInRegisters ? DP / 16 : 1][NR][2];
-    float row_scale[NR][2];
-    int limit[NR][2], lowest[NR][2];
+    // The query operand: row lane / 4 of each eight, asked for before the copies wait for the table. Scores and sums are of rows 2c and 2c + 1, c = lane % 4.
+    uint32_t qf[DP / 16][NR][2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const int r = row0 + member * 8 * NR + 8 * n + (lane >> 2), i = divide(r, p.group);
       const bool real = r < p.queries * p.group.d;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + ((int64_t)b * p.queries + i) * p.q_ldt + ((int64_t)kv * p.group.d + r - i * p.group.d) * p.q_ldh);
-      float top = 0.0f;
-      uint32_t w[DP / 16][2];
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          // a matrix load of e4m3 codes leaves four neighbours in a thread: elements 4c .. 4c + 3 stand at k = 2c, 2c + 1, 2c + 8, 2c + 9
-          const int at = F8 ? kk * 8 + (lane & 3) * 2 + x : kk * 8 + (lane & 3) + 4 * x;
-          w[kk][x] = real && kk * 16 < p.d ? src[at] : 0u;
-          if constexpr (F8) top = fmaxf(top, fmaxf(fabsf(bf16lo_to_f32(w[kk][x])), fabsf(bf16hi_to_f32(w[kk][x]))));
+        // a matrix load of e4m3 codes leaves four neighbours in a thread: elements 4c .. 4c + 3 stand at k = 2c, 2c + 1, 2c + 8, 2c + 9
+        if constexpr (F8) {
+          const uint2 w = real && kk * 16 < p.d ? *reinterpret_cast<const uint2*>(src + kk * 8 + (lane & 3) * 2) : make_uint2(0u, 0u);
+          qf[kk][n][0] = w.x, qf[kk][n][1] = w.y;
+        } else {
+          qf[kk][n][0] = real && kk * 16 < p.d ? src[kk * 8 + (lane & 3)] : 0u;
+          qf[kk][n][1] = real && kk * 16 < p.d ? src[kk * 8 + (lane & 3) + 4] : 0u;
         }
       }
+    }
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) issue(i);
+    float row_scale[NR][2];
+    int limit[NR][2], lowest[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
       row_scale[n][0] = row_scale[n][1] = p.scale_log2;
       if constexpr (F8) {
-        // bf16 -> f16 without loss: the row is scaled by a power of two that puts its largest element into [2^14, 2^15)
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        const int e = (int)(__float_as_uint(top) >> 23);  // biased exponent; 0 and infinities are left as they are
-        const int up = e == 0 || e == 255 ? 0 : 127 + 14 - e;
-        const float a = __uint_as_float((uint32_t)(127 + (up >> 1)) << 23), c = __uint_as_float((uint32_t)(127 + (up - (up >> 1))) << 23);
+        // bf16 -> f16 without loss: the row is scaled by a power of two that puts its largest element into [2^14, 2^15), or by 2^126 (its scores are zero to f32 then)
+        float top = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) w[kk][x] = pack_f16x2(bf16lo_to_f32(w[kk][x]) * a * c, bf16hi_to_f32(w[kk][x]) * a * c);
-        const float ia = __uint_as_float((uint32_t)(127 - (up >> 1)) << 23), ic = __uint_as_float((uint32_t)(127 - (up - (up >> 1))) << 23);
-        const float mine = p.scale_log2 * (p.k_scale ? load_f32(p.k_scale + kv) : 1.0f) * ia * ic;
+          for (int x = 0; x < 2; ++x) top = fmaxf(top, fmaxf(fabsf(bf16lo_to_f32(qf[kk][n][x])), fabsf(bf16hi_to_f32(qf[kk][n][x]))));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        const int e = (int)(__float_as_uint(top) >> 23);  // biased exponent; 0 and infinities are left as they are
+        int up = e == 0 || e == 255 ? 0 : 127 + 14 - e;
+        if (up > 126) up = 126;
+        const float grow = __uint_as_float((uint32_t)(127 + up) << 23), shrink = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) qf[kk][n][x] = pack_f16x2(bf16lo_to_f32(qf[kk][n][x]) * grow, bf16hi_to_f32(qf[kk][n][x]) * grow);
+        const float mine = p.scale_log2 * (p.k_scale ? load_f32(p.k_scale + kv) : 1.0f) * shrink;
 #pragma unroll
         for (int h = 0; h < 2; ++h) row_scale[n][h] = __shfl_sync(~0u, mine, (2 * (lane & 3) + h) * 4);
       }
+      if constexpr (!kInRegisters) {
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        if constexpr (kInRegisters)
-          qf[kk][n][0] = w[kk][0], qf[kk][n][1] = w[kk][1];
-        else  // in the order of use: a thread's two words of a step, neighbours' behind one another
-          *reinterpret_cast<uint2*>(queries + ((kk * NR + n) * 32 + lane) * 8) = make_uint2(w[kk][0], w[kk][1]);
+        for (int kk = 0; kk < DP / 16; ++kk)  // in the order of use: a thread's two words of a step, neighbours' behind one another
+          *reinterpret_cast<uint2*>(queries + ((kk * NR + n) * 32 + lane) * 8) = make_uint2(qf[kk][n][0], qf[kk][n][1]);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
