@@ -22,7 +22,7 @@
 namespace tf {
 
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
-constexpr int kHeadCost = 3;  // what starting a head costs a worker, in tiles: 3 to 4 us to its first keys, a tile 1 to 2
+constexpr int kHeadCost = 4;  // what starting a head costs a worker, in tiles: 3 to 5 us to its first keys, a tile 1 to 2 (192 short sequences 30.2 us with 2, 26.4 with 4)
 // ROWS query rows of a kv head, in eights: as many of them to a warp as its registers hold (an accumulator of DP x 8 takes DP / 4 of them), the rest to
 // a team of warps that share the keys' tiles.
 template <int DP, bool F8, int ROWS>
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   constexpr int kEights = ROWS / 8, kSteps = DP / 16, kGroups = kJoinThreads / 32 / kWarps, kTake = 4;
   __shared__ float4 s_stats[kJoinThreads / 32][4], s_sums[kWarps > 1 ? kJoinThreads / 32 : 1][kJoinColumns][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % kWarps;
-  griddep_wait();
+  bool waited = false;
   const int rows = p.queries * p.group.d, eights = rows < ROWS ? (rows + 7) / 8 : kEights, columns = (p.d + 16 * kJoinColumns - 1) / (16 * kJoinColumns);
   const int64_t items = (int64_t)p.spans * p.kv_heads * eights * columns;
   for (int64_t first = (int64_t)blockIdx.x * kGroups; first < items; first += (int64_t)gridDim.x * kGroups) {
@@ -668,6 +668,10 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
     const int t0 = (int)(item - x0 * columns) * kJoinColumns, eight = (int)(x0 - at * eights), index = (int)(at / p.kv_heads), kv = (int)(at - (int64_t)index * p.kv_heads);
     const int b = p.row_tiles == 1 ? index : index / p.row_tiles, row0 = (index - b * p.row_tiles) * ROWS + 8 * eight;
     const Span sp = span_of<ROWS, UNIT>(p, index);
+    if (!waited) {  // lengths and counts are the caller's: the kernel in front has waited for them and does not write them
+      griddep_wait();
+      waited = true;
+    }
     const int4 sh = sp.units ? p.shares[at] : make_int4(0, 1, 0, 0);
     const int n = sp.units ? sh.y - sh.x + 1 : 0;  // parts
     if (row0 >= rows || n == 1) continue;
