@@ -80,7 +80,7 @@ TF_API tf_status tf_set_sm_margin(int32_t sms);
 /* Programmatic dependent launch (PROCESS-WIDE, as tf_set_sm_margin): 1 for all quantize, rmsnorm, GEMM and split-K reduction kernels, 0 for
  * none, -1 (what is in force until the first call) for short ones, as long as the SM margin is 0: GEMMs of at most 128 rows, of at most 256 rows as CTA
  * pairs or with all tiles at once, gated CTA pairs of one wave up to 1024 rows, row kernels of at most 4 rows, the quantizer of tf_quantize_nvfp4_dynamic
- * up to 2^24 elements. Such a kernel may be scheduled while the kernel before it on the stream is still draining; each waits (griddepcontrol.wait) for that
+ * up to 2^24 elements, and always the two kernels of tf_paged_attention. Such a kernel may be scheduled while the kernel before it on the stream is still draining; each waits (griddepcontrol.wait) for that
  * kernel to complete before it reads or writes anything that kernel may write or read, so results are unchanged (a GEMM asks weights into L2
  * before that, and the quantizer loads the tensor that its own amax launch in front reads). It hides launch latency and kernel set-up in chains of short kernels (small M, decode, many GPUs). No
  * counterpart in the reference. */
@@ -190,7 +190,8 @@ enum { TF_BF16 = 0, TF_F32 = 1 };
 /* Rotary positions: pair i of every head of token t is turned by the angle positions[t] * f_i and multiplied by `magnitude`; with `inverse` by
  * the negative angle, which is the gradient of the forward call. Elements from rot on are copied. f32 arithmetic, one rounding at the end.
  *   x, out     [tokens, heads, head_dim] of `dtype` (TF_BF16, TF_F32); token and head strides in elements. out may be x itself (in place), but
- *              must not overlap it in another way
+ *              must not overlap it in another way. Fastest where both are 16-byte aligned with strides of whole 16 bytes, head_dim is a multiple of
+ *              16 and, in the half layout, rot too
  *   positions  int32 or int64 [tokens] (position_bits); any value, negative ones turn back
  *   turns      uint64 [rot / 2]: the fraction of a full turn that f_i makes per position, times 2^64. Products wrap modulo a turn, so a far
  *              position loses nothing
@@ -225,7 +226,8 @@ TF_API tf_status tf_cache_append(const tf_paged_cache* cache, const void* k, int
  *   tables     int32 [seqs, table_cols], row stride table_stride
  *   lse        f32 [seqs * queries, q_heads] dense or NULL: ln sum_e exp(scale * q . k_e)
  *   workspace  tf_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, whose content does not matter
- * Scores, softmax statistics and sums are f32. The order of the sums depends on all lengths of the call, not on timing. */
+ * Scores, softmax statistics and sums are f32. Weights have 16 bits for a bf16 cache; for e4m3 11 bits down to 2^-21 of the largest, and 2^-32 of it is
+ * the least that counts. The order of the sums depends on all lengths of the call, not on timing. */
 TF_API int64_t tf_paged_attention_workspace_bytes(int64_t seqs, int64_t queries, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t cache_dtype,
                                                   int64_t max_entries);
 TF_API tf_status tf_paged_attention(const tf_paged_cache* cache, const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t seqs, int64_t queries,

@@ -194,6 +194,9 @@ def test_empty_and_refusals(A):
     refused("shape", cache, k, k, tables, positions, rows=tables[0])
     refused("argument", cache, k, k, tables, positions, q_out=k)
     refused("alias", cache, k, k, tables, positions, q=k, q_out=torch.zeros((1, 2, 64), dtype=torch.bfloat16, device="cuda").expand(4, 2, 64))
+    wide = torch.zeros((4, 8, 64), dtype=torch.bfloat16, device="cuda")
+    refused("alias", cache, wide[:, 4:6], wide[:, 6:], tables, positions, q=torch.zeros((4, 4, 64), dtype=torch.bfloat16, device="cuda"), q_out=wide[:, 1:5])
+    assert A.cache_append(cache, wide[:, 4:6], wide[:, 6:], tables, positions, q=wide[:, :4], q_out=wide[:, :4]) is not None  # columns of one matrix
     refused("shape", cache, k, k, tables, positions, rotary=A.RotaryTable(A.rotary_frequencies(128)[0]))
     refused("alignment", cache, torch.zeros((4, 2, 68), dtype=torch.bfloat16, device="cuda")[..., :64], k, tables, positions)
     refused("pointer_alignment", cache, torch.zeros(4 * 2 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 2, 64), k, tables, positions)

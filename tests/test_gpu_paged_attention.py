@@ -92,6 +92,16 @@ def test_heads_and_queries(A, dtype, kv, group, queries):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("dim", [48, 96, 128, 240])
+@pytest.mark.parametrize("group,queries", [(8, 1), (3, 5), (8, 3), (8, 4), (8, 5), (16, 3), (7, 9), (13, 10)])
+def test_every_number_of_rows(A, dtype, dim, group, queries):
+    """8 to 130 rows of a kv head in every head size's kernels, with sequences that several workers share, empty ones and padding."""
+    q, cache, tables, lengths = setup(A, [400, 0, 33, 2, 90], queries, 2, group, dim, 16 if group % 2 else 48, dtype)
+    run(A, q, cache, tables, lengths)
+    run(A, q, cache, tables, lengths, counts=torch.tensor([queries, 1, queries - 1, queries, 1], dtype=torch.int32), window=50)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 @pytest.mark.parametrize("page", [1, 3, 8, 24, 64, 100, 1000])
 def test_page_sizes(A, dtype, page):
     run(A, *setup(A, LENGTHS, 2, 2, 3, 64, page, dtype))
@@ -148,6 +158,19 @@ def test_scale(A, scale):
 
 def test_e4m3_without_scales(A):
     run(A, *setup(A, [77, 5], 1, 2, 4, 64, 16, "e4m3", scales=False))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_rising_scores(A, dtype):
+    """Each key's score passes the ones before it by less than 2^8, in steps that add up to far more: the exponents' reference has to follow."""
+    q, cache, tables, lengths = setup(A, [600], 1, 1, 2, 32, 16, dtype, scales=False)
+    for e in range(600):
+        row = torch.full((32,), 0.0)
+        row[e % 32] = min(448.0, 0.75 * e)
+        cache.k[int(tables[0, e // 16]), 0, e % 16] = row.to(R.E4M3).view(torch.uint8).cuda() if dtype == "e4m3" else row.bfloat16().cuda()
+    q.fill_(1.0)
+    run(A, q, cache, tables, lengths, scale=1.0)
+    run(A, q, cache, tables, lengths, scale=-1.0)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])

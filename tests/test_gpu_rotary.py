@@ -77,6 +77,9 @@ def test_strided_in_place_and_out(A, layout, dim, rot):
     by_heads = torch.full((heads, 11, dim), 7.0, dtype=torch.bfloat16, device="cuda")  # heads outside, tokens inside
     A.rotary(x, positions.cuda(), table, out=by_heads.transpose(0, 1))
     assert torch.equal(by_heads.transpose(0, 1), fresh)
+    both = torch.cat([x, torch.full_like(x, 5.0)], dim=1)  # into other columns of the same matrix
+    A.rotary(both[:, :heads], positions.cuda(), table, out=both[:, heads:])
+    assert torch.equal(both[:, heads:], fresh) and torch.equal(both[:, :heads], x)
     assert A.rotary(x, positions.cuda(), table, out=x) is x
     assert torch.equal(x, fresh)
     assert torch.equal(gpu[:, :dim].cpu(), wide[:, :dim]) and torch.equal(gpu[:, (heads + 1) * dim:].cpu(), wide[:, (heads + 1) * dim:])

@@ -25,7 +25,7 @@ from . import kernels as K
 from .kernels import _check, _dense, _pre, _stream, _torch
 
 LAYOUTS = {"half": N.ROTARY_HALF, "interleaved": N.ROTARY_INTERLEAVED}
-_PI = Fraction("3.14159265358979323846264338327950288419716939937510")
+_TURN = round(2**192 / (2 * Fraction("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")))  # 2^64 / 2 pi, times 2^128
 
 
 # A call's checks run in front of launches of a few microseconds: shape, strides and address of a tensor are asked for once and device indexes are
@@ -68,11 +68,23 @@ def _ints(t, name: str, n: Optional[int], index: int) -> int:
 
 
 def _overlap(a, b) -> bool:
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + (1 + sum((s - 1) * st for s, st in zip(t.shape, t.stride()))) * t.element_size()
+    """Whether two [tokens, heads, dim] tensors share memory. Slices of the columns of one matrix do not."""
 
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a.numel() > 0 and b.numel() > 0 and a0 < b1 and b0 < a1
+    def span(t):
+        size = t.element_size()
+        row = (1 + sum((n - 1) * st for n, st in zip(t.shape[1:], t.stride()[1:]))) * size
+        step = t.stride(0) * size
+        return t.data_ptr(), row, step, t.data_ptr() + (t.shape[0] - 1) * step + row
+
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, arow, astep, a1), (b0, brow, bstep, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if astep != bstep or arow > astep or brow > astep:
+        return True
+    apart = (b0 - a0) % astep
+    return apart < arow or apart + brow > astep
 
 
 def _result(t, name: str) -> None:
@@ -84,10 +96,11 @@ def _result(t, name: str) -> None:
 
 
 def _turns(frequencies):
-    """Frequencies (radians per position) as the fraction of a full turn per position, times 2^64, in two's complement."""
+    """Frequencies (radians per position) as the fraction of a full turn per position, times 2^64, in two's complement: exact integer arithmetic, rounded once."""
     out = []
     for f in frequencies:
-        turns = round(Fraction(f) / (2 * _PI) * 2**64) % 2**64
+        n, d = f.as_integer_ratio()  # d is a power of two
+        turns = (2 * n * _TURN + (d << 128)) // (d << 129) & (2**64 - 1)
         out.append(turns - 2**64 if turns >= 2**63 else turns)
     return out
 
@@ -113,7 +126,7 @@ class RotaryTable:
             inv_freq = inv_freq.double().tolist()
         values = [float(f) for f in inv_freq]
         _pre(1 <= len(values) <= 512, f"inv_freq: {len(values)} frequencies; 1 to 512 are possible", "shape", "inv_freq")
-        _pre(all(math.isfinite(f) for f in values), "inv_freq: not finite", "argument", "inv_freq")
+        _pre(all(abs(f) <= 2.0**32 for f in values), "inv_freq: not finite, or more than 2^32 radians", "argument", "inv_freq")
         self.rot, self.layout, self.magnitude, self._layout = 2 * len(values), layout, float(magnitude), LAYOUTS[layout]
         self.turns = torch.tensor(_turns(values), dtype=torch.int64, device=device if device is not None else "cuda")
         self.index = self.turns.get_device()
@@ -338,6 +351,7 @@ def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=Non
             _, ot, oh, op = _heads(q_out, "q_out", tokens, q_heads, dim, index)
             _result(q_out, "q_out")
             _pre((op == qp and ot == qt and oh == qh) or not _overlap(q_out, q), "q_out overlaps q without being q", "alias", "q_out")
+            _pre(not _overlap(q_out, k) and not _overlap(q_out, v), "q_out overlaps k or v", "alias", "q_out")
         if q_heads == 0:
             qp = op = None
     elif q_out is not None:
