@@ -54,21 +54,36 @@ extern template struct AttendCall<256, true, 16>;
 extern template struct AttendCall<256, true, 32>;
 extern template struct AttendCall<256, true, 64>;
 
-// As few rows as hold a kv head's query heads times the new tokens, up to 64; more are several tiles.
+// Rows of a tile: as few as hold a kv head's query heads times the new tokens, up to 64; more are several tiles, which read the keys again. 40 rows of more
+// than 96 elements are more than a warp's registers hold, and of more than 128 a warp holds 16. One tile is faster than several small ones (12 sequences of up
+// to 16384, bf16: 64 rows of 128 elements 116 us, in tiles of 32, 24 and 16 118, 137 and 181; 40 of 96 elements 72, 98, 84 and 94) but for 33 to 48
+// rows of more than 128 elements, for which 64 is a third too many (256 elements: 284 us, in tiles of 16 270; e4m3 169 and 143).
+static int attend_rows(int64_t rows, int64_t d) {
+  if (d > 128) return rows <= 8 ? 8 : rows <= 16 || (rows > 32 && rows <= 48) ? 16 : rows <= 32 ? 32 : 64;
+  const int eights = rows > 64 ? 8 : (int)(rows + 7) / 8;
+  return eights <= 4 ? 8 * eights : eights == 5 && d <= 96 ? 40 : eights <= 6 ? 48 : 64;
+}
+static int64_t attend_row_tiles(int64_t rows, int64_t d) {
+  const int tile = attend_rows(rows, d);
+  return (rows + tile - 1) / tile;
+}
+
 template <class Use>
 static auto with_attend_call(int64_t rows, int64_t d, int32_t dtype, Use use) {
   auto by_rows = [&](auto dp, auto f8) {
     constexpr int kDP = decltype(dp)::value;
     constexpr bool kF8 = decltype(f8)::value;
-    if (rows <= 8) return use(AttendCall<kDP, kF8, 8>{});
-    if (rows <= 16) return use(AttendCall<kDP, kF8, 16>{});
+    const int tile = attend_rows(rows, d);
+    if (tile == 8) return use(AttendCall<kDP, kF8, 8>{});
+    if (tile == 16) return use(AttendCall<kDP, kF8, 16>{});
+    if (tile == 32) return use(AttendCall<kDP, kF8, 32>{});
     if constexpr (kDP < 256) {
-      if (rows <= 24) return use(AttendCall<kDP, kF8, 24>{});
-      if constexpr (kDP < 128)  // 40 rows of 128 elements are more than a warp's registers
-        if (rows > 32 && rows <= 40) return use(AttendCall<kDP, kF8, 40>{});
-      if (rows > 32 && rows <= 48) return use(AttendCall<kDP, kF8, 48>{});
+      if (tile == 24) return use(AttendCall<kDP, kF8, 24>{});
+      if (tile == 48) return use(AttendCall<kDP, kF8, 48>{});
     }
-    return rows <= 32 ? use(AttendCall<kDP, kF8, 32>{}) : use(AttendCall<kDP, kF8, 64>{});
+    if constexpr (kDP < 128)
+      if (tile == 40) return use(AttendCall<kDP, kF8, 40>{});
+    return use(AttendCall<kDP, kF8, 64>{});
   };
   auto by_dim = [&](auto f8) {
     return d <= 64 ? by_rows(std::integral_constant<int, 64>{}, f8) : d <= 96 ? by_rows(std::integral_constant<int, 96>{}, f8) : d <= 128 ? by_rows(std::integral_constant<int, 128>{}, f8) : by_rows(std::integral_constant<int, 256>{}, f8);
@@ -76,14 +91,12 @@ static auto with_attend_call(int64_t rows, int64_t d, int32_t dtype, Use use) {
   return dtype == TF_CACHE_E4M3 ? by_dim(std::true_type{}) : by_dim(std::false_type{});
 }
 
-static int64_t attend_row_tiles(int64_t rows) { return (rows + 63) / 64; }
-
 // Sizes that the kernels' 32-bit counts hold.
-static bool attend_sizes_ok(int64_t seqs, int64_t queries, int64_t q_heads, int64_t kv_heads) {
+static bool attend_sizes_ok(int64_t seqs, int64_t queries, int64_t q_heads, int64_t kv_heads, int64_t d) {
   if (seqs < 0 || queries < 1 || q_heads < 1 || kv_heads < 1 || kv_heads > 65535 || q_heads > 65535 || q_heads % kv_heads) return false;
   if (seqs > (1 << 30) || queries > (1 << 20)) return false;
   const int64_t rows = queries * (q_heads / kv_heads);
-  return rows < (1 << 30) && seqs * queries <= INT32_MAX && seqs * attend_row_tiles(rows) * kv_heads <= INT32_MAX;
+  return rows < (1 << 30) && seqs * queries <= INT32_MAX && seqs * attend_row_tiles(rows, d) * kv_heads <= INT32_MAX;
 }
 
 }  // namespace tf
@@ -92,10 +105,10 @@ using namespace tf;
 
 extern "C" int64_t tf_paged_attention_workspace_bytes(int64_t seqs, int64_t queries, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t cache_dtype,
                                                       int64_t max_entries) {
-  if (!attend_sizes_ok(seqs, queries, q_heads, kv_heads) || head_dim < 16 || head_dim > 256 || head_dim % 16 || max_entries < 1 || cache_dtype < 0 || cache_dtype > 1) return -1;
+  if (!attend_sizes_ok(seqs, queries, q_heads, kv_heads, head_dim) || head_dim < 16 || head_dim > 256 || head_dim % 16 || max_entries < 1 || cache_dtype < 0 || cache_dtype > 1) return -1;
   const int64_t rows = queries * (q_heads / kv_heads), entries = max_entries > INT32_MAX / 2 ? INT32_MAX / 2 : max_entries;
   if (seqs == 0) return 0;
-  return with_attend_call(rows, head_dim, cache_dtype, [&](auto call) { return decltype(call)::workspace(seqs * attend_row_tiles(rows), kv_heads, entries); });
+  return with_attend_call(rows, head_dim, cache_dtype, [&](auto call) { return decltype(call)::workspace(seqs * attend_row_tiles(rows, head_dim), kv_heads, entries); });
 }
 
 extern "C" tf_status tf_paged_attention(const tf_paged_cache* cache, const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t seqs, int64_t queries,
@@ -105,7 +118,7 @@ extern "C" tf_status tf_paged_attention(const tf_paged_cache* cache, const void*
   clear_error();
   if (tf_status st = check_cache(cache, __func__)) return st;
   TF_CHECK_ARG(q && out && tables && lengths, "%s: null pointer", __func__);
-  TF_CHECK_ARG(attend_sizes_ok(seqs, queries, q_heads, cache->kv_heads) && table_cols > 0 && window >= 0,
+  TF_CHECK_ARG(attend_sizes_ok(seqs, queries, q_heads, cache->kv_heads, cache->head_dim) && table_cols > 0 && window >= 0,
                "%s: bad shape seqs=%lld queries=%lld q_heads=%lld kv_heads=%lld table_cols=%lld window=%lld", __func__, (long long)seqs, (long long)queries,
                (long long)q_heads, (long long)cache->kv_heads, (long long)table_cols, (long long)window);
   TF_CHECK_ALIGNED(q, 16, "q");
@@ -125,7 +138,7 @@ extern "C" tf_status tf_paged_attention(const tf_paged_cache* cache, const void*
   p.q = static_cast<const __nv_bfloat16*>(q), p.out = static_cast<__nv_bfloat16*>(out), p.lse = lse;
   p.q_ldt = q_stride_token, p.q_ldh = q_stride_head, p.out_ldt = out_stride_token, p.out_ldh = out_stride_head;
   p.tables = tables, p.table_stride = table_stride, p.lengths = lengths, p.counts = counts, p.entries = (int)entries;
-  p.queries = (int)queries, p.q_heads = (int)q_heads, p.row_tiles = (int)attend_row_tiles(rows), p.spans = (int)(seqs * p.row_tiles);
+  p.queries = (int)queries, p.q_heads = (int)q_heads, p.row_tiles = (int)attend_row_tiles(rows, cache->head_dim), p.spans = (int)(seqs * p.row_tiles);
   p.window = (int)(window > INT32_MAX / 2 ? 0 : window);
   p.group = divisor((int)(q_heads / cache->kv_heads));
   p.scale_log2 = scale * 1.4426950408889634f;

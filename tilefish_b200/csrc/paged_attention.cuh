@@ -248,8 +248,22 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
   const int owner = __popc(__ballot_sync(~0u, upto * p.kv_heads <= u0));  // the lane whose spans u0 falls into
   int index = owner * share;
   long long before = __shfl_sync(~0u, upto - cost, owner) * p.kv_heads;  // where span `index` begins
-  if (share > 1)
-    for (long long c = (long long)cost_of(index) * p.kv_heads; u0 >= before + c; c = (long long)cost_of(index) * p.kv_heads) before += c, ++index;
+  for (int at = 0; at < share && share > 1; at += 32) {  // which of them: 32 at a time
+    const long long c = at + lane < share ? (long long)cost_of(owner * share + at + lane) * p.kv_heads : 0;
+    long long here = c;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const long long y = __shfl_up_sync(~0u, here, x);
+      if (lane >= x) here += y;
+    }
+    const int passed = __popc(__ballot_sync(~0u, before + here <= u0));  // all spans that end at or before this range
+    if (passed < 32) {
+      index = owner * share + at + passed;
+      before += __shfl_sync(~0u, here - c, passed);
+      break;
+    }
+    before += __shfl_sync(~0u, here, 31);
+  }
 
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + team * C::kStages * 2 * C::kHalf;
   [[maybe_unused]] uint8_t* queries = smem + C::kRing + warp * C::kQueryBytes;  // this warp's, written and read by the same threads
