@@ -16,6 +16,7 @@
 #pragma once
 
 #include <cmath>
+#include <type_traits>
 
 #include "paged_attention.h"
 
@@ -663,14 +664,21 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
 }
 
 // Adds up what the workers that shared a head left, and writes the rows that see nothing. A group of kWarps warps has one eight of rows and 32 of their
-// elements; its warps take the parts in turn, each with a maximum of its own, and are joined through shared memory: one warp where a head has few parts, eight
-// where few heads are in many.
-constexpr int kJoinThreads = 256, kJoinColumns = 2;  // of 16 elements
+// elements; its warps take the parts in turn, each with a maximum of its own, and are joined through shared memory. One warp where a head has few parts, 16
+// where few heads are in many (a warp per row of 128 elements took 16 us to add up 111 parts). Bound by the latency of four dependent loads.
+constexpr int kJoinColumns = 2;  // of 16 elements
+
+template <int kWarps>
+struct JoinCfg {
+  static constexpr int kThreads = kWarps == 1 ? 256 : 32 * kWarps, kGroups = kThreads / 32 / kWarps;
+  static constexpr int kTake = kWarps == 16 ? 4 : 2;  // parts whose loads are in flight together
+  static constexpr int kBlocksPerSm = kWarps == 16 ? 1 : 1024 / kThreads;
+};
 
 template <int DP, bool F8, int ROWS, int UNIT, int kWarps>
-__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const AttendArgs p, float shift) {
-  constexpr int kEights = ROWS / 8, kSteps = DP / 16, kGroups = kJoinThreads / 32 / kWarps, kTake = 4;
-  __shared__ float4 s_stats[kJoinThreads / 32][4], s_sums[kWarps > 1 ? kJoinThreads / 32 : 1][kJoinColumns][32];
+__global__ void __launch_bounds__(JoinCfg<kWarps>::kThreads, JoinCfg<kWarps>::kBlocksPerSm) paged_attention_join_kernel(const AttendArgs p, float shift) {
+  constexpr int kEights = ROWS / 8, kSteps = DP / 16, kGroups = JoinCfg<kWarps>::kGroups, kTake = JoinCfg<kWarps>::kTake;
+  __shared__ float4 s_stats[kWarps][4], s_sums[kWarps > 1 ? kWarps : 1][kJoinColumns][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % kWarps;
   bool waited = false;
   const int rows = p.queries * p.group.d, eights = rows < ROWS ? (rows + 7) / 8 : kEights, columns = (p.d + 16 * kJoinColumns - 1) / (16 * kJoinColumns);
@@ -797,14 +805,23 @@ tf_status AttendCall<DP, F8, ROWS>::launch(AttendArgs p, void* workspace_at, int
   p.shares = reinterpret_cast<int4*>(p.part_stats + slots * C::kRows / 2);
   TF_CUDA(launch_dependent(true, kernel, dim3((unsigned)blocks), dim3(kAttendThreads), C::kSmem, stream, p));
   const int64_t rows = (int64_t)p.queries * p.group.d, eights = ((rows < C::kRows ? rows : C::kRows) + 7) / 8;
-  const int64_t items = heads * eights * ((p.d + 16 * kJoinColumns - 1) / (16 * kJoinColumns)), most = (int64_t)sm_count() * 8;
-  if (heads * 8 < (int64_t)blocks * C::kTeams && items <= most) {  // more than eight parts of a head on average
-    TF_CUDA(launch_dependent(true, paged_attention_join_kernel<DP, F8, C::kRows, C::kKeys, 8>, dim3((unsigned)items), dim3(kJoinThreads), 0, stream, p, C::kShift));
-  } else {
-    const int64_t groups = (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
-    TF_CUDA(launch_dependent(true, paged_attention_join_kernel<DP, F8, C::kRows, C::kKeys, 1>, dim3((unsigned)(groups < most ? groups : most)), dim3(kJoinThreads), 0, stream, p,
-                             C::kShift));
-  }
+  const int64_t items = heads * eights * ((p.d + 16 * kJoinColumns - 1) / (16 * kJoinColumns)), most = (int64_t)sm_count() * 16;
+  auto join = [&](auto form) -> cudaError_t {
+    constexpr int kWarps = decltype(form)::value;
+    using J = JoinCfg<kWarps>;
+    const int64_t groups = (items + J::kGroups - 1) / J::kGroups;
+    return launch_dependent(true, paged_attention_join_kernel<DP, F8, C::kRows, C::kKeys, kWarps>, dim3((unsigned)(groups < most ? groups : most)), dim3(J::kThreads), 0, stream, p,
+                            C::kShift);
+  };
+  // workers over heads are the parts of a head on average. 16 warps only where all items are resident at once (40 rows of 120 heads, ten parts each: 69 us with
+  // 16 warps, 42 with four; two sequences of 131072, 111 parts of 16 heads: 116 us with 16, 125 with four).
+  const int64_t workers = (int64_t)blocks * C::kTeams;
+  if (workers > heads * 8 && items <= 2 * (int64_t)sm_count())
+    TF_CUDA(join(std::integral_constant<int, 16>{}));
+  else if (workers > heads * 4)
+    TF_CUDA(join(std::integral_constant<int, 4>{}));
+  else
+    TF_CUDA(join(std::integral_constant<int, 1>{}));
   return TF_OK;
 }
 
