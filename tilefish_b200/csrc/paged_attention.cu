@@ -59,8 +59,10 @@ extern template struct AttendCall<256, true, 64>;
 // to 16384, bf16: 64 rows of 128 elements 116 us, in tiles of 32, 24 and 16 118, 137 and 181; 40 of 96 elements 72, 98, 84 and 94) but for 33 to 48
 // rows of more than 128 elements, for which 64 is a third too many (256 elements: 284 us, in tiles of 16 270; e4m3 169 and 143).
 static int attend_rows(int64_t rows, int64_t d) {
+  const int64_t tiles = (rows + 63) / 64;
+  rows = (rows + tiles - 1) / tiles;  // 80 are twice 40
   if (d > 128) return rows <= 8 ? 8 : rows <= 16 || (rows > 32 && rows <= 48) ? 16 : rows <= 32 ? 32 : 64;
-  const int eights = rows > 64 ? 8 : (int)(rows + 7) / 8;
+  const int eights = (int)(rows + 7) / 8;
   return eights <= 4 ? 8 * eights : eights == 5 && d <= 96 ? 40 : eights <= 6 ? 48 : 64;
 }
 static int64_t attend_row_tiles(int64_t rows, int64_t d) {

@@ -42,7 +42,8 @@ struct AttendCfg {
   static constexpr int kBlocksPerSm = DP == 256 && !F8 ? 1 : kEights * DP <= 128 ? 3 : 2;
   static constexpr int kFit = (200704 - kBlocksPerSm * kAttendWarps * kQueryBytes) / (kBlocksPerSm * kTeams * 2 * kHalf);
   static constexpr int kStages = kFit < 2 ? 2 : kFit > 6 ? 6 : kFit;
-  static constexpr int kRing = kTeams * kStages * 2 * kHalf, kSmem = kRing + kAttendWarps * kQueryBytes;
+  static constexpr int kRing = kTeams * kStages * 2 * kHalf, kParts = kTeams * kRows * (DP + 2) * 4;  // kParts: what a block joins of its own
+  static constexpr int kSmem = kRing + kAttendWarps * kQueryBytes > kParts ? kRing + kAttendWarps * kQueryBytes : kParts;
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
   static constexpr int kRowsPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
   static_assert(kBlocksPerSm * (kSmem + 2560) <= 228 * 1024 && kSmem <= 225 * 1024, "the grid counts on so many blocks an SM");
@@ -638,6 +639,49 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
 
     // the result, or this worker's part of it: its registers in their order
     const bool all = tiles == sp.units;
+    if constexpr (C::kTeams > 1) {
+      // Where the head began before this block's ranges and goes on behind them, all of the block's workers have this head alone: they leave one part.
+      const int first_worker = blockIdx.x * C::kTeams;
+      if (!all && unit > 0 && unit + tiles < sp.units && ranges.of_position(head_end - cost + kHeadCost) < first_worker && ranges.of_position(head_end - 1) >= first_worker + C::kTeams) {
+        constexpr int kEights = C::kRows / 8, kSteps = DP / 16;
+        float4* sums = reinterpret_cast<float4*>(smem);  // [teams][eights][steps][32]
+        float4* stats = sums + C::kTeams * kEights * kSteps * 32;
+        copy_wait<0>();
+        __syncthreads();  // the rings are free
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const int eight = team * kEights + member * NR + n;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            for (int x = 4; x < 32; x <<= 1) l[n][h] += __shfl_xor_sync(~0u, l[n][h], x);
+#pragma unroll
+          for (int t = 0; t < kSteps; ++t) sums[(eight * kSteps + t) * 32 + lane] = make_float4(o[t][n][0], o[t][n][1], o[t][n][2], o[t][n][3]);
+          if (lane < 4) stats[eight * 4 + lane] = make_float4(m[n][0], m[n][1], l[n][0], l[n][1]);
+        }
+        __syncthreads();
+        for (int i = warp; i < kEights * kSteps; i += kAttendWarps) {
+          const int eight = i / kSteps, t = i - eight * kSteps;
+          float4 st[C::kTeams], sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          float2 top = make_float2(-INFINITY, -INFINITY), total = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int w = 0; w < C::kTeams; ++w) {
+            st[w] = stats[(w * kEights + eight) * 4 + (lane & 3)];
+            top = make_float2(fmaxf(top.x, st[w].x), fmaxf(top.y, st[w].y));
+          }
+#pragma unroll
+          for (int w = 0; w < C::kTeams; ++w) {
+            const float a = exp2_approx(st[w].x - (top.x == -INFINITY ? 0.0f : top.x)), c = exp2_approx(st[w].y - (top.y == -INFINITY ? 0.0f : top.y));
+            const float4 v = sums[((w * kEights + eight) * kSteps + t) * 32 + lane];
+            total = make_float2(fmaf(a, st[w].z, total.x), fmaf(c, st[w].w, total.y));
+            sum = make_float4(fmaf(a, v.x, sum.x), fmaf(c, v.y, sum.y), fmaf(a, v.z, sum.z), fmaf(c, v.w, sum.w));
+          }
+          const int64_t at = 2 * (int64_t)first_worker * kEights + eight;
+          if (16 * t < p.d) p.part_sums[(at * kSteps + t) * 32 + lane] = sum;
+          if (t == 0 && lane < 4) p.part_stats[at * 4 + lane] = make_float4(top.x, top.y, total.x, total.y);
+        }
+        return;  // the range ends here
+      }
+    }
     const float v_scale = p.v_scale ? load_f32(p.v_scale + kv) : 1.0f;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -677,7 +721,7 @@ struct JoinCfg {
 
 template <int DP, bool F8, int ROWS, int UNIT, int kWarps>
 __global__ void __launch_bounds__(JoinCfg<kWarps>::kThreads, JoinCfg<kWarps>::kBlocksPerSm) paged_attention_join_kernel(const AttendArgs p, float shift) {
-  constexpr int kEights = ROWS / 8, kSteps = DP / 16, kGroups = JoinCfg<kWarps>::kGroups, kTake = JoinCfg<kWarps>::kTake;
+  constexpr int kEights = ROWS / 8, kSteps = DP / 16, kGroups = JoinCfg<kWarps>::kGroups, kTake = JoinCfg<kWarps>::kTake, T = AttendCfg<DP, F8, ROWS>::kTeams;
   __shared__ float4 s_stats[kWarps][4], s_sums[kWarps > 1 ? kWarps : 1][kJoinColumns][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % kWarps;
   bool waited = false;
@@ -695,7 +739,9 @@ __global__ void __launch_bounds__(JoinCfg<kWarps>::kThreads, JoinCfg<kWarps>::kB
       waited = true;
     }
     const int4 sh = sp.units ? p.shares[at] : make_int4(0, 1, 0, 0);
-    const int n = sp.units ? sh.y - sh.x + 1 : 0;  // parts
+    // Parts of workers, but of the blocks between the first worker's and the last one's one part each.
+    const int kept = T > 1 ? (sh.x / T + 1) * T - sh.x : 1, between = T > 1 ? sh.y / T - sh.x / T - 1 : 0;
+    const int n = !sp.units ? 0 : between <= 0 ? sh.y - sh.x + 1 : kept + between + sh.y % T + 1;
     if (row0 >= rows || n == 1) continue;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     float4 acc[kJoinColumns];
@@ -706,7 +752,8 @@ __global__ void __launch_bounds__(JoinCfg<kWarps>::kThreads, JoinCfg<kWarps>::kB
 #pragma unroll
       for (int y = 0; y < kTake; ++y) {  // all loads before the first use; those behind the last part read it again
         const int z = x + y * kWarps < n ? x + y * kWarps : x;
-        const int64_t slot = z == 0 ? (int64_t)sh.z : 2 * (int64_t)(sh.x + z);  // all but the first worker of a head begin with it
+        const int worker = between <= 0 || z < kept ? sh.x + z : z < kept + between ? (sh.x / T + 1 + z - kept) * T : sh.y / T * T + z - kept - between;
+        const int64_t slot = z == 0 ? (int64_t)sh.z : 2 * (int64_t)worker;  // all but the first worker of a head begin with it
         st[y] = p.part_stats[(slot * kEights + eight) * 4 + (lane & 3)];
 #pragma unroll
         for (int t = 0; t < kJoinColumns; ++t) v[y][t] = p.part_sums[((slot * kEights + eight) * kSteps + (16 * (t0 + t) < p.d ? t0 + t : t0)) * 32 + lane];
@@ -813,12 +860,12 @@ tf_status AttendCall<DP, F8, ROWS>::launch(AttendArgs p, void* workspace_at, int
     return launch_dependent(true, paged_attention_join_kernel<DP, F8, C::kRows, C::kKeys, kWarps>, dim3((unsigned)(groups < most ? groups : most)), dim3(J::kThreads), 0, stream, p,
                             C::kShift);
   };
-  // workers over heads are the parts of a head on average. 16 warps only where all items are resident at once (40 rows of 120 heads, ten parts each: 69 us with
-  // 16 warps, 42 with four; two sequences of 131072, 111 parts of 16 heads: 116 us with 16, 125 with four).
-  const int64_t workers = (int64_t)blocks * C::kTeams;
-  if (workers > heads * 8 && items <= 2 * (int64_t)sm_count())
+  // Workers over heads are the parts of a head on average, and over heads and teams where blocks join their own. 16 warps only where all items are resident
+  // at once (40 rows of 120 heads, ten parts each: 69 us with 16 warps, 42 with four; two sequences of 131072, 111 parts of 16 heads: 116 us with 16, 125 with four).
+  const int64_t workers = (int64_t)blocks * C::kTeams, parts = workers / heads <= 2 * C::kTeams ? workers / heads : workers / heads / C::kTeams + C::kTeams;
+  if (parts > 8 && items <= 2 * (int64_t)sm_count())
     TF_CUDA(join(std::integral_constant<int, 16>{}));
-  else if (workers > heads * 4)
+  else if (parts > 4)
     TF_CUDA(join(std::integral_constant<int, 4>{}));
   else
     TF_CUDA(join(std::integral_constant<int, 1>{}));

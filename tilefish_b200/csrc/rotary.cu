@@ -163,16 +163,23 @@ struct VectorPlan {
   int items;           // threads that have 16 elements of it
   Divisor heads, half; // rows of a token; pairs of a head
   int max_tokens;      // that one block's rows touch
+  int staged;          // where in shared memory the block's rows are
   int lanes, table;    // cosines of pair i of a token: at (i % p) * lanes + i / p of its `table` ones, p pairs in a vector
 };
 
-template <typename T, bool kAppend, bool kInterleaved, int kRows, int kBlocks>
+// How a thread comes by the other half of its pairs: it has them (half layout, halves of whole vectors; interleaved), or reads them from the row in shared
+// memory (half layout, any rot).
+enum { kHalves, kNeighbours, kStaged };
+
+template <typename T, bool kAppend, int kMode, int kRows, int kBlocks>
 __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(const RotaryArgs p, const VectorPlan plan) {
   using X = Vectors<T>;
+  constexpr bool kInterleaved = kMode == kNeighbours;
   constexpr int kE = X::kElems, kV = X::kCount, kPairs = kInterleaved ? kE / 2 : kE;
   extern __shared__ __align__(16) uint8_t smem[];
   float2* table = reinterpret_cast<float2*>(smem);
   int64_t* entry = reinterpret_cast<int64_t*>(table + plan.max_tokens * plan.table);  // [tokens of the block] where keys and values go
+  [[maybe_unused]] T* staged = reinterpret_cast<T*>(smem + plan.staged);               // [rows of the block][d]
   const int slots = kRotaryThreads >> plan.lanes_log2, slot = threadIdx.x >> plan.lanes_log2, item = threadIdx.x & ((1 << plan.lanes_log2) - 1);
   const int64_t r0 = (int64_t)blockIdx.x * (slots * kRows), t0 = r0 / p.heads;
   const int first = (int)(r0 - t0 * p.heads), half = p.rot / 2;
@@ -182,8 +189,8 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
     for (int t = threadIdx.x; t < tokens; t += kRotaryThreads) entry[t] = entry_offset(p, t0 + t, 0);
 
   // this thread's vectors of a row lie at base + v * step. Half layout: vectors v and v + kV / 2 are pairs' two halves, or, from rot on, copied
-  const bool pairs = kInterleaved || item * 16 < p.rot;
-  const int base = pairs ? item * kE : p.rot + (item - p.rot / 16) * kE, step = kInterleaved ? p.d / kV : pairs ? p.rot / kV : (p.d - p.rot) / kV;
+  const bool pairs = kMode != kHalves || item * 16 < p.rot;
+  const int base = pairs ? item * kE : p.rot + (item - p.rot / 16) * kE, step = kMode != kHalves ? p.d / kV : pairs ? p.rot / kV : (p.d - p.rot) / kV;
   X x[kRows];
   int token[kRows], head[kRows];
 #pragma unroll
@@ -202,7 +209,10 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
       if (h >= 0) src = reinterpret_cast<const T*>(h < kv ? p.k + t * p.k_ldt + h * p.k_ldh : p.v + t * p.v_ldt + (h - kv) * p.v_ldh);
     }
 #pragma unroll
-    for (int v = 0; v < kV; ++v) x[u].w[v] = *reinterpret_cast<const uint4*>(src + base + v * step);
+    for (int v = 0; v < kV; ++v) {
+      x[u].w[v] = *reinterpret_cast<const uint4*>(src + base + v * step);
+      if constexpr (kMode == kStaged) *reinterpret_cast<uint4*>(staged + (slot + u * slots) * p.d + base + v * step) = x[u].w[v];
+    }
   }
   for (int i = threadIdx.x; i < tokens * half; i += kRotaryThreads) {
     const int t = divide(i, plan.half), pair = i - t * half;
@@ -220,11 +230,23 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
     auto turned = [&](auto put) {
       const X y = x[u];
 #pragma unroll
-      for (int v = 0; v < (kInterleaved ? kV : kV / 2); ++v) {
+      for (int v = 0; v < (kMode != kHalves ? kV : kV / 2); ++v) {
         const float2* c = cs + (base + v * step) / kE;
 #pragma unroll
         for (int e = 0; e < kE; e += 2) {
-          if constexpr (kInterleaved) {
+          if constexpr (kMode == kStaged) {
+            const T* row = staged + (slot + u * slots) * p.d;
+            float z[2] = {y.get(v, e), y.get(v, e + 1)};
+            const int j0 = base + v * step + e;
+            if (j0 >= p.rot) continue;  // copied: keeps its bits (rot is even)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int j = j0 + i, pair = j < half ? j : j - half;
+              const float2 c0 = cs[(pair & (kPairs - 1)) * plan.lanes + pair / kPairs];
+              z[i] = j < half ? fmaf(z[i], c0.x, -(as_f32(row[j + half]) * c0.y)) : fmaf(z[i], c0.x, as_f32(row[j - half]) * c0.y);
+            }
+            put(v, e, z[0], z[1]);
+          } else if constexpr (kInterleaved) {
             if (base + v * step + e >= p.rot) continue;  // copied: keeps its bits
             const float2 c0 = c[e / 2 * plan.lanes];
             const float a = y.get(v, e), b = y.get(v, e + 1);
@@ -283,8 +305,15 @@ static tf_status launch_rotary_rows(const RotaryArgs& p, VectorPlan plan, cudaSt
   const int per = Vectors<T>::kElems / (p.interleaved ? 2 : 1);
   plan.lanes = (p.rot / 2 + per - 1) / per;
   plan.table = per * plan.lanes;
-  const size_t smem = (size_t)plan.max_tokens * (plan.table * sizeof(float2) + (kAppend ? sizeof(int64_t) : 0));
-  auto kernel = p.interleaved ? rotary_vector_kernel<T, kAppend, true, kRows, kBlocks> : rotary_vector_kernel<T, kAppend, false, kRows, kBlocks>;
+  size_t smem = (size_t)plan.max_tokens * (plan.table * sizeof(float2) + (kAppend ? sizeof(int64_t) : 0));
+  auto kernel = p.interleaved ? rotary_vector_kernel<T, kAppend, kNeighbours, kRows, kBlocks> : rotary_vector_kernel<T, kAppend, kHalves, kRows, kBlocks>;
+  if constexpr (kRows == 1) {
+    if (!p.interleaved && p.rot % 16) {  // at most 16 KB of angles, 4 of entries and 16 of rows
+      plan.staged = (int)((smem + 15) / 16 * 16);
+      smem = plan.staged + (size_t)rows * p.d * sizeof(T);
+      kernel = rotary_vector_kernel<T, kAppend, kStaged, kRows, kBlocks>;
+    }
+  }
   kernel<<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(p, plan);
   TF_LAUNCH_CHECK();
   return TF_OK;
@@ -299,16 +328,16 @@ static tf_status launch_rotary_vectors(const RotaryArgs& p, cudaStream_t stream)
   plan.items = p.d / 16;
   while ((1 << plan.lanes_log2) < plan.items) ++plan.lanes_log2;
   const int64_t two = (int64_t)(kRotaryThreads >> plan.lanes_log2) * 2;
-  if (p.tokens * p.heads <= two * 2 * sm_count()) return launch_rotary_rows<T, kAppend, 1, sizeof(T) == 2 ? 6 : 4>(p, plan, stream);
+  if (p.tokens * p.heads <= two * 2 * sm_count() || (!p.interleaved && p.rot % 16)) return launch_rotary_rows<T, kAppend, 1, sizeof(T) == 2 ? 6 : 4>(p, plan, stream);
   return launch_rotary_rows<T, kAppend, 2, !kAppend && sizeof(T) == 2 ? 5 : kAppend ? 3 : 4>(p, plan, stream);
 }
 
 template <typename T, bool kAppend>
 static tf_status launch_rotary(const RotaryArgs& p, cudaStream_t stream) {
-  // Whole vectors need 16-byte aligned rows, whole vectors of pairs in the half layout, and a row that at most one block's threads hold.
+  // Whole vectors need 16-byte aligned rows of whole vectors.
   const int64_t unit = 16 / (int64_t)sizeof(T);
   auto aligned = [&](const void* x, int64_t a, int64_t b) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && a % unit == 0 && b % unit == 0; };
-  if (p.d % 16 == 0 && (p.interleaved || p.rot % 16 == 0) && aligned(p.q, p.q_ldt, p.q_ldh) && aligned(p.q_out, p.qo_ldt, p.qo_ldh))
+  if (p.d % 16 == 0 && aligned(p.q, p.q_ldt, p.q_ldh) && aligned(p.q_out, p.qo_ldt, p.qo_ldh))
     return launch_rotary_vectors<T, kAppend>(p, stream);
   const int64_t total = p.tokens * p.heads * (p.d - p.rot / 2), cap = (int64_t)sm_count() * 8;
   const int64_t need = (total + kRotaryThreads - 1) / kRotaryThreads;
