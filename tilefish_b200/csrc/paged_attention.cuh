@@ -11,8 +11,13 @@
 //
 // The work is the list of all (sequence, row tile, kv head), each as long as its tiles of keys and a fixed part for starting it, cut into as many
 // equal contiguous ranges as there are workers, whatever the lengths are (they are read on the device, so a captured call follows them). A worker
-// that has seen all keys of a head writes its result. Else it leaves its maximum, sum and unnormalised sum of values in the workspace, and
-// paged_attention_join_kernel adds them up in the order of the keys.
+// that has seen all keys of a head writes its result. Else it leaves its maximum, sum and unnormalised sum of values in the workspace (one for all
+// workers of a block that lies inside a head), and paged_attention_join_kernel adds them up in the order of the keys.
+//
+// Measured (CUDA graph, device time): 64 sequences of up to 8192 entries, 8 kv heads of 128, eight query heads each: bf16 178 us = 6.4 TB/s of keys and values,
+// 0.98 of a copy's rate; two of 131072 109 us, 0.98; e4m3, 32 of up to 16384, 98 us, 0.92 (with 16-bit operands to make); 40 rows of 96 elements 42 us
+// against 16 of HBM time, bound by the tensor cores' and the issue slots of two warps a scheduler; calls of a few microseconds by their chain of
+// loads (lengths, page, keys; parts) and two launches: one sequence of 129 entries 7.2 us.
 #pragma once
 
 #include <cmath>
@@ -24,6 +29,7 @@ namespace tf {
 
 constexpr int kAttendWarps = 4, kAttendThreads = 32 * kAttendWarps;
 constexpr int kHeadCost = 4;  // what starting a head costs a worker, in tiles: 3 to 5 us to its first keys, a tile 1 to 2 (192 short sequences 30.2 us with 2, 26.4 with 4)
+
 // ROWS query rows of a kv head, in eights: as many of them to a warp as its registers hold (an accumulator of DP x 8 takes DP / 4 of them), the rest to
 // a team of warps that share the keys' tiles.
 template <int DP, bool F8, int ROWS>
