@@ -55,7 +55,7 @@ def test_rotary_refuses(status, change):
 
 BAD_CACHES = [(BAD, {"k": None}), (BAD, {"v": None}), (BAD, {"dtype": 2}), (BAD, {"pages": 0}), (BAD, {"pages": 1 << 31}), (BAD, {"page_size": 0}), (BAD, {"kv_heads": 0}),
               (NOT, {"head_dim": 40}), (NOT, {"head_dim": 272}), (NOT, {"head_dim": 0}), (ODD, {"k": AT + 8}), (ODD, {"v": AT + 8}), (ODD, {"stride_slot": 68}), (ODD, {"stride_page": -2048}),
-              (ODD, {"stride_head": 1032, "dtype": 1}), (BAD, {"k_scale": AT})]
+              (ODD, {"stride_head": 1032, "dtype": 1}), (BAD, {"k_scale": AT}), (ODD, {"v_scale": AT + 2, "dtype": 1})]
 
 
 @needs_library
@@ -69,7 +69,8 @@ def test_a_bad_cache_is_refused(status, change):
 @pytest.mark.parametrize("status,change", [(BAD, {"k": None}), (BAD, {"v": None}), (BAD, {"tables": None}), (BAD, {"positions": None}), (BAD, {"q": None}), (BAD, {"q_out": None}),
                                            (BAD, {"q": None, "q_out": None}), (BAD, {"tokens": -1}), (BAD, {"tokens": 3}), (BAD, {"table_rows": 0}), (BAD, {"table_cols": 0}),
                                            (BAD, {"q_heads": -1}), (BAD, {"bits": 8}), (BAD, {"layout": -1}), (BAD, {"rot": 66}), (BAD, {"turns": None}), (BAD, {"rot": 0}),
-                                           (ODD, {"k": AT + 2}), (ODD, {"v": AT + 4}), (ODD, {"q": AT + 8}), (ODD, {"q_out": AT + 8}), (ODD, {"kt": 100}), (ODD, {"oh": 4})])
+                                           (ODD, {"k": AT + 2}), (ODD, {"v": AT + 4}), (ODD, {"q": AT + 8}), (ODD, {"q_out": AT + 8}), (ODD, {"kt": 100}), (ODD, {"oh": 4}), (ODD, {"tables": AT + 2}),
+                                           (ODD, {"rows": AT + 1}), (ODD, {"positions": AT + 2})])
 def test_append_refuses(status, change):
     assert append(**change) == status and N.last_error()
 
@@ -77,7 +78,8 @@ def test_append_refuses(status, change):
 @needs_library
 @pytest.mark.parametrize("status,change", [(BAD, {"q": None}), (BAD, {"out": None}), (BAD, {"tables": None}), (BAD, {"lengths": None}), (BAD, {"seqs": -1}), (BAD, {"queries": 0}),
                                            (BAD, {"q_heads": 0}), (BAD, {"q_heads": 3}), (BAD, {"table_cols": 0}), (BAD, {"window": -1}), (BAD, {"seqs": 1 << 31}),
-                                           (ODD, {"q": AT + 8}), (ODD, {"out": AT + 8}), (ODD, {"workspace": AT + 8}), (ODD, {"qt": 100}), (ODD, {"oh": 12})])
+                                           (ODD, {"q": AT + 8}), (ODD, {"out": AT + 8}), (ODD, {"workspace": AT + 8}), (ODD, {"qt": 100}), (ODD, {"oh": 12}), (ODD, {"tables": AT + 2}), (ODD, {"lengths": AT + 1}),
+                                           (ODD, {"counts": AT + 2}), (ODD, {"lse": AT + 2}), (BAD, {"scale": math.inf}), (BAD, {"scale": math.nan})])
 def test_attention_refuses(status, change):
     assert attend(**change) == status and N.last_error()
 
@@ -127,7 +129,7 @@ def test_frequencies_refuse(kwargs):
 
 
 def test_a_table_refuses():
-    for args, kwargs in (([[1.0]], {"layout": "pairs"}), ([[]], {}), ([[math.nan]], {}), ([[1.0]], {"magnitude": math.inf}), ([[1.0] * 513], {})):
+    for args, kwargs in (([[1.0]], {"layout": "pairs"}), ([[]], {}), ([[math.nan]], {}), ([[2.0**33]], {}), ([[1.0]], {"magnitude": math.inf}), ([[1.0]], {"magnitude": 1e39}), ([[1.0] * 513], {})):
         with pytest.raises(TilefishPreconditionError):
             A.RotaryTable(*args, device="cpu", **kwargs)
     assert A.RotaryTable([1.0, 0.5], device="cpu").rot == 4

@@ -146,6 +146,16 @@ def test_many_sequences(A, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("level", [-30000.0, 30000.0])
+def test_parts_of_high_and_low_scores_are_joined_as_they_are(A, dtype, level):
+    """A large common level of the scores (an element of q and k apart from the others) changes no weight, in one worker or between the parts of many."""
+    q, cache, tables, lengths = setup(A, [3000], 1, 1, 4, 32, 16, dtype, scales=False, peak=0.25)
+    q[:, :, 0] = level / 128
+    cache.k[..., 0] = torch.tensor(128.0).to(R.E4M3).view(torch.uint8).cuda() if dtype == "e4m3" else 128.0
+    run(A, q, cache, tables, lengths, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 @pytest.mark.parametrize("peak", [0.0, 30.0, 1000.0])
 def test_flat_and_peaked_scores(A, dtype, peak):
     run(A, *setup(A, [129, 1000], 1, 2, 4, 64, 16, dtype, peak=peak))
@@ -337,7 +347,10 @@ def test_empty_and_refusals(A):
     refused("dtype", q, cache, tables, lengths.long())
     refused("shape", q, cache, tables, lengths, counts=lengths[:1])
     refused("argument", q, cache, tables, lengths, window=-1)
+    refused("argument", q, cache, tables, lengths, window=2**64 + 5)
     refused("argument", q, cache, tables, lengths, scale=math.nan)
+    refused("argument", q, cache, tables, lengths, scale=1e39)
+    assert torch.equal(A.paged_attention(q, cache, tables, lengths, window=2**62), A.paged_attention(q, cache, tables, lengths))
     refused("alias", q, cache, tables, lengths, out=q)
     refused("shape", q, cache, tables, lengths, out=q[:2].clone())
     refused("shape", q, cache, tables, lengths, lse=torch.empty((4, 7), device="cuda"))

@@ -118,7 +118,7 @@ class RotaryTable:
     def __init__(self, inv_freq, *, layout: str = "half", magnitude: float = 1.0, device=None) -> None:
         torch = _torch()
         _pre(layout in LAYOUTS, f"unknown layout {layout!r}: one of {sorted(LAYOUTS)}", "argument", "layout")
-        _pre(math.isfinite(magnitude), f"magnitude: {magnitude} is not finite", "argument", "magnitude")
+        _pre(abs(magnitude) <= 2.0**127, f"magnitude: {magnitude} is not a finite float32", "argument", "magnitude")
         if isinstance(inv_freq, torch.Tensor):
             _pre(inv_freq.dim() == 1, f"inv_freq: expected rank 1, got {inv_freq.dim()}", "rank", "inv_freq")
             if device is None and inv_freq.is_cuda:
@@ -401,10 +401,10 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
         _pre(False, f"q: {tokens} tokens cannot be dealt out evenly to {seqs} sequences", "divisible", "q")
     if scale is None:
         scale = dim**-0.5
-    elif not math.isfinite(scale):
-        _pre(False, f"scale: {scale} is not finite", "argument", "scale")
-    if window < 0:
-        _pre(False, f"window: {window} is negative", "argument", "window")
+    elif not abs(scale) <= 2.0**127:
+        _pre(False, f"scale: {scale} is not a finite float32", "argument", "scale")
+    if not 0 <= window < 2**63:
+        _pre(False, f"window: {window} is negative or more than 63 bits", "argument", "window")
     if out is None:
         out = torch.empty_strided(shape, (heads * dim, dim, 1), dtype=q.dtype, device=cache.device)
         ot, oh, op = heads * dim, dim, out.data_ptr()

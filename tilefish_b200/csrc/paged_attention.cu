@@ -1,4 +1,5 @@
 // The entry points of attention over a paged key-value cache. The kernels are in paged_attention.cuh, built by head size in paged_attention_<type>_d<size>.cu.
+#include <cmath>
 #include <type_traits>
 
 #include "paged_attention.h"
@@ -126,6 +127,11 @@ extern "C" tf_status tf_paged_attention(const tf_paged_cache* cache, const void*
   TF_CHECK_ALIGNED(q, 16, "q");
   TF_CHECK_ALIGNED(out, 16, "out");
   TF_CHECK_ALIGNED(workspace, 16, "workspace");
+  TF_CHECK_ALIGNED(tables, 4, "tables");
+  TF_CHECK_ALIGNED(lengths, 4, "lengths");
+  TF_CHECK_ALIGNED(counts, 4, "counts");
+  TF_CHECK_ALIGNED(lse, 4, "lse");
+  TF_CHECK_ARG(std::isfinite(scale), "%s: scale is not finite", __func__);
   if (q_stride_token % 8 || q_stride_head % 8 || out_stride_token % 8 || out_stride_head % 8)
     return fail(TF_ERR_ALIGNMENT, "%s: the strides must be multiples of 8 elements", __func__);
   if (seqs == 0) return TF_OK;

@@ -538,7 +538,8 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
             t = fmaxf(t, __shfl_xor_sync(~0u, t, 4));
             t = fmaxf(t, __shfl_xor_sync(~0u, t, 8));
             t = fmaxf(t, __shfl_xor_sync(~0u, t, 16));
-            const float now = fmaxf(m[n][h], t - offset[n][h]);  // what was unset has offset 0
+            // A whole number: its differences, and the factors between parts, are exact. What was unset has offset 0.
+            const float now = fmaxf(m[n][h], ceilf(t - offset[n][h]));
             const float next = now == -INFINITY ? 0.0f : C::kShift - now;
             const float keep = exp2_approx(m[n][h] - (now == -INFINITY ? 0.0f : now));
             l[n][h] *= keep;

@@ -17,6 +17,7 @@ inline tf_status check_cache(const tf_paged_cache* c, const char* fn) {
   if (c->stride_page % unit || c->stride_head % unit || c->stride_slot % unit || c->stride_page < 0 || c->stride_head < 0 || c->stride_slot < 0)
     return fail(TF_ERR_ALIGNMENT, "%s: the cache's strides must be multiples of 16 bytes", fn);
   if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16) return fail(TF_ERR_ALIGNMENT, "%s: k and v must be 16-byte aligned", fn);
+  if (reinterpret_cast<uintptr_t>(c->k_scale) % 4 || reinterpret_cast<uintptr_t>(c->v_scale) % 4) return fail(TF_ERR_ALIGNMENT, "%s: the scales must be 4-byte aligned", fn);
   if (c->dtype == TF_CACHE_BF16 && (c->k_scale || c->v_scale)) return fail(TF_ERR_INVALID_ARGUMENT, "%s: a bf16 cache has no scales", fn);
   return TF_OK;
 }

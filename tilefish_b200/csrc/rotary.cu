@@ -401,6 +401,8 @@ extern "C" tf_status tf_cache_append(const tf_paged_cache* cache, const void* k,
   TF_CHECK_ALIGNED(v, 16, "v");
   TF_CHECK_ALIGNED(q, 16, "q");
   TF_CHECK_ALIGNED(q_out, 16, "q_out");
+  TF_CHECK_ALIGNED(tables, 4, "tables");
+  TF_CHECK_ALIGNED(rows, 4, "rows");
   TF_CHECK_ALIGNED(positions, position_bits / 8, "positions");
   if (k_stride_token % 8 || k_stride_head % 8 || v_stride_token % 8 || v_stride_head % 8 || q_stride_token % 8 || q_stride_head % 8 || q_out_stride_token % 8 ||
       q_out_stride_head % 8)
