@@ -298,6 +298,34 @@ def test_captured_with_new_lengths_and_two_graphs(A):
         assert torch.equal(eager, graphs[0][1])
 
 
+def test_captured_on_a_forked_stream(A):
+    """Both launches behind an event, a copy and a memset of another stream, and in front of a kernel of it."""
+    q, cache, tables, lengths = setup(A, [2000, 70, 5], 1, 2, 4, 64, 16, "bf16")
+    qs, ts, ls = q.cuda(), tables.cuda(), lengths.cuda()
+    source, held = qs.clone(), torch.empty_like(qs)
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    main.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(main):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            held.zero_()
+            held.copy_(source)
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                out = A.paged_attention(held, cache, ts, ls)
+                twice = A.paged_attention(held, cache, ts, ls, window=33)
+            main.wait_stream(side)
+            total = out.float() + twice.float()
+    for scale in (1.0, 0.5):
+        source.copy_(qs * scale)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for o, window in ((out, 0), (twice, 33)):
+            R.check_attention(o, None, R.attention(q * scale, cache.k, cache.v, tables, lengths, window=window))
+        assert torch.equal(total, out.float() + twice.float())
+
+
 def test_own_workspace_of_any_content(A):
     q, cache, tables, lengths = setup(A, [3000, 70], 1, 2, 8, 128, 16, "bf16")
     need = A.attention_workspace_bytes(cache, 2, 1, 16, tables.shape[1])
