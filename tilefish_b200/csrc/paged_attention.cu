@@ -10,28 +10,24 @@ extern template struct AttendCall<64, false, 8>;
 extern template struct AttendCall<64, false, 16>;
 extern template struct AttendCall<64, false, 24>;
 extern template struct AttendCall<64, false, 32>;
-extern template struct AttendCall<64, false, 40>;
 extern template struct AttendCall<64, false, 48>;
 extern template struct AttendCall<64, false, 64>;
 extern template struct AttendCall<64, true, 8>;
 extern template struct AttendCall<64, true, 16>;
 extern template struct AttendCall<64, true, 24>;
 extern template struct AttendCall<64, true, 32>;
-extern template struct AttendCall<64, true, 40>;
 extern template struct AttendCall<64, true, 48>;
 extern template struct AttendCall<64, true, 64>;
 extern template struct AttendCall<96, false, 8>;
 extern template struct AttendCall<96, false, 16>;
 extern template struct AttendCall<96, false, 24>;
 extern template struct AttendCall<96, false, 32>;
-extern template struct AttendCall<96, false, 40>;
 extern template struct AttendCall<96, false, 48>;
 extern template struct AttendCall<96, false, 64>;
 extern template struct AttendCall<96, true, 8>;
 extern template struct AttendCall<96, true, 16>;
 extern template struct AttendCall<96, true, 24>;
 extern template struct AttendCall<96, true, 32>;
-extern template struct AttendCall<96, true, 40>;
 extern template struct AttendCall<96, true, 48>;
 extern template struct AttendCall<96, true, 64>;
 extern template struct AttendCall<128, false, 8>;
@@ -55,16 +51,15 @@ extern template struct AttendCall<256, true, 16>;
 extern template struct AttendCall<256, true, 32>;
 extern template struct AttendCall<256, true, 64>;
 
-// Rows of a tile: as few as hold a kv head's query heads times the new tokens, up to 64; more are several tiles, which read the keys again. 40 rows of more
-// than 96 elements are more than a warp's registers hold, and of more than 128 a warp holds 16. One tile is faster than several small ones (12 sequences of up
-// to 16384, bf16: 64 rows of 128 elements 116 us, in tiles of 32, 24 and 16 118, 137 and 181; 40 of 96 elements 72, 98, 84 and 94) but for 33 to 48
-// rows of more than 128 elements, for which 64 is a third too many (256 elements: 284 us, in tiles of 16 270; e4m3 169 and 143).
+// Rows of a tile: as few as hold a kv head's query heads times the new tokens, up to 64; more are several tiles, which read the keys again. One tile is faster
+// than several small ones (12 sequences of up to 16384, bf16: 64 rows of 128 elements 112 us, in tiles of 24 and 16 137 and 181; 48 of 96 elements 67, 84 and 94)
+// but for 33 to 48 rows of more than 128 elements, for which 64 is a third too many (256 elements: 284 us, in tiles of 16 270; e4m3 169 and 143).
 static int attend_rows(int64_t rows, int64_t d) {
   const int64_t tiles = (rows + 63) / 64;
   rows = (rows + tiles - 1) / tiles;  // 80 are twice 40
   if (d > 128) return rows <= 8 ? 8 : rows <= 16 || (rows > 32 && rows <= 48) ? 16 : rows <= 32 ? 32 : 64;
   const int eights = (int)(rows + 7) / 8;
-  return eights <= 4 ? 8 * eights : eights == 5 && d <= 96 ? 40 : eights <= 6 ? 48 : 64;
+  return eights <= 4 ? 8 * eights : eights <= 6 ? 48 : 64;
 }
 static int64_t attend_row_tiles(int64_t rows, int64_t d) {
   const int tile = attend_rows(rows, d);
@@ -84,8 +79,6 @@ static auto with_attend_call(int64_t rows, int64_t d, int32_t dtype, Use use) {
       if (tile == 24) return use(AttendCall<kDP, kF8, 24>{});
       if (tile == 48) return use(AttendCall<kDP, kF8, 48>{});
     }
-    if constexpr (kDP < 128)
-      if (tile == 40) return use(AttendCall<kDP, kF8, 40>{});
     return use(AttendCall<kDP, kF8, 64>{});
   };
   auto by_dim = [&](auto f8) {

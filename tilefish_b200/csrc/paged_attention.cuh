@@ -34,14 +34,15 @@ constexpr int kHeadCost = 4;  // what starting a head costs a worker, in tiles: 
 // a team of warps that share the keys' tiles.
 template <int DP, bool F8, int ROWS>
 struct AttendCfg {
-  static constexpr int kEights = DP == 256 ? (ROWS > 8 ? 2 : 1) : ROWS <= 40 ? ROWS / 8 : ROWS / 16, kTeam = ROWS / (8 * kEights);
+  static constexpr int kEights = DP == 256 ? (ROWS > 8 ? 2 : 1) : ROWS <= 32 ? ROWS / 8 : ROWS / 16, kTeam = ROWS / (8 * kEights);
   static constexpr int kTeams = kAttendWarps / kTeam, kRows = ROWS;
   static constexpr int kItem = F8 ? 1 : 2, kRowBytes = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) * kItem;  // of a staged row: a power of two
   // The query operand takes half the accumulators' registers. Where both do not fit it is read from shared memory with every tile.
   static constexpr bool kQueriesInRegisters = kEights * DP <= 384;
   static constexpr int kQueryBytes = kQueriesInRegisters ? 0 : 8 * kEights * (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) * 2;  // of a warp
-  // keys of a team's tile: a tile costs what ten copies do besides its keys, so 32 where two stages of them fit (e4m3 32 x 16384: 103 us, 116 with 16)
-  static constexpr int kKeys = kRowBytes <= 128 && kEights == 1 ? 32 : 16;
+  // Keys of a team's tile: a tile costs as much as the products of eight rows do besides its keys, so 32 where two stages of them fit (12 sequences of up to 16384:
+  // e4m3 8 rows of 128 elements 39 -> 35 us, 16 40 -> 37, 24 49 -> 44; bf16 48 rows of 96 76 -> 67).
+  static constexpr int kKeys = kRowBytes <= 128 || (kTeam == 2 && kRowBytes <= 256) ? 32 : 16;
   static constexpr int kLoadRows = kKeys / kTeam;  // of them, a warp loads
   static constexpr int kHalf = kKeys * kRowBytes;  // the keys of a tile, or its values
   // three blocks an SM where the registers allow it without spilling (64 x 8192 bf16 183 us, 187 with two and a third stage)

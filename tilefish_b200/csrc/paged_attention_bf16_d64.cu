@@ -7,7 +7,6 @@ template struct AttendCall<64, false, 8>;
 template struct AttendCall<64, false, 16>;
 template struct AttendCall<64, false, 24>;
 template struct AttendCall<64, false, 32>;
-template struct AttendCall<64, false, 40>;
 template struct AttendCall<64, false, 48>;
 template struct AttendCall<64, false, 64>;
 

@@ -7,7 +7,6 @@ template struct AttendCall<96, false, 8>;
 template struct AttendCall<96, false, 16>;
 template struct AttendCall<96, false, 24>;
 template struct AttendCall<96, false, 32>;
-template struct AttendCall<96, false, 40>;
 template struct AttendCall<96, false, 48>;
 template struct AttendCall<96, false, 64>;
 

@@ -7,7 +7,6 @@ template struct AttendCall<64, true, 8>;
 template struct AttendCall<64, true, 16>;
 template struct AttendCall<64, true, 24>;
 template struct AttendCall<64, true, 32>;
-template struct AttendCall<64, true, 40>;
 template struct AttendCall<64, true, 48>;
 template struct AttendCall<64, true, 64>;
 

@@ -7,7 +7,6 @@ template struct AttendCall<96, true, 8>;
 template struct AttendCall<96, true, 16>;
 template struct AttendCall<96, true, 24>;
 template struct AttendCall<96, true, 32>;
-template struct AttendCall<96, true, 40>;
 template struct AttendCall<96, true, 48>;
 template struct AttendCall<96, true, 64>;
 
