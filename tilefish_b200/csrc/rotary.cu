@@ -69,6 +69,8 @@ __device__ __forceinline__ void put(__nv_bfloat16* to, float x) { *to = __float2
 // One element or pair per thread: any even rot, any alignment.
 template <typename T, bool kAppend>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(RotaryArgs p) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int half = p.rot / 2, items = half + (p.d - p.rot);
   const int64_t total = p.tokens * p.heads * items;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
@@ -180,6 +182,8 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
   float2* table = reinterpret_cast<float2*>(smem);
   int64_t* entry = reinterpret_cast<int64_t*>(table + plan.max_tokens * plan.table);  // [tokens of the block] where keys and values go
   [[maybe_unused]] T* staged = reinterpret_cast<T*>(smem + plan.staged);               // [rows of the block][d]
+  griddep_wait();
+  griddep_launch_dependents();  // what follows (attention over the cache) may take its place while this call's few blocks run
   const int slots = kRotaryThreads >> plan.lanes_log2, slot = threadIdx.x >> plan.lanes_log2, item = threadIdx.x & ((1 << plan.lanes_log2) - 1);
   const int64_t r0 = (int64_t)blockIdx.x * (slots * kRows), t0 = r0 / p.heads;
   const int first = (int)(r0 - t0 * p.heads), half = p.rot / 2;
@@ -294,6 +298,8 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
   }
 }
 
+// Dependents where one block an SM is enough: 16 sequences of 1000 in a decoder layer 56.2 -> 52.4 us, 64 of 2000 167.4 -> 165.9 (captured; the attention behind
+// them starts early too).
 template <typename T, bool kAppend, int kRows, int kBlocks>
 static tf_status launch_rotary_rows(const RotaryArgs& p, VectorPlan plan, cudaStream_t stream) {
   plan.heads = divisor(p.heads);
@@ -314,8 +320,7 @@ static tf_status launch_rotary_rows(const RotaryArgs& p, VectorPlan plan, cudaSt
       kernel = rotary_vector_kernel<T, kAppend, kStaged, kRows, kBlocks>;
     }
   }
-  kernel<<<(unsigned)blocks, kRotaryThreads, smem, stream>>>(p, plan);
-  TF_LAUNCH_CHECK();
+  TF_CUDA(launch_dependent(blocks <= sm_count(), kernel, dim3((unsigned)blocks), dim3(kRotaryThreads), smem, stream, p, plan));
   return TF_OK;
 }
 
@@ -341,8 +346,7 @@ static tf_status launch_rotary(const RotaryArgs& p, cudaStream_t stream) {
     return launch_rotary_vectors<T, kAppend>(p, stream);
   const int64_t total = p.tokens * p.heads * (p.d - p.rot / 2), cap = (int64_t)sm_count() * 8;
   const int64_t need = (total + kRotaryThreads - 1) / kRotaryThreads;
-  rotary_kernel<T, kAppend><<<(unsigned)(need < cap ? need : cap), kRotaryThreads, 0, stream>>>(p);
-  TF_LAUNCH_CHECK();
+  TF_CUDA(launch_dependent(need <= sm_count(), rotary_kernel<T, kAppend>, dim3((unsigned)(need < cap ? need : cap)), dim3(kRotaryThreads), 0, stream, p));
   return TF_OK;
 }
 
