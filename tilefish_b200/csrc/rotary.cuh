@@ -190,9 +190,22 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
     // `put(v, e, a, b)` receives elements e and e + 1 of vector v, turned
     auto turned = [&](auto put) {
       const X y = x[u];
+      [[maybe_unused]] auto neighbours = [&](int v, int e, float2 c0) {
+        const float a = y.get(v, e), b = y.get(v, e + 1);
+        put(v, e, fmaf(a, c0.x, -(b * c0.y)), fmaf(b, c0.x, a * c0.y));
+      };
 #pragma unroll
       for (int v = 0; v < (kMode != kHalves ? kV : kV / 2); ++v) {
         const float2* c = cs + (base + v * step) / kE;
+        [[maybe_unused]] const int left = p.rot - (base + v * step);
+        if constexpr (kInterleaved) {  // what a vector has beyond rot is copied: it keeps its bits
+          if (left <= 0) continue;
+          if (left >= kE) {
+#pragma unroll
+            for (int e = 0; e < kE; e += 2) neighbours(v, e, c[e / 2 * plan.lanes]);
+            continue;
+          }
+        }
 #pragma unroll
         for (int e = 0; e < kE; e += 2) {
           if constexpr (kMode == kStaged) {
@@ -208,10 +221,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
             }
             put(v, e, z[0], z[1]);
           } else if constexpr (kInterleaved) {
-            if (base + v * step + e >= p.rot) continue;  // copied: keeps its bits
-            const float2 c0 = c[e / 2 * plan.lanes];
-            const float a = y.get(v, e), b = y.get(v, e + 1);
-            put(v, e, fmaf(a, c0.x, -(b * c0.y)), fmaf(b, c0.x, a * c0.y));
+            if (e < left) neighbours(v, e, c[e / 2 * plan.lanes]);
           } else {
             const float2 c0 = c[e * plan.lanes], c1 = c[(e + 1) * plan.lanes];
             const float a0 = y.get(v, e), b0 = y.get(v + kV / 2, e), a1 = y.get(v, e + 1), b1 = y.get(v + kV / 2, e + 1);
