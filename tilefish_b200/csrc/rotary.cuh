@@ -146,8 +146,9 @@ __global__ void __launch_bounds__(kRotaryThreads, kBlocks) rotary_vector_kernel(
   const int first = (int)(r0 - t0 * p.heads), half = p.rot / 2;
   int tokens = divide(first + slots * kRows - 1, plan.heads) + 1;
   if (tokens > p.tokens - t0) tokens = (int)(p.tokens - t0);
-  if constexpr (kAppend)  // the longest chain of loads (position, page) goes first
-    for (int t = threadIdx.x; t < tokens; t += kRotaryThreads) entry[t] = entry_offset(p, t0 + t);
+  if constexpr (kAppend)  // the longest chain of loads (position, page) goes first, in the warp that
+    // has the fewest angles to make (64 tokens of 80 heads 3.1 -> 2.75 us, 8000 of 48 into e4m3 24.4 -> 23.9)
+    for (int t = kRotaryThreads - 1 - (int)threadIdx.x; t < tokens; t += kRotaryThreads) entry[t] = entry_offset(p, t0 + t);
 
   // this thread's vectors of a row lie at base + v * step. Half layout: vectors v and v + kV / 2 are pairs' two halves, or, from rot on, copied
   const bool pairs = kMode != kHalves || item * 16 < p.rot;
@@ -291,9 +292,9 @@ static tf_status launch_rotary_rows(const RotaryArgs& p, VectorPlan plan, cudaSt
   return TF_OK;
 }
 
-// Two rows a thread keep the loads of a long call in flight (8192 x 64 x 128 bf16: 41.2 us with five blocks an SM, 43.2 with four; one row 42.3 to 54); a
-// call that two rows would not spread over two blocks an SM takes one (64 tokens of 80 heads into a cache 3.2 -> 2.9 us). The append kernel
-// spills at five blocks and the f32 one is slower (5.3 us at four for 1777 x 20 x 80, 6.8 at five).
+// Two rows a thread keep the loads of a long call in flight (8192 x 64 x 128 bf16: 40.8 us with five blocks an SM, 43.2 with four; one row 42.3 to 54;
+// 1777 x 20 x 80 f32 5.05 us, one row 5.8); a call that two rows would not spread over two blocks an SM takes one (4 tokens of 10 heads 2.1 -> 2.0 us;
+// 64 of 80 into a cache 2.75 and 2.85: either will do). The append kernel spills at five blocks and the f32 one is slower (by a quarter).
 template <typename T, bool kAppend>
 static tf_status launch_rotary_vectors(const RotaryArgs& p, cudaStream_t stream) {
   VectorPlan plan = {};
