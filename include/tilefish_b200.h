@@ -225,7 +225,8 @@ TF_API tf_status tf_cache_append(const tf_paged_cache* cache, const void* k, int
  *   q, out     bf16 [seqs * queries, q_heads, head_dim], 16-byte aligned, strides in elements, multiples of 8; out must not overlap q
  *   tables     int32 [seqs, table_cols], row stride table_stride
  *   lse        f32 [seqs * queries, q_heads] dense or NULL: ln sum_e exp(scale * q . k_e)
- *   workspace  tf_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, whose content does not matter
+ *   workspace  tf_paged_attention_workspace_bytes(...) bytes for max_entries = table_cols * page_size (-1: sizes that are not taken), 16-byte aligned,
+ *              whose content does not matter; its size goes by the current device
  * Scores, softmax statistics and sums are f32. Weights have 16 bits for a bf16 cache; for e4m3 11 bits down to 2^-21 of the largest, and 2^-32 of it is
  * the least that counts. The order of the sums depends on all lengths of the call, not on timing. */
 TF_API int64_t tf_paged_attention_workspace_bytes(int64_t seqs, int64_t queries, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t cache_dtype,

@@ -384,3 +384,15 @@ def test_empty_and_refusals(A):
     refused("shape", q, cache, tables, lengths, lse=torch.empty((4, 7), device="cuda"))
     refused("alignment", torch.zeros((4, 8, 68), dtype=torch.bfloat16, device="cuda")[..., :64], cache, tables, lengths)
     refused("argument", q, cache, tables, lengths, stream=torch.cuda.Stream())
+
+
+@pytest.mark.parametrize("sequences,queries,heads,width", [(2, 0, 8, 3), (-1, 1, 8, 3), (2, 1, 7, 3), (2, 1, 0, 3), (2, 1, 8, 0), (2**31, 1, 8, 3)])
+def test_no_workspace_for_what_is_not_taken(A, sequences, queries, heads, width):
+    from tilefish_b200 import TilefishPreconditionError
+
+    _, cache, _, _ = setup(A, [40, 5], 2, 2, 4, 64, 16, "bf16")
+    with pytest.raises(TilefishPreconditionError) as e:
+        A.attention_workspace_bytes(cache, sequences, queries, heads, width)
+    assert e.value.kind == "unsupported"
+    with pytest.raises(TilefishPreconditionError):
+        A.attention_workspace_bytes((cache.k, cache.v), 2, 1, 8, 3)

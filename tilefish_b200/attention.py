@@ -438,7 +438,12 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
 
 def attention_workspace_bytes(cache: PagedCache, sequences: int, queries: int, q_heads: int, width: int) -> int:
     """Bytes of the ``workspace`` that ``paged_attention`` takes for tables of ``width`` pages (for callers that keep one; it must not serve two calls at once)."""
-    return _workspace_bytes(cache.index, sequences, queries, q_heads, cache.kv_heads, cache.head_dim, cache._desc.dtype, width * cache.page_size)
+    _check_cache(cache)
+    _here(cache.index)  # the size goes by the current device's number of SMs
+    need = _workspace_bytes(cache.index, sequences, queries, q_heads, cache.kv_heads, cache.head_dim, cache._desc.dtype, width * cache.page_size)
+    if need < 0:
+        _pre(False, f"paged_attention does not take {sequences} sequences of {queries} queries of {q_heads} heads over {cache.kv_heads}, tables of {width} pages", "unsupported")
+    return need
 
 
 # ---- the block ------------------------------------------------------------------------------------------------------------------
