@@ -159,6 +159,7 @@ def rotary_frequencies(rot: int, *, base: float = 10000.0, scaling: Optional[str
         return inv, 1.0
     high = (4.0 if scaling == "bands" else 32.0) if high is None else high
     _pre(length > 0 and 0 < low < high, f"scaling {scaling!r} needs length > 0 and 0 < low < high (length={length}, low={low}, high={high})", "argument", "length")
+    _pre(scaling == "bands" or base > 1, f"base={base}: scaling 'yarn' needs frequencies that fall from pair to pair, so more than 1", "argument", "base")
     if scaling == "bands":
         keep = [min(1.0, max(0.0, (length * f / (2 * math.pi) - low) / (high - low))) for f in inv]
         return [f * (k + (1 - k) / factor) for f, k in zip(inv, keep)], 1.0
@@ -166,8 +167,10 @@ def rotary_frequencies(rot: int, *, base: float = 10000.0, scaling: Optional[str
     def index_of(turns: float) -> float:  # the index whose frequency makes so many turns over `length`
         return rot * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    first, last = max(0, math.floor(index_of(high))), min(half - 1, math.ceil(index_of(low)))
-    keep = [1 - min(1.0, max(0.0, (i - first) / max(last - first, 1e-3))) for i in range(half)]
+    # The line between the ends may go on behind the last pair (the method stops it at rot - 1): the slowest pair is then on it, or kept.
+    last = min(rot - 1, math.ceil(index_of(low)))
+    first = min(last - 1, max(0, math.floor(index_of(high))))
+    keep = [1 - min(1.0, max(0.0, (i - first) / (last - first))) for i in range(half)]
     return [f * (k + (1 - k) / factor) for f, k in zip(inv, keep)], 0.1 * math.log(factor) + 1.0
 
 
