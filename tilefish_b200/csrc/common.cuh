@@ -39,10 +39,9 @@ tf_status scale_padding(void* scales, int32_t format, int64_t rows, int64_t k, i
 // Programmatic dependent launch (tf_set_programmatic_launch): a kernel launched through launch_dependent() may be scheduled
 // while the kernel before it on the stream is still draining, so that its launch latency and set-up overlap that tail. Every
 // thread of such a kernel executes griddep_wait() before it reads or writes anything that the kernel in front may write or read; the wait
-// ends when that kernel has completed and its writes are visible. Three things happen before it: a GEMM asks weights into L2
-// (prefetch_b_stage: nothing is read), the nvfp4 quantizer loads the tensor that its own amax launch in front only reads
-// (quantize_tiles_kernel: that launch is a plain one, so the tensor is complete), and the join of paged attention reads lengths that the kernel in
-// front has waited for and only reads.
+// ends when that kernel has completed and its writes are visible. Two things happen before it: a GEMM asks weights into L2
+// (prefetch_b_stage: nothing is read), and the nvfp4 quantizer loads the tensor that its own amax launch in front only reads
+// (quantize_tiles_kernel: that launch is a plain one, so the tensor is complete).
 // Three settings: never, always, or (until the caller says otherwise) for chains of short kernels only (`chain`, see chain_gemm_launch),
 // and those only without an SM margin: a dependent GEMM's waiting CTAs would take the SMs that the margin leaves to the kernel beside it.
 int sm_margin();
