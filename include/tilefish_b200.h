@@ -205,11 +205,12 @@ TF_API tf_status tf_rotary(const void* x, int32_t dtype, int64_t tokens, int64_t
  *   tables     int32 [table_rows, table_cols], row stride table_stride: the pages of each sequence
  *   positions  int32 or int64 [tokens]: the entry that a token's key and value become, and the position of its rotation
  *   rows       int32 [tokens]: the table row of each token's sequence; NULL: token t belongs to row t / (tokens / table_rows)
- *   q, q_out   bf16 [tokens, q_heads, head_dim] or both NULL (q_heads 0); q_out may be q
+ *   q, q_out   bf16 [tokens, q_heads, head_dim] or both NULL (q_heads 0); q_out may be q, and shares memory with nothing else of the call
  *   turns      as in tf_rotary, or NULL (rot 0): nothing is turned
  * An e4m3 entry is the code nearest to x * (1 / scale) (1 / scale rounded once), saturating at 448. k is turned in f32 and rounded once.
  * A token whose position is negative or beyond the table, whose row is outside the table, or whose page is outside the cache is left out: nothing
- * of it is written to the cache (its query is turned like any other). When two tokens name one entry, which of them stays is not specified. */
+ * of it is written to the cache (its query is turned like any other). When two tokens name one entry, which of them stays is not specified.
+ * k, v and q may lie in the cache's memory, but not in entries that the call writes. */
 TF_API tf_status tf_cache_append(const tf_paged_cache* cache, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
                                  int64_t v_stride_token, int64_t v_stride_head, int64_t tokens, const int32_t* tables, int64_t table_rows,
                                  int64_t table_cols, int64_t table_stride, const void* positions, int32_t position_bits, const int32_t* rows, const void* q,
@@ -222,7 +223,8 @@ TF_API tf_status tf_cache_append(const tf_paged_cache* cache, const void* k, int
  * [max(0, E - window), E) with E = L - n + 1 + i (window 0: from 0 on). Queries n and later are padding. Where a query sees nothing, out is 0
  * and lse -inf. An entry whose page number is outside the cache is seen by nobody; lengths and counts are taken within [0, what the table can name]
  * and [0, queries].
- *   q, out     bf16 [seqs * queries, q_heads, head_dim], 16-byte aligned, strides in elements, multiples of 8; out must not overlap q
+ *   q, out     bf16 [seqs * queries, q_heads, head_dim], 16-byte aligned, strides in elements, multiples of 8; out, lse and workspace share memory
+ *              with nothing else of the call
  *   tables     int32 [seqs, table_cols], row stride table_stride
  *   lse        f32 [seqs * queries, q_heads] dense or NULL: ln sum_e exp(scale * q . k_e)
  *   workspace  tf_paged_attention_workspace_bytes(...) bytes for max_entries = table_cols * page_size (-1: sizes that are not taken), 16-byte aligned,

@@ -67,29 +67,75 @@ def _ints(t, name: str, n: Optional[int], index: int) -> int:
     return t.data_ptr()
 
 
+def _span(t):
+    """(first, behind the last) address of a tensor that has elements."""
+    at = t.data_ptr()
+    return at, at + (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _meet(apart: int, axes) -> bool:
+    """Whether two boxes of ``axes`` (stride, lengths in the one and in the other; falling strides, none shorter than what the axes behind it reach) share an
+    element when they begin ``apart`` of each other."""
+    if not axes:
+        return apart == 0
+    stride, na, nb = axes[0]
+    steps = apart // stride  # what is left over lies between two steps
+    return any(-nb < d < na and _meet(apart - d * stride, axes[1:]) for d in (steps, steps + 1))
+
+
 def _overlap(a, b) -> bool:
-    """Whether two [tokens, heads, dim] tensors share memory. Slices of the columns of one matrix do not."""
-
-    def span(t):
-        size = t.element_size()
-        row = (1 + sum((n - 1) * st for n, st in zip(t.shape[1:], t.stride()[1:]))) * size
-        step = t.stride(0) * size
-        return t.data_ptr(), row, step, t.data_ptr() + (t.shape[0] - 1) * step + row
-
+    """Whether two tensors of one rank and a dense last axis share memory. Slices of one tensor with all its strides do not; of tensors whose strides differ,
+    or that overlap themselves, the whole ranges are compared."""
     if a.numel() == 0 or b.numel() == 0:
         return False
-    (a0, arow, astep, a1), (b0, brow, bstep, b1) = span(a), span(b)
+    (a0, a1), (b0, b1) = _span(a), _span(b)
     if a1 <= b0 or b1 <= a0:
         return False
-    if astep != bstep or arow > astep or brow > astep:
-        return True
-    apart = (b0 - a0) % astep
-    return apart < arow or apart + brow > astep
+    size, axes = a.element_size(), [(1, a.shape[-1] * a.element_size(), b.shape[-1] * b.element_size())]
+    for na, nb, sa, sb in zip(a.shape[:-1], b.shape[:-1], a.stride(), b.stride()):
+        na, nb = na if sa else 1, nb if sb else 1  # a broadcast axis is one element
+        if na > 1 or nb > 1:
+            if na > 1 and nb > 1 and sa != sb:
+                return True
+            axes.append(((sa if na > 1 else sb) * size, na, nb))
+    axes.sort()
+    reach = [0, 0]
+    for stride, *n in axes:
+        if stride < max(reach):
+            return True
+        reach = [r + stride * (m - 1) if r else m for r, m in zip(reach, n)]
+    return _meet(b0 - a0, axes[::-1])
+
+
+def _columns(a, b, size: int) -> bool:
+    """Whether two [tokens, heads, dim] tensors, as ``_rows`` gives them, are columns of one matrix that do not meet: what slices of a qkv product are. Most calls with a
+    result of the caller's need no other look (an append in place 13 us a call; with ``_overlap`` alone 31)."""
+    (_, ha, dim), step, sa, a0 = a
+    (_, hb, _), other, sb, b0 = b
+    if step != other or step <= 0:
+        return False
+    wide_a, wide_b, apart = sa * (ha - 1) + dim, sb * (hb - 1) + dim, (b0 - a0) // size % step
+    return wide_a <= apart and apart + wide_b <= step
+
+
+def _ends(rows, size: int):
+    """``_span`` of what ``_rows`` gives."""
+    (tokens, heads, dim), st, sh, at = rows
+    return at, at + ((tokens - 1) * st + (heads - 1) * sh + dim) * size
 
 
 def _result(t, name: str) -> None:
-    """An axis of a result has no stride 0: several elements would be one."""
-    _pre(all(s <= 1 or st > 0 for s, st in zip(t.shape, t.stride())), f"{name}: a broadcast view cannot be written", "alias", name)
+    """No two elements of a [tokens, heads, dim] result are one: no stride 0, and one of the first two axes lies inside a step of the other."""
+    (tokens, heads, dim), (st, sh, _) = t.shape, t.stride()
+    if tokens and heads and not ((heads == 1 or sh >= dim) and (tokens == 1 or st >= (sh * (heads - 1) + dim)) or (tokens == 1 or st >= dim) and (heads == 1 or sh >= st * (tokens - 1) + dim)):
+        _pre(False, f"{name}: elements share memory (strides {tuple(t.stride())}): a broadcast or overlapping view cannot be written", "alias", name)
+
+
+def _apart(lo: int, hi: int, name: str, others) -> None:
+    """The range of what a call writes shares nothing with those of ``others`` (span, name)."""
+    for span, other in others:
+        if lo < span[1] and span[0] < hi:
+            _pre(False, f"{name} overlaps {other}", "alias", name)
 
 
 # ---- rotary positions ---------------------------------------------------------------------------------------------------------
@@ -238,7 +284,7 @@ class PagedCache:
     Which pages belong to which sequence stands in the int32 [sequences, width] tables that the operators take, not here.
     """
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "index", "_desc", "_ref")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "index", "_desc", "_ref", "_spans")
 
     def __init__(self, k, v, k_scale=None, v_scale=None) -> None:
         torch = _torch()
@@ -259,7 +305,7 @@ class PagedCache:
         for st, n in axes:
             _pre(st >= reach, f"k: strides {tuple(k.stride())}: entries overlap", "alias", "k")
             reach = st * (n - 1) + reach
-        _pre(k.data_ptr() != v.data_ptr(), "k and v are the same memory", "alias", "v")
+        _pre(not _overlap(k, v), "k and v share memory", "alias", "v")
         for s, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
             if s is not None:
                 _pre(codes, f"{name}: a bf16 cache has no scales", "argument", name)
@@ -272,6 +318,7 @@ class PagedCache:
                                             v_scale.data_ptr() if v_scale is not None else None, self.pages, self.page_size, self.kv_heads, self.head_dim,
                                             strides[0], strides[1], strides[2], N.CACHE_E4M3 if codes else N.CACHE_BF16, 0)
         self._ref = ctypes.addressof(self._desc)
+        self._spans = (_span(k), "the cache's k"), (_span(v), "the cache's v")
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "bf16", *, k_scale=None, v_scale=None, device="cuda") -> "PagedCache":
@@ -322,6 +369,8 @@ def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=Non
     without ``rows`` the tokens belong to the sequences in turn, tokens / sequences each. With ``rotary`` k and q (bf16 [tokens, q_heads, head_dim]) are
     turned by ``positions``; returns the turned q (``q_out``, which may be q itself, or a new tensor), or None without q.
 
+    k, v and q may lie in the cache's own memory (entries that move), but not in entries that this call writes: which ones those are stands on the device.
+
     A token with a negative position (padding), one beyond its table, a row outside the tables or a page outside the cache is not written. Two tokens
     for one entry: which of them stays is not specified."""
     _check_cache(cache)
@@ -329,7 +378,8 @@ def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=Non
     _here(index)
     kshape, kt, kh, kp = _heads(k, "k", None, cache.kv_heads, dim, index)
     tokens = kshape[0]
-    _, vt, vh, vp = _heads(v, "v", tokens, cache.kv_heads, dim, index)
+    krows, vrows = (kshape, kt, kh, kp), _heads(v, "v", tokens, cache.kv_heads, dim, index)
+    _, vt, vh, vp = vrows
     seqs, cols, table_stride, tp = _check_tables(tables, index)
     pp, bits = _check_positions(positions, tokens, index)
     if rows is not None:
@@ -351,10 +401,13 @@ def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=Non
             q_out = _torch().empty_strided(qshape, (q_heads * dim, dim, 1), dtype=q.dtype, device=cache.device)
             ot, oh, op = q_heads * dim, dim, q_out.data_ptr()
         else:
-            _, ot, oh, op = _heads(q_out, "q_out", tokens, q_heads, dim, index)
+            orows = _heads(q_out, "q_out", tokens, q_heads, dim, index)
+            _, ot, oh, op = orows
             _result(q_out, "q_out")
             _pre((op == qp and ot == qt and oh == qh) or not _overlap(q_out, q), "q_out overlaps q without being q", "alias", "q_out")
-            _pre(not _overlap(q_out, k) and not _overlap(q_out, v), "q_out overlaps k or v", "alias", "q_out")
+            _pre((_columns(orows, krows, 2) or not _overlap(q_out, k)) and (_columns(orows, vrows, 2) or not _overlap(q_out, v)), "q_out overlaps k or v", "alias", "q_out")
+            if tokens and q_heads:
+                _apart(*_ends(orows, 2), "q_out", cache._spans)
         if q_heads == 0:
             qp = op = None
     elif q_out is not None:
@@ -393,7 +446,8 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
     _check_cache(cache)
     index, dim, kv_heads = cache.index, cache.head_dim, cache.kv_heads
     _here(index)
-    shape, qt, qh, qp = _heads(q, "q", None, None, dim, index)
+    qrows = _heads(q, "q", None, None, dim, index)
+    shape, qt, qh, qp = qrows
     tokens, heads = shape[0], shape[1]
     seqs, width, table_stride, tp = _check_tables(tables, index)
     lp = _ints(lengths, "lengths", seqs, index)
@@ -412,13 +466,20 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
         out = torch.empty_strided(shape, (heads * dim, dim, 1), dtype=q.dtype, device=cache.device)
         ot, oh, op = heads * dim, dim, out.data_ptr()
     else:
-        _, ot, oh, op = _heads(out, "out", tokens, heads, dim, index)
+        orows = _heads(out, "out", tokens, heads, dim, index)
+        _, ot, oh, op = orows
         _result(out, "out")
-        _pre(not _overlap(out, q), "out overlaps q", "alias", "out")
+        if tokens:
+            (lo, hi), (first, end) = _ends(orows, 2), _ends(qrows, 2)
+            if lo < end and first < hi:
+                _pre(not _overlap(out, q), "out overlaps q", "alias", "out")
+            _apart(lo, hi, "out", cache._spans)
     if lse is not None:
         _check(lse, "lse", torch.float32, 2, cache.device, align=4)
         _pre(tuple(lse.shape) == (tokens, heads), f"lse: shape {tuple(lse.shape)}, expected {(tokens, heads)}", "shape", "lse")
         _dense(lse, "lse")
+        if tokens:
+            _apart(*_span(lse), "lse", (*cache._spans, (_span(q), "q"), (_span(out), "out")))
         return_lse = True
     elif return_lse:
         lse = torch.empty_strided((tokens, heads), (heads, 1), dtype=torch.float32, device=cache.device)
@@ -434,6 +495,13 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
             _dense(workspace, "workspace")
             have = workspace.numel()
             _pre(have >= need, f"workspace: {need} bytes needed", "workspace", "workspace")
+            at = workspace.data_ptr()
+            _apart(at, at + need, "workspace", (*cache._spans, (_ends(qrows, 2), "q"), (_ends((shape, ot, oh, op), 2), "out"), ((lp, lp + 4 * seqs), "lengths"),
+                                                ((tp, tp + 4 * ((seqs - 1) * table_stride + width)), "tables")))
+            if cp is not None:
+                _apart(at, at + need, "workspace", (((cp, cp + 4 * seqs), "counts"),))
+            if return_lse:
+                _apart(at, at + need, "workspace", ((_span(lse), "lse"),))
         N.check(N.load().tf_paged_attention(cache._ref, qp, qt, qh, seqs, queries, heads, tp, width, table_stride, lp, cp, scale, window, op, ot, oh,
                                             lse.data_ptr() if return_lse else None, workspace.data_ptr(), have, _stream(stream)), "tf_paged_attention")
     return (out, lse) if return_lse else out
