@@ -545,27 +545,61 @@ def quantize_attention_weights(w_n, w_qkv, w_o, fmt: str, *, q_heads: int, kv_he
     return AttentionWeights(w_n, K.quantize(w_qkv, fmt), K.quantize(w_o, fmt), q_heads, kv_heads)
 
 
+def _check_product(b, name: str, rows: int, k: int, device) -> None:
+    if not (isinstance(b, K.BlockScaledTensor) and b.layout == "swizzled" and tuple(b.shape) == (rows, k) and b.device == device):
+        _pre(isinstance(b, K.BlockScaledTensor) and b.layout == "swizzled", f"{name}: expected a BlockScaledTensor with swizzled scales", "dtype", name)
+        _pre(tuple(b.shape) == (rows, k), f"{name}: shape {tuple(b.shape)}, expected {(rows, k)}", "shape", name)
+        _pre(False, f"{name}: on {b.device}, the other arguments are on {device}", "device", name)
+
+
+def _check_block(x, w, cache, tables, positions, lengths, rotary, rows, counts, window) -> None:
+    """What the operators of ``attention_block`` would refuse, before the first of them has changed the residual or the cache."""
+    _check_cache(cache)
+    index, dim = cache.index, cache.head_dim
+    _here(index)
+    _check(x, "x", _torch().bfloat16, 2, cache.device)
+    tokens, h = x.shape
+    _pre(w.w_qkv.shape[0] == (w.q_heads + 2 * w.kv_heads) * dim and w.kv_heads == cache.kv_heads,
+         f"the weights' heads ({w.q_heads} + 2 * {w.kv_heads}, {w.w_qkv.shape[0]} rows) do not match the cache's ({cache.kv_heads} of {dim})", "shape", "cache")
+    _check_product(w.w_qkv, "w_qkv", w.w_qkv.shape[0], h, cache.device)
+    _check_product(w.w_o, "w_o", h, w.q_heads * dim, cache.device)
+    seqs = _check_tables(tables, index)[0]
+    _check_positions(positions, tokens, index)
+    if rows is not None:
+        _ints(rows, "rows", tokens, index)
+    if rotary is not None:
+        _check_table(rotary, dim, index)
+    _ints(lengths, "lengths", seqs, index)
+    if counts is not None:
+        _ints(counts, "counts", seqs, index)
+    if tokens and (seqs == 0 or tokens % seqs):
+        _pre(False, f"x: {tokens} tokens cannot be dealt out evenly to {seqs} sequences", "divisible", "x")
+    if tokens and _workspace_bytes(index, seqs, tokens // seqs, w.q_heads, w.kv_heads, dim, cache._desc.dtype, tables.shape[1] * cache.page_size) < 0:
+        _pre(False, f"x: {seqs} sequences of {tokens // seqs} tokens are more than paged_attention takes", "unsupported", "x")
+    if not 0 <= window < 2**63:
+        _pre(False, f"window: {window} is negative or more than 63 bits", "argument", "window")
+
+
 def attention_block(x, residual, w: AttentionWeights, cache: PagedCache, tables, positions, lengths, rotary: Optional[RotaryTable] = None, *, rows=None, counts=None,
                     window: int = 0, eps: float = 1e-6):
     """One attention block: ``residual += x`` (f32, in place), returns bf16 [tokens, H] = attention(rmsnorm(residual) * w_n) @ w_o^T, the keys and values of the
     tokens written into the cache on the way. ``positions``, ``tables``, ``rows`` as in ``cache_append``, ``lengths`` (after these tokens) and ``counts`` as in
-    ``paged_attention``; the tokens of a sequence stand together, as many for each."""
+    ``paged_attention``; the tokens of a sequence stand together, as many for each. A call that is refused has changed nothing."""
     torch = _torch()
     fmt = w.fmt
-    dim = cache.head_dim
-    _pre(w.w_qkv.shape[0] == (w.q_heads + 2 * w.kv_heads) * dim and w.kv_heads == cache.kv_heads,
-         f"the weights' heads ({w.q_heads} + 2 * {w.kv_heads}, {w.w_qkv.shape[0]} rows) do not match the cache's ({cache.kv_heads} of {dim})", "shape", "cache")
+    _check_block(x, w, cache, tables, positions, lengths, rotary, rows, counts, window)
+    tokens, dim = x.shape[0], cache.head_dim
     if fmt == "nvfp4":
         amax = torch.zeros(1, dtype=torch.float32, device=x.device)
         h = K.residual_add_rmsnorm(x, residual, w.w_n, eps, amax_out=amax)
         hq = K.quantize(h, fmt, amax=amax)
     else:
         _, hq = K.residual_add_rmsnorm(x, residual, w.w_n, eps, quantize_to=fmt, want_bf16=False)
-    qkv = K.gemm_blockscaled(hq, w.w_qkv).view(x.shape[0], -1, dim)
+    qkv = K.gemm_blockscaled(hq, w.w_qkv).view(tokens, w.q_heads + 2 * w.kv_heads, dim)
     q, k, v = qkv.split([w.q_heads, w.kv_heads, w.kv_heads], dim=1)
     cache_append(cache, k, v, tables, positions, rows=rows, q=q, rotary=rotary, q_out=q)
     o = paged_attention(q, cache, tables, lengths, counts=counts, window=window)
-    return K.gemm(o.view(x.shape[0], -1), w.w_o)
+    return K.gemm(o.view(tokens, w.q_heads * dim), w.w_o)
 
 
 def decoder_layer(x, residual, attention: AttentionWeights, mlp, cache: PagedCache, tables, positions, lengths, rotary: Optional[RotaryTable] = None, *, rows=None,
@@ -573,5 +607,11 @@ def decoder_layer(x, residual, attention: AttentionWeights, mlp, cache: PagedCac
     """A whole decoder layer: ``attention_block``, then ``mlp.decoder_block`` on its result (``mlp``: ``MlpWeights``). The result is the next layer's ``x``."""
     from .mlp import decoder_block
 
+    _check(x, "x", _torch().bfloat16, 2)
+    _check_product(mlp.w_gu, "w_gu", 2 * mlp.w_d.shape[1], x.shape[1], x.device)
+    _check_product(mlp.w_d, "w_d", x.shape[1], mlp.w_d.shape[1], x.device)
+    _pre(mlp.w_gu.fmt == mlp.w_d.fmt, f"w_gu is {mlp.w_gu.fmt} but w_d is {mlp.w_d.fmt}", "dtype", "w_d")
+    _check(mlp.w_n, "w_n", x.dtype, 1, x.device)
+    _pre(mlp.w_n.shape[0] == x.shape[1], f"w_n: shape {tuple(mlp.w_n.shape)}, expected {(x.shape[1],)}", "shape", "w_n")
     y = attention_block(x, residual, attention, cache, tables, positions, lengths, rotary, rows=rows, counts=counts, window=window, eps=eps)
     return decoder_block(y, residual, mlp, eps)
