@@ -281,7 +281,8 @@ class PagedCache:
                   both), so ``empty(...)``'s order and views of [pages, page_size, kv_heads, head_dim] tensors are both fine
     ``k_scale``, ``v_scale``  float32 [kv_heads] for e4m3 (an entry's value is code * scale; None: 1)
 
-    Which pages belong to which sequence stands in the int32 [sequences, width] tables that the operators take, not here.
+    Which pages belong to which sequence stands in the int32 [sequences, width] tables that the operators take, not here. The tensors' contents, scales included,
+    may change between calls; other tensors are another cache (the operators go by the addresses that the cache was made with).
     """
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "device", "index", "_desc", "_ref", "_spans")
@@ -294,14 +295,14 @@ class PagedCache:
         _check(v, "v", dtype, 4, k.device)
         _pre(k.shape == v.shape, f"v: shape {tuple(v.shape)}, expected {tuple(k.shape)}", "shape", "v")
         _pre(min(k.shape) > 0, f"k: shape {tuple(k.shape)} has an empty axis", "shape", "k")
-        self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        _pre(self.head_dim % 16 == 0 and self.head_dim <= 256, f"k: head_dim {self.head_dim} is not a multiple of 16 up to 256", "divisible", "k")
+        pages, kv_heads, page_size, head_dim = k.shape
+        _pre(head_dim % 16 == 0 and head_dim <= 256, f"k: head_dim {head_dim} is not a multiple of 16 up to 256", "divisible", "k")
         _pre(k.stride(3) == 1 and v.stride(3) == 1, "k, v: the last axis must be dense", "contiguous", "k")
         strides = [k.stride(i) if k.shape[i] > 1 else 0 for i in range(3)]
         _pre(strides == [v.stride(i) if v.shape[i] > 1 else 0 for i in range(3)], f"v: strides {tuple(v.stride())}, expected those of k, {tuple(k.stride())}", "contiguous", "v")
         _pre(all(s % unit == 0 for s in strides), f"k: strides {tuple(k.stride())} must be multiples of {unit} elements", "alignment", "k")
         axes = sorted((st, n) for st, n in zip(strides, k.shape[:3]) if n > 1)
-        reach = self.head_dim
+        reach = head_dim
         for st, n in axes:
             _pre(st >= reach, f"k: strides {tuple(k.stride())}: entries overlap", "alias", "k")
             reach = st * (n - 1) + reach
@@ -311,14 +312,19 @@ class PagedCache:
                 _pre(codes, f"{name}: a bf16 cache has no scales", "argument", name)
                 _check(s, name, torch.float32, 1, k.device, align=4)
                 _dense(s, name)
-                _pre(s.shape[0] == self.kv_heads, f"{name}: {s.shape[0]} of them for {self.kv_heads} heads", "shape", name)
-        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
-        self.index = k.get_device()
-        self._desc = N.PagedCacheDescriptor(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
-                                            v_scale.data_ptr() if v_scale is not None else None, self.pages, self.page_size, self.kv_heads, self.head_dim,
-                                            strides[0], strides[1], strides[2], N.CACHE_E4M3 if codes else N.CACHE_BF16, 0)
-        self._ref = ctypes.addressof(self._desc)
-        self._spans = (_span(k), "the cache's k"), (_span(v), "the cache's v")
+                _pre(s.shape[0] == kv_heads, f"{name}: {s.shape[0]} of them for {kv_heads} heads", "shape", name)
+        desc = N.PagedCacheDescriptor(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else None, v_scale.data_ptr() if v_scale is not None else None,
+                                      pages, page_size, kv_heads, head_dim, strides[0], strides[1], strides[2], N.CACHE_E4M3 if codes else N.CACHE_BF16, 0)
+        values = (k, v, k_scale, v_scale, pages, kv_heads, page_size, head_dim, k.device, k.get_device(), desc, ctypes.addressof(desc),
+                  ((_span(k), "the cache's k"), (_span(v), "the cache's v")))
+        for name, value in zip(self.__slots__, values, strict=True):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value) -> None:
+        raise AttributeError(f"PagedCache.{name} cannot be exchanged: its tensors' contents may be changed in place, other tensors are another cache")
+
+    def __reduce__(self):  # a copy is a cache over the tensors' copies
+        return type(self), (self.k, self.v, self.k_scale, self.v_scale)
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "bf16", *, k_scale=None, v_scale=None, device="cuda") -> "PagedCache":
