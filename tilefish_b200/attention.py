@@ -157,6 +157,8 @@ class RotaryTable:
     ``inv_freq``   radians per position, rot / 2 of them (a tensor or a sequence; taken in 64 bits, read on the host once, here)
     ``layout``     "half": pairs (i, i + rot / 2); "interleaved": pairs (2i, 2i + 1)
     ``magnitude``  factor of the turned elements (long-context scalings use it); elements from rot on are left alone
+
+    Made once per set of frequencies, and not while a CUDA graph is captured: frequencies on the device are waited for, and the table is copied there.
     """
 
     __slots__ = ("rot", "layout", "magnitude", "turns", "index", "_layout")
@@ -173,9 +175,16 @@ class RotaryTable:
         values = [float(f) for f in inv_freq]
         _pre(1 <= len(values) <= 512, f"inv_freq: {len(values)} frequencies; 1 to 512 are possible", "shape", "inv_freq")
         _pre(all(abs(f) <= 2.0**32 for f in values), "inv_freq: not finite, or more than 2^32 radians", "argument", "inv_freq")
-        self.rot, self.layout, self.magnitude, self._layout = 2 * len(values), layout, float(magnitude), LAYOUTS[layout]
-        self.turns = torch.tensor(_turns(values), dtype=torch.int64, device=device if device is not None else "cuda")
-        self.index = self.turns.get_device()
+        turns = torch.tensor(_turns(values), dtype=torch.int64, device=device if device is not None else "cuda")
+        for name, value in zip(self.__slots__, (2 * len(values), layout, float(magnitude), turns, turns.get_device(), LAYOUTS[layout]), strict=True):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value) -> None:
+        raise AttributeError(f"RotaryTable.{name} cannot be exchanged: other frequencies, layouts or magnitudes are another table")
+
+    def __setstate__(self, state) -> None:
+        for name, value in state[1].items():
+            object.__setattr__(self, name, value)
 
     def __repr__(self) -> str:
         return f"RotaryTable(rot={self.rot}, {self.layout}, magnitude={self.magnitude:g})"
