@@ -253,7 +253,8 @@ def _check_table(table, dim: int, index: int) -> None:
 def rotary(x, positions, table: RotaryTable, *, out=None, inverse: bool = False, stream=None):
     """``x`` (bf16 or f32 [tokens, heads, head_dim], dense heads at any strides) with each token's heads turned by its position; f32 arithmetic, one rounding.
     ``inverse`` turns back by the same angle: the transposed map, so the gradient of ``rotary`` is ``rotary(grad, ..., inverse=True)``. ``out=x`` works in place.
-    Positions are int32 or int64 of any size: an angle is exact to 2^-65 turns times the position."""
+    Positions are int32 or int64 of any size: an angle is exact to 2^-65 turns times the position, and rounded to f32 as its distance from the nearest
+    quarter turn (2^-28 turns at the most)."""
     torch = _torch()
     f32 = isinstance(x, torch.Tensor) and x.dtype == torch.float32
     dtype, item = (torch.float32, 4) if f32 else (torch.bfloat16, 2)
