@@ -209,7 +209,8 @@ TF_API tf_status tf_rotary(const void* x, int32_t dtype, int64_t tokens, int64_t
  *   turns      as in tf_rotary, or NULL (rot 0): nothing is turned
  * An e4m3 entry is the code nearest to x * (1 / scale) (1 / scale rounded once), saturating at 448. k is turned in f32 and rounded once.
  * A token whose position is negative or beyond the table, whose row is outside the table, or whose page is outside the cache is left out: nothing
- * of it is written to the cache (its query is turned like any other). When two tokens name one entry, which of them stays is not specified.
+ * of it is written to the cache (its query is turned like any other). When two tokens name one entry, its content is unspecified: it may hold parts of both, and
+ * the key of one beside the value of the other.
  * k, v and q may lie in the cache's memory, but not in entries that the call writes. */
 TF_API tf_status tf_cache_append(const tf_paged_cache* cache, const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
                                  int64_t v_stride_token, int64_t v_stride_head, int64_t tokens, const int32_t* tables, int64_t table_rows,

@@ -387,8 +387,8 @@ def cache_append(cache: PagedCache, k, v, tables, positions, *, rows=None, q=Non
 
     k, v and q may lie in the cache's own memory (entries that move), but not in entries that this call writes: which ones those are stands on the device.
 
-    A token with a negative position (padding), one beyond its table, a row outside the tables or a page outside the cache is not written. Two tokens
-    for one entry: which of them stays is not specified."""
+    A token with a negative position (padding), one beyond its table, a row outside the tables or a page outside the cache is not written. Where two
+    tokens name one entry its content is unspecified: parts of both, or the key of one beside the value of the other. No entry of another position changes."""
     _check_cache(cache)
     index, dim = cache.index, cache.head_dim
     _here(index)
