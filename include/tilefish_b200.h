@@ -174,7 +174,8 @@ enum { TF_CACHE_BF16 = 0, TF_CACHE_E4M3 = 1 };
 typedef struct {
   void* k;              /* 16-byte aligned */
   void* v;
-  const float* k_scale; /* TF_CACHE_E4M3: f32 [kv_heads] on the device, an entry's value is code * scale; NULL stands for 1. Else NULL */
+  const float* k_scale; /* TF_CACHE_E4M3: f32 [kv_heads] on the device, an entry's value is code * scale; NULL stands for 1. Neither 0 nor below
+                         * 2^-126, so that 1 / scale is finite (0 * infinity is a NaN entry). Else NULL */
   const float* v_scale;
   int64_t pages, page_size, kv_heads;
   int64_t head_dim;     /* a multiple of 16, at most 256 */
@@ -230,8 +231,9 @@ TF_API tf_status tf_cache_append(const tf_paged_cache* cache, const void* k, int
  *   lse        f32 [seqs * queries, q_heads] dense or NULL: ln sum_e exp(scale * q . k_e)
  *   workspace  tf_paged_attention_workspace_bytes(...) bytes for max_entries = table_cols * page_size (-1: sizes that are not taken), 16-byte aligned,
  *              whose content does not matter; its size goes by the current device
- * Scores, softmax statistics and sums are f32. Weights have 16 bits for a bf16 cache; for e4m3 11 bits down to 2^-21 of the largest, and 2^-32 of it is
- * the least that counts. The order of the sums depends on all lengths of the call, not on timing. */
+ * Scores, softmax statistics and sums are f32. Weights have 16 bits for a bf16 cache. For e4m3 they have 11 bits down to 2^-20 of the largest, fewer
+ * below, and below 2^-31 of it they are zero; queries are multiplied exactly where they are at least 2^-31 of the largest element of their head, with
+ * fewer bits below, and as zero below 2^-39 of it. The order of the sums depends on all lengths of the call, not on timing. */
 TF_API int64_t tf_paged_attention_workspace_bytes(int64_t seqs, int64_t queries, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int32_t cache_dtype,
                                                   int64_t max_entries);
 TF_API tf_status tf_paged_attention(const tf_paged_cache* cache, const void* q, int64_t q_stride_token, int64_t q_stride_head, int64_t seqs, int64_t queries,

@@ -289,7 +289,7 @@ class PagedCache:
 
     ``k``, ``v``  [pages, kv_heads, page_size, head_dim], bf16, or uint8 holding e4m3 codes; the last axis dense, the others at any strides (the same for
                   both), so ``empty(...)``'s order and views of [pages, page_size, kv_heads, head_dim] tensors are both fine
-    ``k_scale``, ``v_scale``  float32 [kv_heads] for e4m3 (an entry's value is code * scale; None: 1)
+    ``k_scale``, ``v_scale``  float32 [kv_heads] for e4m3 (an entry's value is code * scale; None: 1); not 0 and not below 2^-126
 
     Which pages belong to which sequence stands in the int32 [sequences, width] tables that the operators take, not here. The tensors' contents, scales included,
     may change between calls; other tensors are another cache (the operators go by the addresses that the cache was made with).
@@ -457,7 +457,10 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
     The last real query of a sequence sees all its entries, the one before all but the last, and so on; ``window`` > 0 bounds it to that many of the newest.
     ``scale`` is 1 / sqrt(head_dim) unless given. With ``return_lse`` (or ``lse``, float32 [tokens, q_heads]) returns (out, lse), lse = ln of the sum of
     exp(scale * q . k). A query that sees nothing (padding, an empty sequence) gets 0 and -inf. Entries on pages outside the cache are seen by nobody, and
-    what is not seen does not matter, infinities and NaN included."""
+    what is not seen does not matter, infinities and NaN included.
+
+    f32 arithmetic, one rounding of the result, but for softmax weights, which are multiplied with the values in 16 bits (bf16 cache) or 11 (e4m3), and queries of
+    an e4m3 cache, which are exact down to 2^-31 of their head's largest element."""
     torch = _torch()
     _check_cache(cache)
     index, dim, kv_heads = cache.index, cache.head_dim, cache.kv_heads

@@ -2,8 +2,8 @@
 //
 // The rows of one kv head (its query heads times the new tokens) read the same keys, so keys stream through once, as the 16-row operand of
 // mma.sync m16n8k16: S^T = K Q^T and O^T = V^T P^T, rows in eights. (Rows as the 16-row operand took twice the products and accumulators for the
-// eight rows that most models have.) Bound by HBM: a bf16 key and value of 128 elements are 512 bytes for 512 operations per row, while eight
-// rows use about a twentieth of the tensor cores.
+// eight rows that most models have.) Bound by HBM: a bf16 key and value of 128 elements are 512 bytes for 512 operations per row, while the products of
+// eight rows keep the tensor pipe 15 % busy.
 //
 // One pass with a running maximum and sum (base 2, f32). The workers are single warps, or teams of 2 or 4 warps with rows of their own where
 // one warp's registers do not hold them. Each has a ring of its own in shared memory, filled by cp.async, and never waits for another: while one waits for a
@@ -54,7 +54,7 @@ struct AttendCfg {
   static constexpr int kChunks = kRowBytes / 16;      // of a staged row
   static constexpr int kRowsPerCopy = 32 / kChunks;   // rows that one copy instruction of a warp covers
   static_assert(kBlocksPerSm * (kSmem + 2560) <= 228 * 1024 && kSmem <= 225 * 1024, "the grid counts on so many blocks an SM");
-  // An e4m3 entry is multiplied as f16: weights are scaled by 2^kShift, so that the largest is 2^15 and small ones keep their bits.
+  // An e4m3 entry is multiplied as f16: weights are scaled by 2^kShift, so that the largest is above 2^6 and at most 2^15, and small ones keep their bits.
   static constexpr float kSlack = 8.0f;
   static constexpr float kShift = F8 ? 15.0f - kSlack : 0.0f;
 };
@@ -403,7 +403,8 @@ __global__ void __launch_bounds__(kAttendThreads, (AttendCfg<DP, F8, ROWS>::kBlo
     for (int n = 0; n < NR; ++n) {
       row_scale[n][0] = row_scale[n][1] = p.scale_log2;
       if constexpr (F8) {
-        // bf16 -> f16 without loss: the row is scaled by a power of two that puts its largest element into [2^14, 2^15), or by 2^126 (its scores are zero to f32 then)
+        // bf16 -> f16: the row is scaled by a power of two that puts its largest element into [2^14, 2^15), or by 2^126 (its scores are zero to f32 then). Elements of
+        // at least 2^-31 of that one keep all their bits, those below 2^-39 become zero
         float top = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
