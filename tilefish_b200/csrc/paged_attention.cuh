@@ -15,9 +15,9 @@
 // workers of a block that lies inside a head), and paged_attention_join_kernel adds them up in the order of the keys.
 //
 // Measured (CUDA graph, device time): 64 sequences of up to 8192 entries, 8 kv heads of 128, eight query heads each: bf16 178 us = 6.4 TB/s of keys and values,
-// 0.98 of a copy's rate; two of 131072 109 us, 0.98; e4m3, 32 of up to 16384, 98 us, 0.92 (with 16-bit operands to make); 40 rows of 96 elements 41 us
+// 0.98 of a copy's rate; two of 131072 109 us, 0.98; e4m3, 32 of up to 16384, 97 us, 0.93 (with 16-bit operands to make); 40 rows of 96 elements 42 us
 // against 16 of HBM time, bound by products and softmax of two warps a scheduler taking turns; calls of a few microseconds by their chain of
-// loads (lengths, page, keys; parts) and two launches: one sequence of 129 entries 7.5 us.
+// loads (lengths, page, keys; parts) and two launches: one sequence of 129 entries 7.6 us.
 #pragma once
 
 #include <cmath>

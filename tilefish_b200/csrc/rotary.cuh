@@ -297,7 +297,7 @@ static tf_status launch_rotary_rows(const RotaryArgs& p, VectorPlan plan, cudaSt
 }
 
 // Two rows a thread keep the loads of a long call in flight (8192 x 64 x 128 bf16: 40.8 us with five blocks an SM, 43.2 with four; one row 42.3 to 54;
-// 1777 x 20 x 80 f32 5.05 us, one row 5.8); a call that two rows would not spread over two blocks an SM takes one (4 tokens of 10 heads 2.1 -> 2.0 us;
+// 1777 x 20 x 80 f32 5.2 us, one row 5.8); a call that two rows would not spread over two blocks an SM takes one (4 tokens of 10 heads 2.1 -> 2.0 us;
 // 64 of 80 into a cache 2.75 and 2.85: either will do). The append kernel spills at five blocks and the f32 one is slower (by a quarter).
 template <typename T, bool kAppend>
 static tf_status launch_rotary_vectors(const RotaryArgs& p, cudaStream_t stream) {
