@@ -65,3 +65,54 @@ def test_lengths_and_counts_written_directly_in_front(A, captured, seqs, longest
     torch.cuda.synchronize()
     for i, (w, g) in enumerate(zip(want, got)):
         assert torch.equal(w[0], g[0]) and torch.equal(w[1], g[1]), i
+
+
+def test_two_threads_on_streams_of_their_own(A):
+    """Rotations, appends and attention from two threads at once, in other forms each, give what they give one after the other."""
+    import threading
+
+    def work(seed):
+        seqs, longest, kv, group, dim = ((4, 1500, 2, 8, 128), (40, 200, 1, 5, 64))[seed]
+        g = torch.Generator().manual_seed(seed)
+        table = A.RotaryTable(A.rotary_frequencies(dim)[0], layout=("half", "interleaved")[seed])
+        _, cache, tables = state(A, seqs, longest, kv, group, dim, 16, seed)
+        kept = cache.k.clone(), cache.v.clone()
+        qkv = torch.randn((seqs, kv * (group + 2), dim), generator=g).bfloat16().cuda()
+        starts = torch.randint(0, longest - 30, (seqs,), generator=g).cuda()
+
+        def steps():
+            cache.k.copy_(kept[0]), cache.v.copy_(kept[1])
+            positions, got = starts.clone(), []
+            for _ in range(25):
+                q, k, v = qkv.split([kv * group, kv, kv], dim=1)
+                turned = A.cache_append(cache, k, v, tables, positions, q=q, rotary=table)
+                positions += 1
+                out = A.paged_attention(turned, cache, tables, positions.int())
+                got += [turned, out, A.rotary(out, positions, table)]
+            return got
+
+        return steps
+
+    both = [work(0), work(1)]
+    want = [f() for f in both]
+    torch.cuda.synchronize()
+    found, failed = [None, None], []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(3):
+                    found[i] = both[i]()
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for w, f in zip(want, found):
+        assert all(torch.equal(a, b) for a, b in zip(w, f, strict=True))
