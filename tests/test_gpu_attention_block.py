@@ -39,7 +39,7 @@ def test_a_refused_call_changes_nothing(A):
     bad = [("tables", good["tables"].long(), "dtype"), ("tables", good["tables"].cpu(), "device"), ("tables", good["tables"][0], "rank"), ("tables", good["tables"].t(), "contiguous"),
            ("tables", ints(0, 1, 2).view(3, 1), "shape"), ("positions", good["positions"][:3], "shape"), ("positions", good["positions"].float(), "dtype"), ("rows", ints(0, 1), "shape"),
            ("rotary", A.rotary_frequencies(DIM), "dtype"), ("rotary", A.RotaryTable(A.rotary_frequencies(128)[0]), "shape"), ("lengths", ints(2, 2).long(), "dtype"), ("lengths", ints(2), "shape"),
-           ("counts", ints(2, 2, 2), "shape"), ("counts", ints(2, 2).float(), "dtype"), ("window", -1, "argument"), ("cache", (cache.k, cache.v), "dtype"),
+           ("counts", ints(2, 2, 2), "shape"), ("counts", ints(2, 2).float(), "dtype"), ("window", -1, "argument"), ("window", 2.5, "argument"), ("cache", (cache.k, cache.v), "dtype"),
            ("cache", A.PagedCache.empty(8, 16, KV, 32), "shape"), ("x", x.float(), "dtype"), ("residual", res[:2], "shape"),
            ("w", AttentionWeights(att.w_n, att.w_qkv, other.w_o, HEADS, KV), "shape"), ("w", AttentionWeights(att.w_n, other.w_qkv, att.w_o, HEADS, KV), "shape"),
            ("w", AttentionWeights(other.w_n, att.w_qkv, att.w_o, HEADS, KV), "shape")]

@@ -16,6 +16,18 @@ def test_nothing_of_a_table_is_exchanged(name, value):
     assert (table.rot, table.layout, table.magnitude, table.index, table._layout) == (4, "half", 1.0, -1, A.LAYOUTS["half"]) and table.turns.tolist() == A._turns([1.0, 0.5])
 
 
+def test_a_subclass_has_attributes_of_its_own():
+    class Named(A.RotaryTable):
+        pass
+
+    table = Named([1.0], device="cpu")
+    table.name = "first"
+    with pytest.raises(AttributeError, match="rot"):
+        table.rot = 8
+    other = copy.deepcopy(table)
+    assert other.name == "first" and other.rot == 2
+
+
 def test_copies():
     table = A.RotaryTable([1.0, 0.5], layout="interleaved", magnitude=1.5, device="cpu")
     for other in (copy.copy(table), copy.deepcopy(table)):

@@ -176,15 +176,18 @@ class RotaryTable:
         _pre(1 <= len(values) <= 512, f"inv_freq: {len(values)} frequencies; 1 to 512 are possible", "shape", "inv_freq")
         _pre(all(abs(f) <= 2.0**32 for f in values), "inv_freq: not finite, or more than 2^32 radians", "argument", "inv_freq")
         turns = torch.tensor(_turns(values), dtype=torch.int64, device=device if device is not None else "cuda")
-        for name, value in zip(self.__slots__, (2 * len(values), layout, float(magnitude), turns, turns.get_device(), LAYOUTS[layout]), strict=True):
+        for name, value in zip(RotaryTable.__slots__, (2 * len(values), layout, float(magnitude), turns, turns.get_device(), LAYOUTS[layout]), strict=True):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value) -> None:
-        raise AttributeError(f"RotaryTable.{name} cannot be exchanged: other frequencies, layouts or magnitudes are another table")
+        if name in RotaryTable.__slots__:
+            raise AttributeError(f"RotaryTable.{name} cannot be exchanged: other frequencies, layouts or magnitudes are another table")
+        object.__setattr__(self, name, value)
 
     def __setstate__(self, state) -> None:
-        for name, value in state[1].items():
-            object.__setattr__(self, name, value)
+        for part in state:
+            for name, value in (part or {}).items():
+                object.__setattr__(self, name, value)
 
     def __repr__(self) -> str:
         return f"RotaryTable(rot={self.rot}, {self.layout}, magnitude={self.magnitude:g})"
@@ -327,11 +330,13 @@ class PagedCache:
                                       pages, page_size, kv_heads, head_dim, strides[0], strides[1], strides[2], N.CACHE_E4M3 if codes else N.CACHE_BF16, 0)
         values = (k, v, k_scale, v_scale, pages, kv_heads, page_size, head_dim, k.device, k.get_device(), desc, ctypes.addressof(desc),
                   ((_span(k), "the cache's k"), (_span(v), "the cache's v")))
-        for name, value in zip(self.__slots__, values, strict=True):
+        for name, value in zip(PagedCache.__slots__, values, strict=True):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value) -> None:
-        raise AttributeError(f"PagedCache.{name} cannot be exchanged: its tensors' contents may be changed in place, other tensors are another cache")
+        if name in PagedCache.__slots__:
+            raise AttributeError(f"PagedCache.{name} cannot be exchanged: its tensors' contents may be changed in place, other tensors are another cache")
+        object.__setattr__(self, name, value)
 
     def __reduce__(self):  # a copy is a cache over the tensors' copies
         return type(self), (self.k, self.v, self.k_scale, self.v_scale)
@@ -479,8 +484,8 @@ def paged_attention(q, cache: PagedCache, tables, lengths, *, counts=None, scale
         scale = dim**-0.5
     elif not abs(scale) <= 2.0**127:
         _pre(False, f"scale: {scale} is not a finite float32", "argument", "scale")
-    if not 0 <= window < 2**63:
-        _pre(False, f"window: {window} is negative or more than 63 bits", "argument", "window")
+    if not (isinstance(window, int) and 0 <= window < 2**63):
+        _pre(False, f"window: {window!r} is no whole number of 0 to 63 bits", "argument", "window")
     if out is None:
         out = torch.empty_strided(shape, (heads * dim, dim, 1), dtype=q.dtype, device=cache.device)
         ot, oh, op = heads * dim, dim, out.data_ptr()
@@ -595,8 +600,8 @@ def _check_block(x, w, cache, tables, positions, lengths, rotary, rows, counts, 
         _pre(False, f"x: {tokens} tokens cannot be dealt out evenly to {seqs} sequences", "divisible", "x")
     if tokens and _workspace_bytes(index, seqs, tokens // seqs, w.q_heads, w.kv_heads, dim, cache._desc.dtype, tables.shape[1] * cache.page_size) < 0:
         _pre(False, f"x: {seqs} sequences of {tokens // seqs} tokens are more than paged_attention takes", "unsupported", "x")
-    if not 0 <= window < 2**63:
-        _pre(False, f"window: {window} is negative or more than 63 bits", "argument", "window")
+    if not (isinstance(window, int) and 0 <= window < 2**63):
+        _pre(False, f"window: {window!r} is no whole number of 0 to 63 bits", "argument", "window")
 
 
 def attention_block(x, residual, w: AttentionWeights, cache: PagedCache, tables, positions, lengths, rotary: Optional[RotaryTable] = None, *, rows=None, counts=None,
