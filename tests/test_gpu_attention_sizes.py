@@ -63,9 +63,10 @@ def test_more_sequences_than_the_lanes_look_at_once(A, dtype, seqs, kv, dim):
 
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_joins_of_more_items_than_blocks(A, dtype):
-    """64 rows of a few dozen heads that several workers share: four warps to an item, and more items than the grid has blocks."""
+    """64 rows of some 80 heads that seven workers share each: four warps to an item (an eight of rows and 32 elements), and more items than 16 blocks an SM."""
     sms = torch.cuda.get_device_properties(0).multi_processor_count
-    seqs = max(2, sms * 54 // 800)
+    seqs = sms // 16 + 1
+    assert seqs * 8 * 8 * 4 > 16 * sms
     run(A, [1900 + 13 * i for i in range(seqs)], 8, 8, 8, 128, 32, dtype)
 
 
